@@ -26,6 +26,31 @@ class QMat(C.Structure):
                 ("blk_r", C.c_int), ("blk_c", C.c_int)]
 
 
+ROPE_MAX = 256                  # DSV4B_ROPE_MAX: rotated elements of a head
+KVQ_MAX_D = 576                 # DSV4B_KVQ_MAX_D: elements of a cache row
+TREE_MAX = 64                   # DSV4B_TREE_MAX: drafted tokens of a sequence
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+
+
+class RopeCfg(C.Structure):
+    """dsv4b_rope_cfg: angle per position of every pair, and the layout."""
+    _fields_ = [("freq", C.c_double * (ROPE_MAX // 2)), ("rd", C.c_int), ("layout", C.c_int)]
+
+
+class KvqC(C.Structure):
+    """dsv4b_kvq."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("n_pages", C.c_long),
+                ("page_rows", C.c_int), ("d", C.c_int), ("tail", C.c_int)]
+
+
+class LogitAdjustC(C.Structure):
+    """dsv4b_logit_adjust."""
+    _fields_ = [("hist", C.c_void_p), ("hist_stride", C.c_long), ("hist_len", C.c_void_p), ("n_prompt", C.c_void_p),
+                ("rep", C.c_void_p), ("freq", C.c_void_p), ("pres", C.c_void_p), ("bias_ids", C.c_void_p),
+                ("bias", C.c_void_p), ("bias_stride", C.c_long), ("bias_len", C.c_void_p), ("mask", C.c_void_p),
+                ("mask_stride", C.c_long)]
+
+
 def build():
     """Compile the library in-tree (nvcc cross-compiles without a GPU)."""
     subprocess.run(["make", "-C", HERE, "-j8"], check=True)
@@ -74,6 +99,13 @@ def _declare(L):
         "dsv4b_topk": ([vp, vp, i, i, i, vp], i),
         "dsv4b_sparse_attn_scratch": ([i, i, i, i], sz),
         "dsv4b_sparse_attn": ([vp, vp, vp, i, C.c_long, vp, vp, i, i, i, f, i, vp, sz, vp], i),
+        "dsv4b_rope_init": ([C.POINTER(RopeCfg), i, i, C.c_double, C.c_double, i, C.c_double, C.c_double], i),
+        "dsv4b_rope": ([vp, i, C.c_long, C.c_long, vp, i, C.c_long, C.c_long, vp, vp, i, i, i, i, i, vp], i),
+        "dsv4b_kv_write": ([vp, vp, i, C.c_long, vp, i, vp, vp, vp], i),
+        "dsv4b_kv_read": ([vp, vp, i, C.c_long, vp, i, vp], i),
+        "dsv4b_tree_attn_scratch": ([i, i, i, i, i], sz),
+        "dsv4b_tree_attn": ([vp, vp, i, C.c_long, C.c_long, vp, vp, i, vp, vp, vp, vp, i, i, i, i, f, vp, sz, vp], i),
+        "dsv4b_logits": ([vp, vp, i, C.c_long, C.c_long, vp, vp, i, i, vp], i),
         "dsv4_cuda_model_create": ([vp, vp, vp, vp, i], vp),
         "dsv4_cuda_model_begin": ([vp, vp, i], i),
         "dsv4_cuda_model_step": ([vp, vp, vp], i),
@@ -330,6 +362,258 @@ def sparse_attn_dev(o, q, kv, kv_dt, seq_kv_rows, sink, idxs, n_heads, d, topk_n
     check(lib().dsv4b_sparse_attn(ptr(o), ptr(q), ptr(kv), kv_dt, seq_kv_rows, ptr(sink), ptr(idxs),
                                   n_heads, d, topk_n, scale, batch, ptr(scratch), nbytes,
                                   stream_ptr(stream)), "dsv4b_sparse_attn")
+
+
+# ----------------------------------------- verifying a tree of drafted tokens
+#
+# These take torch CUDA tensors of one device and check them (ValueError) before
+# the C ABI does. With stream=None they run on torch's current stream of that
+# device, so they are ordered after the torch work that made their tensors.
+
+F16 = 3
+_row_dt = None
+
+
+def _dt(t, what):
+    """The row type (F32, BF16, F16) of a tensor."""
+    global _row_dt
+    if _row_dt is None:
+        import torch
+        _row_dt = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+    dt = _row_dt.get(t.dtype)
+    if dt is None:
+        raise ValueError("%s must be float32, bfloat16 or float16" % what)
+    return dt
+
+
+def _want(t, what, dev, dtype, shape):
+    """A contiguous tensor of dev with the given element type name and shape
+    (None: any); None passes through."""
+    if t is None:
+        return None
+    if t.device != dev or not t.is_cuda:
+        raise ValueError("%s must be on the device of the other tensors" % what)
+    if dtype is not None and str(t.dtype)[6:] not in dtype:
+        raise ValueError("%s must be %s" % (what, " or ".join(dtype)))
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError("%s must have shape %s" % (what, shape))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % what)
+    return t.data_ptr()
+
+
+def _enqueue(fn, what, dev, stream, *args):
+    """Call fn(*args, stream) with dev current; torch's current stream for None
+    (its default stream by the legacy handle, as NULL is the backend's own)."""
+    import torch
+    if stream is None:
+        s = torch._C._cuda_getCurrentRawStream(dev.index)
+    else:
+        if stream.device != dev:
+            raise ValueError("the stream belongs to another device than the tensors")
+        s = stream.cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, s or 1)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, s or 1)
+    if rc != 0:
+        raise RuntimeError("%s %s (rc=%d)" % (what, "refused its arguments" if rc == -1 else "could not launch", rc))
+
+
+def rope_cfg(rd, base, layout=ROPE_INTERLEAVED, factor=1.0, orig=0, beta_fast=32.0, beta_slow=1.0):
+    """Frequencies of a rotation of rd elements (dsv4b_rope_init); orig > 0
+    scales them by factor for contexts beyond orig positions."""
+    r = RopeCfg()
+    check(lib().dsv4b_rope_init(C.byref(r), int(rd), int(layout), float(base), float(factor), int(orig),
+                                float(beta_fast), float(beta_slow)), "dsv4b_rope_init")
+    return r
+
+
+def rope_dev(out, x, pos, cfg, first, inverse=False, stream=None):
+    """out = x [tokens, heads, width] with elements first .. first + cfg.rd of
+    every head rotated to pos [tokens] (int32); inverse rotates back. Any
+    strides with unit-stride heads; out may be x."""
+    dev = x.device
+    if x.dim() != 3 or out.shape != x.shape or x.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("x and out must be [tokens, heads, width] with unit-stride heads")
+    if out.device != dev or not x.is_cuda:
+        raise ValueError("x and out must be on one CUDA device")
+    n, h, w = x.shape
+    p = _want(pos, "pos", dev, ("int32",), (n,))
+
+    def strides(t):                 # torch leaves the stride of a length-1 axis free
+        sh = t.stride(1) if h > 1 else w
+        return (t.stride(0) if n > 1 else (h - 1) * sh + w), sh
+
+    ot, oh = strides(out)
+    xt, xh = strides(x)
+    _enqueue(lib().dsv4b_rope, "dsv4b_rope", dev, stream, out.data_ptr(), _dt(out, "out"), ot, oh, x.data_ptr(),
+             _dt(x, "x"), xt, xh, C.byref(cfg), p, n, h, w, int(first), 1 if inverse else 0)
+
+
+class KvCache:
+    """A paged cache of quantised rows (dsv4b_kvq) in the caller's tensors:
+    codes [pages, page_rows, d + tail] and scales [pages, page_rows], uint8.
+    page_rows is a power of two; d and tail are multiples of 64."""
+
+    def __init__(self, codes, scales, d, tail):
+        if codes.dim() != 3 or codes.shape[2] != d + tail:
+            raise ValueError("codes must be [pages, page_rows, d + tail]")
+        pages, rows = codes.shape[:2]
+        if d < 64 or d > KVQ_MAX_D or d % 64 or tail < 0 or tail > d or tail % 64:
+            raise ValueError("d must be a multiple of 64 up to %d, tail one up to d" % KVQ_MAX_D)
+        if rows < 1 or rows & (rows - 1) or pages < 1:
+            raise ValueError("page_rows must be a power of two, and there must be a page")
+        self.device = codes.device
+        self.c = KvqC(_want(codes, "codes", self.device, ("uint8",), None),
+                      _want(scales, "scales", self.device, ("uint8",), (pages, rows)), pages, rows, d, tail)
+        self.codes, self.scales, self.d, self.tail = codes, scales, d, tail
+        self.ref = C.byref(self.c)
+
+    @classmethod
+    def empty(cls, pages, page_rows, d, tail, device="cuda"):
+        """A cache of newly allocated, zeroed pages."""
+        import torch
+        return cls(torch.zeros((pages, page_rows, d + tail), dtype=torch.uint8, device=device),
+                   torch.zeros((pages, page_rows), dtype=torch.uint8, device=device), d, tail)
+
+
+def _rows(t, what, cache):
+    if t.dim() != 2 or t.shape[1] != cache.d or t.stride(1) != 1 or t.device != cache.device:
+        raise ValueError("%s must be [n, d] with unit-stride rows on the cache's device" % what)
+    return t.data_ptr(), _dt(t, what), t.stride(0) if t.shape[0] > 1 else cache.d
+
+
+def kv_write_dev(cache, rows, slots, rope=None, pos=None, stream=None):
+    """Quantise rows [n, d] into the cache's slots [n] (int64, distinct; -1
+    skips a row). With rope and pos [n] (int32) the last rope.rd elements of
+    each row are rotated first."""
+    p, dt, st = _rows(rows, "rows", cache)
+    n, dev = rows.shape[0], cache.device
+    if (rope is None) != (pos is None):
+        raise ValueError("rope and pos go together")
+    _enqueue(lib().dsv4b_kv_write, "dsv4b_kv_write", dev, stream, cache.ref, p, dt, st,
+             _want(slots, "slots", dev, ("int64",), (n,)), n, None if rope is None else C.byref(rope),
+             _want(pos, "pos", dev, ("int32",), (n,)))
+
+
+def kv_read_dev(out, cache, slots, stream=None):
+    """out [n, d] = the values of the cache's rows slots [n]; zeros for a slot
+    outside the cache."""
+    p, dt, st = _rows(out, "out", cache)
+    n, dev = out.shape[0], cache.device
+    _enqueue(lib().dsv4b_kv_read, "dsv4b_kv_read", dev, stream, cache.ref, p, dt, st,
+             _want(slots, "slots", dev, ("int64",), (n,)), n)
+
+
+def tree_mask(parents):
+    """Ancestor masks (int64, for tree_attn_dev) of drafted tokens: parents[i]
+    is the index of token i's parent among the drafted tokens (an earlier one),
+    or -1 for a child of the context. Every token attends to itself."""
+    m = []
+    for i, p in enumerate(parents):
+        if i >= TREE_MAX or not -1 <= p < i:
+            raise ValueError("at most %d tokens, each after its parent" % TREE_MAX)
+        m.append((1 << i) | (m[p] if p >= 0 else 0))
+    return np.array(m, np.uint64).view(np.int64)
+
+
+def tree_attn_scratch(n_heads, d, n_tok, batch, max_ctx):
+    """Bytes of scratch a tree_attn_dev call of these sizes needs."""
+    n = lib().dsv4b_tree_attn_scratch(int(n_heads), int(d), int(n_tok), int(batch), int(max_ctx))
+    if n == 0:
+        raise ValueError("sizes that dsv4b_tree_attn does not take")
+    return n
+
+
+def tree_attn_dev(o, q, cache, pages, ctx, n_draft, mask, sink, max_ctx, scale, scratch, stream=None):
+    """Attention of drafted tokens q [batch, tokens, heads, d] (bfloat16 or
+    float16) over the cache, into o (same type). pages [batch, max_pages],
+    ctx [batch] and n_draft [batch] (or None) are int32, mask [batch, tokens]
+    int64 (tree_mask), sink [heads] float32 or None, scratch at least
+    tree_attn_scratch() bytes that no other call uses meanwhile."""
+    dev = cache.device
+    if q.dim() != 4 or o.shape != q.shape or o.dtype != q.dtype or q.shape[3] != cache.d:
+        raise ValueError("q and o must be [batch, tokens, heads, d] of one type")
+    b, t, h, d = q.shape
+    tok = []
+    for x, what in ((o, "o"), (q, "q")):
+        s = x.stride()
+        if x.device != dev or s[3] != 1 or (h > 1 and s[2] != d):
+            raise ValueError("%s must have contiguous heads on the cache's device" % what)
+        st = s[1] if t > 1 else (s[0] if b > 1 else h * d)
+        if b > 1 and s[0] != t * st:
+            raise ValueError("%s: the tokens of all sequences must be evenly spaced" % what)
+        tok.append(st)
+    if pages.dim() != 2 or pages.shape[0] != b:
+        raise ValueError("pages must be [batch, max_pages]")
+    if scratch.device != dev or not scratch.is_contiguous():
+        raise ValueError("scratch must be contiguous, on the cache's device")
+    _enqueue(lib().dsv4b_tree_attn, "dsv4b_tree_attn", dev, stream, o.data_ptr(), q.data_ptr(), _dt(q, "q"), tok[0],
+             tok[1], cache.ref, _want(pages, "pages", dev, ("int32",), None), pages.shape[1],
+             _want(ctx, "ctx", dev, ("int32",), (b,)), _want(n_draft, "n_draft", dev, ("int32",), (b,)),
+             _want(mask, "mask", dev, ("int64",), (b, t)), _want(sink, "sink", dev, ("float32",), (h,)), h, t, b,
+             int(max_ctx), float(scale), scratch.data_ptr(), scratch.numel() * scratch.element_size())
+
+
+class LogitAdjust:
+    """What logits_dev does to each row (dsv4b_logit_adjust); the tensors are
+    kept, and may be rewritten between calls. hist [rows, n] int32 token ids
+    with hist_len and n_prompt [rows] int32; rep, freq, pres [rows] float32;
+    bias_ids int32 and bias float32 [rows, n] with bias_len [rows] int32; mask
+    [rows, words] int32, one bit per token."""
+
+    def __init__(self, hist=None, hist_len=None, n_prompt=None, rep=None, freq=None, pres=None, bias_ids=None,
+                 bias=None, bias_len=None, mask=None):
+        if hist is not None and hist.shape[-1] == 0:      # no history at all
+            hist = hist_len = n_prompt = rep = freq = pres = None
+        if bias is not None and bias.shape[-1] == 0:
+            bias = bias_ids = bias_len = None
+        given = [t for t in (hist, bias, mask) if t is not None]
+        self.rows = given[0].shape[0] if given else None
+        self.device = given[0].device if given else None
+        if (hist is None) != (hist_len is None) or (bias is None) != (bias_ids is None) or \
+                (bias is None) != (bias_len is None):
+            raise ValueError("hist goes with hist_len, bias with bias_ids and bias_len")
+        if hist is None and any(t is not None for t in (n_prompt, rep, freq, pres)):
+            raise ValueError("penalties need hist")
+        r, dev = (self.rows,), self.device
+        two = [t for t in (hist, bias_ids, bias, mask) if t is not None]
+        if any(t.dim() != 2 or t.shape[0] != self.rows for t in two):
+            raise ValueError("hist, bias_ids, bias and mask must be [rows, n]")
+        if bias is not None and bias.shape != bias_ids.shape:
+            raise ValueError("bias and bias_ids must have one shape")
+        i32, f32 = ("int32",), ("float32",)
+        self.keep = (hist, hist_len, n_prompt, rep, freq, pres, bias_ids, bias, bias_len, mask)
+        self.words = 0 if mask is None else mask.shape[1]
+        self.masked = mask is not None
+        self.c = LogitAdjustC(
+            _want(hist, "hist", dev, i32, None), 0 if hist is None else hist.shape[1],
+            _want(hist_len, "hist_len", dev, i32, r), _want(n_prompt, "n_prompt", dev, i32, r),
+            _want(rep, "rep", dev, f32, r), _want(freq, "freq", dev, f32, r), _want(pres, "pres", dev, f32, r),
+            _want(bias_ids, "bias_ids", dev, i32, None), _want(bias, "bias", dev, f32, None),
+            0 if bias is None else bias.shape[1], _want(bias_len, "bias_len", dev, i32, r),
+            _want(mask, "mask", dev, i32, None), self.words)
+        self.ref = C.byref(self.c)
+
+
+def logits_dev(out, x, token, adjust=None, stream=None):
+    """Adjusted logits of x [rows, vocab] into out (None: not wanted; may be
+    x), and the greedy tokens into token [rows] (int32, or None)."""
+    dev = x.device
+    if x.dim() != 2 or x.stride(1) != 1 or not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor [rows, vocab] with unit-stride rows")
+    r, v = x.shape
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != dev or out.stride(1) != 1):
+        raise ValueError("out must be like x")
+    if adjust is not None and adjust.rows is not None and (adjust.rows != r or adjust.device != dev):
+        raise ValueError("the adjustments are for other rows or another device")
+    xs = x.stride(0) if r > 1 else v
+    os_ = 0 if out is None else (out.stride(0) if r > 1 else v)
+    _enqueue(lib().dsv4b_logits, "dsv4b_logits", dev, stream, None if out is None else out.data_ptr(), x.data_ptr(),
+             _dt(x, "x"), os_, xs, _want(token, "token", dev, ("int32",), (r,)),
+             None if adjust is None else adjust.ref, r, v)
 
 
 # ------------------------------------------------------------- whole model

@@ -314,8 +314,9 @@ void dsv4_cuda_model_free(dsv4b_model *m);
 int dsv4b_gemv(int wdt, float *y, const float *x, const void *W, const void *S,
                int rows, int cols, int blk_r, int blk_c, int nt, void *stream);
 
-/* Element types of key / KV rows in the sparse-MLA device entries. */
-enum { DSV4B_F32 = 0, DSV4B_BF16 = 1, DSV4B_E4M3 = 2 };
+/* Element types. Key / KV rows in the sparse-MLA entries are F32, BF16 or
+ * E4M3; the tree-verification entries below take F32, BF16 or F16 rows. */
+enum { DSV4B_F32 = 0, DSV4B_BF16 = 1, DSV4B_E4M3 = 2, DSV4B_F16 = 3 };
 
 /* Indexer scores for `batch` sequences: out[b][t], t < n_pos, from
  * q[b][n_heads][head_dim], head weights w[b][n_heads] and key rows of type
@@ -353,6 +354,120 @@ int dsv4b_sparse_attn_static(float *o, const float *q, const void *kv, int kv_dt
                              long seq_kv_rows, const float *sink, const int *idxs,
                              int n_heads, int d, int topk, float scale, int batch,
                              void *stream);
+
+/* ---- verifying a tree of drafted tokens: rotary positions, a quantised
+ * paged cache, attention of the drafted tokens over it, and the logits'
+ * adjustment. No reference counterpart beyond the cited pieces (the reference
+ * drafts nothing and keeps an f32 cache). Device pointers of the current
+ * device, enqueued on `stream`; nothing is allocated, kept between calls or
+ * read back, so every entry can be captured into a graph. All of them return
+ * 0, -1 for an argument that is refused before any device work, or -2 when
+ * the launch failed. ---- */
+
+/* Rotation of rd elements (even, <= DSV4B_ROPE_MAX): pair i turns by
+ * pos * freq[i]. A pair is (2i, 2i + 1) of the rotated part (interleaved, the
+ * reference's layout, src/core/dsv4_rope.c:106-120) or (i, i + rd/2) (half).
+ * Filled by dsv4b_rope_init; a caller may scale freq itself. */
+#define DSV4B_ROPE_MAX 256
+enum { DSV4B_ROPE_INTERLEAVED = 0, DSV4B_ROPE_HALF = 1 };
+typedef struct {
+    double freq[DSV4B_ROPE_MAX / 2];
+    int rd, layout;
+} dsv4b_rope_cfg;
+
+/* freq[i] = base^(-2i / rd); with orig > 0 scaled for contexts beyond orig
+ * positions (YaRN, src/core/dsv4_rope.c:48-99): pairs that turn fewer than
+ * beta_slow times in orig positions are divided by factor, those above
+ * beta_fast are kept, a ramp in between. Host only. */
+int dsv4b_rope_init(dsv4b_rope_cfg *r, int rd, int layout, double base, double factor, int orig,
+                    double beta_fast, double beta_slow);
+
+/* out[t][h][0..width) = x[t][h][0..width) with elements first .. first + rd of
+ * every head rotated to position pos[t] (inverse != 0: rotated back, which is
+ * also the gradient). Strides in elements from token to token and head to
+ * head; out is x with the same type and strides (in place: only the rotated
+ * part is written), or does not overlap it. Any int position; angles are
+ * reduced in double. */
+int dsv4b_rope(void *out, int out_dt, long out_tok, long out_head, const void *x, int x_dt, long x_tok,
+               long x_head, const dsv4b_rope_cfg *r, const int *pos, int n_tok, int n_heads, int width,
+               int first, int inverse, void *stream);
+
+/* A paged cache of quantised rows in the caller's device memory: codes
+ * [n_pages][page_rows][d + tail] bytes (16-byte aligned), scales
+ * [n_pages][page_rows] bytes. Row = d - tail e4m3 codes, then `tail` f16
+ * values; element = code * 2^(scale byte - 127). d a multiple of 64 up to
+ * DSV4B_KVQ_MAX_D, tail a multiple of 64 (0 .. d), page_rows a power of two.
+ * A slot is page * page_rows + row. */
+#define DSV4B_KVQ_MAX_D 576
+typedef struct {
+    void *codes;
+    void *scales;
+    long n_pages;
+    int page_rows, d, tail;
+} dsv4b_kvq;
+
+/* Quantise rows[n][d] (row_stride elements apart) into the slots slots[n]:
+ * scale = the smallest power of two with max|x| <= 448 * scale, codes
+ * rounded to nearest even. With r, the last r->rd elements of row i are
+ * first rotated to pos[i]. A slot outside the cache (-1) skips its row; the
+ * slots of one call differ from each other. A row with an infinity or a NaN
+ * is stored as NaN. */
+int dsv4b_kv_write(const dsv4b_kvq *c, const void *rows, int dt, long row_stride, const long long *slots,
+                   int n, const dsv4b_rope_cfg *r, const int *pos, void *stream);
+
+/* out[n][d] = the values of the rows slots[n]; a slot outside the cache gives
+ * zeros. */
+int dsv4b_kv_read(const dsv4b_kvq *c, void *out, int dt, long row_stride, const long long *slots, int n,
+                  void *stream);
+
+/* Attention of drafted tokens over the cache: o[b][t][h][d] from
+ * q[b][t][h][d] (BF16 or F16, o of the same type; o_tok / q_tok elements from
+ * one token to the next, sequences n_tok tokens apart). Token t < n_draft[b]
+ * of sequence b attends to its sequence's cached positions 0 .. ctx[b] - 1 and
+ * to the drafted positions ctx[b] + k whose bit k is set in mask[b][t] (its
+ * ancestors, and usually itself), whose rows have been written at those
+ * positions; position j is row j % page_rows of page pages[b][j / page_rows]
+ * (a page outside the cache is skipped). Keys and values are the same rows,
+ * shared by all heads; sink[h] (may be NULL) joins the denominator only
+ * (src/core/dsv4_attn.c:60-108); with nothing to attend to the output is
+ * zero. Tokens t >= n_draft[b] are not written (n_draft NULL: n_tok each).
+ * ctx[b] is at most max_ctx, which sizes the launch; n_tok <= DSV4B_TREE_MAX.
+ * `scratch` holds dsv4b_tree_attn_scratch() bytes, 16-byte aligned, for the
+ * duration of the call: calls that may overlap need their own. */
+#define DSV4B_TREE_MAX 64
+size_t dsv4b_tree_attn_scratch(int n_heads, int d, int n_tok, int batch, int max_ctx);
+int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long q_tok, const dsv4b_kvq *c,
+                    const int *pages, int max_pages, const int *ctx, const int *n_draft,
+                    const unsigned long long *mask, const float *sink, int n_heads, int n_tok, int batch,
+                    int max_ctx, float scale, void *scratch, size_t scratch_bytes, void *stream);
+
+/* What to do to the logits of each row; a NULL array is off. hist
+ * [rows][hist_stride] holds the row's hist_len tokens, the first n_prompt of
+ * them its prompt (ids outside the vocabulary are ignored); bias / bias_ids
+ * [rows][bias_stride] its bias_len biases (of a token named twice, the sum);
+ * mask [rows][mask_stride] one bit per token, bit v % 32 of word v / 32, 1 =
+ * allowed. rep, freq and pres need hist. */
+typedef struct {
+    const int *hist;
+    long hist_stride;
+    const int *hist_len, *n_prompt;
+    const float *rep, *freq, *pres;
+    const int *bias_ids;
+    const float *bias;
+    long bias_stride;
+    const int *bias_len;
+    const unsigned *mask;
+    long mask_stride;
+} dsv4b_logit_adjust;
+
+/* out[r][v] (type dt, out_stride elements per row; NULL: not written; may be
+ * x) = x[r][v], divided by rep[r] (multiplied where not positive) if v is in
+ * the history, minus freq[r] * its count among the generated tokens, minus
+ * pres[r] if that count is not 0, plus its bias, -inf where the mask is 0.
+ * token[r] (NULL: not wanted) = the lowest index of the largest stored value,
+ * -1 when none is above -inf (every token masked). */
+int dsv4b_logits(void *out, const void *x, int dt, long out_stride, long x_stride, int *token,
+                 const dsv4b_logit_adjust *adj, int rows, int vocab, void *stream);
 
 /* The prepared MoE on device buffers x[hidden] -> out[hidden], stream-ordered. */
 int dsv4b_moe_forward(dsv4b_moe *m, float *out, const float *x, void *stream);

@@ -9,92 +9,689 @@
 // ctx[b] + k whose bit k is set in mask[b][t]. The sink counts in the
 // denominator only (src/core/dsv4_attn.c:84-92); with nothing to attend to
 // the output is zero. Tokens t >= n_draft[b] are not written.
+//
+// Every head of every drafted token reads the same rows, so T tokens of H
+// heads do 4 T H d flops per row of d + tail bytes: at H = 64 the tensor
+// cores bound the kernel from the first token on. It runs on tcgen05 with
+// the keys on the M side:
+//
+//   S^T [128 keys][rows] = V Q^T      A = V  (K-major),  B = Q  (K-major)
+//   O^T [128 dims][rows] += V^T P^T   A = V^T (M-major), B = P^T (N-major)
+//
+// rows = up to 64 (token, head) pairs. Both products read one f16 copy of the
+// 128 rows in shared memory (V^T is the same bytes, described M-major), and
+// all of O stays in TMEM: d/128 blocks of `rows` columns (the other way
+// round, with queries on the M side, O [128][512] alone would fill TMEM).
+//
+// A block takes one tile of rows and a run of 128-key tiles:
+//   4 loader warps   thread = one key: read its codes (64-byte units, three in
+//                    flight), widen e4m3 to f16 -- exact, the row scale stays
+//                    outside -- and store 64-element chunks in the 128-byte
+//                    swizzle; tail chunks are f16 already;
+//   1 MMA thread     issues both products, chunk by chunk as they arrive, and
+//                    frees chunk pairs as their part of O^T is done;
+//   8 softmax warps  thread = one key and half of the rows.
+//
+// Numbers. With s_j = 2^e_j the row scale, score = S (scale 2^e_j) in float
+// and the weight that multiplies codes is p_j 2^(e_j - E) in f16 (rounding
+// 2^-11; an output of 16 bits rounds as much again). E and the row's
+// reference M are raised only when a score passes M by 2^8 or a scale passes
+// 2^(E + 7) -- both fit f16 -- so O^T is almost never rescaled, and no tile
+// needs the exact maximum: one comparison per score and one vote per tile. q
+// is widened or scaled per row by a power of two into f16 (exact unless an
+// element is below 2^-29 of its row's largest). Sums of p, S and O are float.
 #include "common.cuh"
 #include "internal.h"
 #include "rows.cuh"
+#include "tcgen05.cuh"
 #include "tree.h"
 
 namespace dsv4b {
+namespace {
 
-constexpr int TA_W = 8;                             // heads (warps) per block
-constexpr int TA_E = DSV4B_KVQ_MAX_D / 64;          // element pairs per lane
+constexpr int TA_KEYS = 128;                        // keys of a tile (M of S^T)
+constexpr int TA_SOFT = 8, TA_LOAD = 4;             // softmax and loader warps (13 warps: 128 registers each)
+constexpr int TA_WMMA = TA_SOFT;                    // the MMA warp
+constexpr int TA_T = 32 * (TA_SOFT + 1 + TA_LOAD);
+constexpr int TA_ROWS = 64;                         // most rows of a tile (N)
+constexpr int TA_STAGES = 4, TA_PAIRS = 5;
+constexpr int TA_SLOT = TA_KEYS * 128;              // bytes of one 64-element chunk
+constexpr int TA_SMEM = 232448;                     // a block's limit
+constexpr int TA_SPLITS = 128;
+constexpr int TA_NONE = -1000;                      // scale reference before the first tile
+constexpr float TA_RAISE = 8.0f;                    // log2 of a weight that raises the reference
 
-// grid (n_tok, ceil(heads / TA_W), batch); a warp owns one head's running
-// maximum, sum and output; lane l holds elements 64 k + 2 l, 2 l + 1.
-template <int DT>
-__global__ void __launch_bounds__(TA_W * 32)
-k_tree_attn_simple(const __grid_constant__ TreeAttn a)
+struct Parts {              // one entry per (sequence, split, row)
+    float *o;               // [d] the split's own average
+    float2 *ml;             // reference (log2) and sum of its weights
+};
+
+struct Args {
+    TreeAttn a;
+    Parts part;
+    int nch, stages, page_shift, nsplit, per;       // chunks of a row; tiles of a split
+};
+
+struct Shared {             // behind the operand tiles
+    uint64_t full[TA_STAGES * TA_PAIRS], empty[TA_STAGES * TA_PAIRS], s_full[2], p_full, pv_done;
+    uint64_t rowmask[TA_ROWS];
+    float2 cm[TA_ROWS];     // score factor and reference of a row
+    float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
+    int wk[TA_SOFT];
+    uint32_t tmem;
+    int dead;
+};
+
+__device__ int g_gave_up;   // a bounded wait ran out (dsv4b_tree_attn_status)
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 2^e for an integer e, 0 below the normal range and infinity above it.
+__device__ __forceinline__ float pow2i(int e)
+{
+    return __uint_as_float(e < -126 ? 0u : e > 127 ? 0x7F800000u : (uint32_t)(e + 127) << 23);
+}
+
+// Votes among the 8 softmax warps.
+__device__ __forceinline__ bool soft_any(bool p)
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                 "barrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"((uint32_t)p) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
+
+// 64 bytes of a row.
+struct Unit {
+    uint32_t w[16];
+};
+__device__ __forceinline__ void ld64(Unit &u, const unsigned char *p)
+{
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(u.w[8 * i]), "=r"(u.w[8 * i + 1]), "=r"(u.w[8 * i + 2]), "=r"(u.w[8 * i + 3]),
+                       "=r"(u.w[8 * i + 4]), "=r"(u.w[8 * i + 5]), "=r"(u.w[8 * i + 6]), "=r"(u.w[8 * i + 7])
+                     : "l"(p + 32 * i));
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_f16(uint32_t v)
+{
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, __NV_E4M3);
+    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+
+__device__ __forceinline__ void st_smem16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// mbar_wait by a whole warp: one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(const uint64_t *bar, uint32_t parity, volatile int *dead)
+{
+    return __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(bar), parity, dead));
+}
+
+// A loader thread's place in its stream of 64-byte units: tile, chunk and, in
+// a tail chunk (128 bytes), which half.
+struct Cursor {
+    int j, c, part;
+    const unsigned char *row;       // null: a position that is not there
+};
+
+template <int NR>
+__global__ void __launch_bounds__(TA_T, 1)
+k_tree_attn(const __grid_constant__ Args g)
 {
     pdl_trigger();
     pdl_wait();
-    const int t = blockIdx.x, b = blockIdx.z, lane = threadIdx.x & 31, h = blockIdx.y * TA_W + (threadIdx.x >> 5);
+    constexpr int NC = NR / 2;                  // rows of a softmax thread
+    const TreeAttn &a = g.a;
+    extern __shared__ unsigned char ta_raw[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int split = blockIdx.x, b = blockIdx.z, H = a.n_heads, d = a.c.d, nch = g.nch, ST = g.stages;
     const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
-    if (h >= a.n_heads || t >= nd) return;
-    const int ctx = min(max(__ldcg(a.ctx + b), 0), a.max_ctx), d = a.c.d, dq = d - a.c.tail;
-    const unsigned long long mask = __ldcg(a.mask + (size_t)b * a.n_tok + t);
-    const size_t qi = ((size_t)b * a.n_tok + t) * a.q_tok + (size_t)h * d;
-    float2 q[TA_E], o[TA_E];
-#pragma unroll
-    for (int k = 0; k < TA_E; k++) {
-        const int e = 64 * k + 2 * lane;
-        q[k] = o[k] = make_float2(0.f, 0.f);
-        if (e < d) q[k] = make_float2(ld_row1<DT>(a.q, qi + e), ld_row1<DT>(a.q, qi + e + 1));
+    const int r0 = blockIdx.y * NR, R = nd * H;
+    if (r0 >= R) return;
+    const int nr = min(NR, R - r0);
+    const int ctx = min(max(__ldcg(a.ctx + b), 0), a.max_ctx), n = ctx + nd;
+    const int tb = split * g.per, nt = min((n + TA_KEYS - 1) / TA_KEYS - tb, g.per);
+    const size_t prow = ((size_t)b * g.nsplit + split) * a.n_tok * H + r0;
+    if (nt <= 0) {
+        for (int r = tid; r < nr; r += TA_T) g.part.ml[prow + r] = make_float2(-INFINITY, 0.0f);
+        return;
     }
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < ctx + nd; j++) {
-        if (j >= ctx && !((mask >> (j - ctx)) & 1)) continue;
-        const int pg = __ldcg(a.pages + (size_t)b * a.max_pages + j / a.c.page_rows);
-        if (pg < 0 || pg >= a.c.n_pages) continue;
-        const size_t slot = (size_t)pg * a.c.page_rows + j % a.c.page_rows;
-        const unsigned char *row = (const unsigned char *)a.c.codes + slot * (d + a.c.tail);
-        const float s = e8m0(__ldcg((const unsigned char *)a.c.scales + slot));
-        float2 v[TA_E];
-        float acc = 0.f;
-#pragma unroll
-        for (int k = 0; k < TA_E; k++) {
-            const int e = 64 * k + 2 * lane;
-            v[k] = make_float2(0.f, 0.f);
-            if (e < dq) v[k] = e4m3x2(__ldcg((const unsigned short *)(row + e)));
-            else if (e < d) {
-                const unsigned u = __ldcg((const unsigned *)(row + dq + 2 * (e - dq)));
-                v[k] = __half22float2(*(const __half2 *)&u);
+    const uint32_t base = (tc::smem_u32(ta_raw) + 1023u) & ~1023u;
+    const uint32_t q_s = base, p_s = q_s + nch * NR * 128, kv_s = p_s + TA_KEYS * 128;
+    Shared &sh = *reinterpret_cast<Shared *>(ta_raw + (kv_s - tc::smem_u32(ta_raw)) + ST * nch * TA_SLOT);
+    volatile int *dead = &sh.dead;
+    const int npair = (nch + 1) >> 1;
+
+    if (warp == TA_WMMA) tc::tmem_alloc(tc::smem_u32(&sh.tmem), 512);
+    if (tid == 0) {
+        for (int s = 0; s < ST; s++)
+            for (int p = 0; p < npair; p++) {
+                tc::mbar_init(tc::smem_u32(&sh.full[s * TA_PAIRS + p]), 2 * p + 1 < nch ? 2 * TA_LOAD : TA_LOAD);
+                tc::mbar_init(tc::smem_u32(&sh.empty[s * TA_PAIRS + p]), 1);
             }
-            acc += q[k].x * v[k].x + q[k].y * v[k].y;
-        }
-        const float z = warp_sum_f(acc) * s * a.scale, mn = fmaxf(m, z), f = m == -INFINITY ? 0.f : expf(m - mn);
-        const float p = expf(z - mn);
-        l = l * f + p;
-        m = mn;
+        tc::mbar_init(tc::smem_u32(&sh.s_full[0]), 1);
+        tc::mbar_init(tc::smem_u32(&sh.s_full[1]), 1);
+        tc::mbar_init(tc::smem_u32(&sh.p_full), TA_SOFT);
+        tc::mbar_init(tc::smem_u32(&sh.pv_done), 1);
+        tc::mbar_init_fence();
+        sh.dead = 0;
+    }
+    // q rows to f16, one warp a row: scaled so that the largest magnitude
+    // lies in [2^14, 2^15) (f16 rows are taken as they are)
+    for (int r = warp; r < NR; r += TA_T / 32) {
+        const int gr = r0 + r, t = gr / H;
+        const uint32_t dst = q_s + r * 128;
+        uint4 w[3];
+        uint32_t top = 0;
+        int kq = 0;
 #pragma unroll
-        for (int k = 0; k < TA_E; k++) {
-            o[k].x = o[k].x * f + p * s * v[k].x;
-            o[k].y = o[k].y * f + p * s * v[k].y;
+        for (int i = 0; i < 3; i++) {
+            const int e = i * 256 + lane * 8;
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (r < nr && e < d)
+                w[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const unsigned short *>(a.q) +
+                                                              ((size_t)b * a.n_tok + t) * a.q_tok + (size_t)(gr - t * H) * d + e));
+        }
+        if (a.dt == DSV4B_BF16) {
+            float v[3][8];
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+                Raw8<DSV4B_BF16> x;
+                x.w[0] = w[i];
+                widen8<DSV4B_BF16>(x, v[i]);
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint32_t m = __float_as_uint(v[i][k]) & 0x7FFFFFFFu;
+                    if (m < 0x7F800000u) top = max(top, m);
+                }
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (top) kq = max((int)(top >> 23) - 127 - 14, -112);
+            const float f = pow2i(-kq);
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+                w[i] = make_uint4(pack2<DSV4B_F16>(v[i][0] * f, v[i][1] * f), pack2<DSV4B_F16>(v[i][2] * f, v[i][3] * f),
+                                  pack2<DSV4B_F16>(v[i][4] * f, v[i][5] * f), pack2<DSV4B_F16>(v[i][6] * f, v[i][7] * f));
+        }
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            const int e = i * 256 + lane * 8;
+            if (e < d) st_smem16(dst + (e >> 6) * (NR * 128) + ((((e >> 3) & 7) ^ (r & 7)) << 4), w[i].x, w[i].y, w[i].z, w[i].w);
+        }
+        if (lane == 0) {
+            sh.cm[r] = make_float2(a.scale * 1.4426950408889634f * pow2i(kq), -INFINITY);
+            sh.rowmask[r] = r < nr ? __ldcg(a.mask + (size_t)b * a.n_tok + t) : 0ull;
         }
     }
-    if (a.sink && l > 0.f) l += expf(a.sink[h] - m);
-    const float inv = m == -INFINITY ? 0.f : 1.0f / l;
-    const size_t oi = ((size_t)b * a.n_tok + t) * a.o_tok + (size_t)h * d;
+    tc::fence_async_smem();
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = sh.tmem;
+    const int nblk = npair;                             // 128-element blocks of O^T
+    const uint32_t o_col = 0, s_col = nblk * NR;        // TMEM columns
+
+    if (warp > TA_WMMA) {
+        // ---------------------------------------------------------- loaders
+        const int key = (warp - TA_WMMA - 1) * 32 + lane;
+        const int ndq = (d - a.c.tail) >> 6, shift = g.page_shift, rm = a.c.page_rows - 1;
+        const int *pages = a.pages + (size_t)b * a.max_pages;
+        const size_t row_bytes = d + a.c.tail;
+        auto page_of = [&](int j) {
+            const int pos = (tb + j) * TA_KEYS + key;
+            return j < nt && pos < n ? __ldcg(pages + (pos >> shift)) : -1;
+        };
+        auto row_of = [&](int j, int pg) -> const unsigned char * {
+            const int pos = (tb + j) * TA_KEYS + key;
+            if ((unsigned)pg >= (unsigned)a.c.n_pages) return nullptr;
+            return reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (pos & rm)) * row_bytes;
+        };
+        int pg_next = page_of(0);
+        Cursor at = {0, 0, 0, row_of(0, pg_next)};
+        pg_next = page_of(1);
+        auto fetch = [&](Unit &u) {                     // the cursor's unit, then step
+            if (at.j < nt) {
+                if (at.row) ld64(u, at.row + (at.c < ndq ? at.c * 64 : ndq * 64 + (at.c - ndq) * 128 + at.part * 64));
+                else
 #pragma unroll
-    for (int k = 0; k < TA_E; k++) {
-        const int e = 64 * k + 2 * lane;
-        if (e < d) {
-            st_row1<DT>(a.o, oi + e, o[k].x * inv);
-            st_row1<DT>(a.o, oi + e + 1, o[k].y * inv);
+                    for (int i = 0; i < 16; i++) u.w[i] = 0;
+                if (at.c >= ndq && !at.part) at.part = 1;
+                else {
+                    at.part = 0;
+                    if (++at.c == nch) {
+                        at.c = 0;
+                        at.j++;
+                        at.row = row_of(at.j, pg_next);
+                        pg_next = page_of(at.j + 1);
+                    }
+                }
+            }
+        };
+        Unit u0, u1, u2;
+        fetch(u0);
+        fetch(u1);
+        fetch(u2);
+        auto shift_in = [&]() {
+            u0 = u1;
+            u1 = u2;
+            fetch(u2);
+        };
+        int s = 0, round = 0;
+        bool ok = true;
+        for (int j = 0; ok && j < nt; j++) {
+            for (int c = 0; ok && c < nch; c++) {
+                const uint32_t dst = kv_s + (s * nch + c) * TA_SLOT + key * 128;
+                const uint64_t *empty = &sh.empty[s * TA_PAIRS + (c >> 1)];
+                if (c < ndq) {
+                    uint32_t h[32];             // widened before the slot is free
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        h[2 * i] = e4m3x2_f16(u0.w[i] & 0xFFFFu);
+                        h[2 * i + 1] = e4m3x2_f16(u0.w[i] >> 16);
+                    }
+                    if (round > 0 && !(c & 1)) ok = warp_wait(empty, (round - 1) & 1, dead);
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        st_smem16(dst + ((i ^ (key & 7)) << 4), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+                } else {
+                    if (round > 0 && !(c & 1)) ok = warp_wait(empty, (round - 1) & 1, dead);
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            st_smem16(dst + (((4 * q + i) ^ (key & 7)) << 4), u0.w[4 * i], u0.w[4 * i + 1], u0.w[4 * i + 2], u0.w[4 * i + 3]);
+                        if (q == 0) shift_in();
+                    }
+                }
+                tc::fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.full[s * TA_PAIRS + (c >> 1)]));
+                shift_in();
+            }
+            if (++s == ST) s = 0, round++;
         }
+    } else if (warp == TA_WMMA) {
+        // ------------------------------------------------------- MMA issue
+        if (lane == 0) {
+            constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false), id_o = tc::idesc_f16(128, NR, true, true);
+            bool ok = true;
+            auto scores = [&](int j) {
+                const int s = j % ST;
+                for (int p = 0; ok && p < npair; p++) {
+                    ok = tc::mbar_wait(tc::smem_u32(&sh.full[s * TA_PAIRS + p]), (j / ST) & 1, dead);
+                    tc::fence_after();
+                    for (int c = 2 * p; ok && c < min(2 * p + 2, nch); c++) {
+                        const uint32_t ka = kv_s + (s * nch + c) * TA_SLOT, qa = q_s + c * NR * 128;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            tc::mma_f16(tmem + s_col + (j & 1) * NR, tc::sdesc(ka + 32 * k, 16, 1024), tc::sdesc(qa + 32 * k, 16, 1024),
+                                        id_s, c > 0 || k > 0);
+                    }
+                }
+                if (ok) tc::mma_commit(tc::smem_u32(&sh.s_full[j & 1]));
+            };
+            scores(0);
+            for (int j = 0; ok && j < nt; j++) {
+                if (ST > 1 && j + 1 < nt) scores(j + 1);
+                if (!ok) break;
+                ok = tc::mbar_wait(tc::smem_u32(&sh.p_full), j & 1, dead);
+                if (!ok) break;
+                tc::fence_after();
+                const int s = j % ST;
+                for (int p = 0; p < npair; p++) {
+                    const uint32_t va = kv_s + (s * nch + 2 * p) * TA_SLOT;
+                    // a last single chunk: its second half repeats the first,
+                    // into TMEM lanes that nothing reads
+                    const uint32_t lbo = 2 * p + 1 < nch ? TA_SLOT : 0;
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        tc::mma_f16(tmem + o_col + p * NR, tc::sdesc(va + 2048 * k, lbo, 1024), tc::sdesc(p_s + 2048 * k, 16, 1024), id_o,
+                                    j > 0 || k > 0);
+                    tc::mma_commit(tc::smem_u32(&sh.empty[s * TA_PAIRS + p]));
+                }
+                tc::mma_commit(tc::smem_u32(&sh.pv_done));
+                if (ST == 1 && j + 1 < nt) scores(j + 1);
+            }
+            if (!ok) {          // drain what was issued before TMEM is freed
+                tc::mma_commit(tc::smem_u32(&sh.s_full[0]));
+                const uint64_t t0 = tc::now_ns();
+                while (tc::now_ns() - t0 < 1000000ull) {}
+            }
+        }
+        __syncwarp();
+    } else {
+        // --------------------------------------------------------- softmax
+        const int wg = warp >> 2, key = (warp & 3) * 32 + lane, c0 = wg * NC;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const int shift = g.page_shift, rm = a.c.page_rows - 1;
+        const int *pages = a.pages + (size_t)b * a.max_pages;
+        const unsigned char *scales = reinterpret_cast<const unsigned char *>(a.c.scales);
+        auto page_of = [&](int j) {
+            const int pos = (tb + j) * TA_KEYS + key;
+            return j < nt && pos < n ? __ldcg(pages + (pos >> shift)) : -1;
+        };
+        auto scale_of = [&](int j, int pg) -> int {     // E8M0 byte of the key's row, -1: not there
+            const int pos = (tb + j) * TA_KEYS + key;
+            if ((unsigned)pg >= (unsigned)a.c.n_pages) return -1;
+            return __ldcg(scales + ((size_t)pg << shift) + (pos & rm));
+        };
+        float l[NC];
+#pragma unroll
+        for (int i = 0; i < NC; i++) l[i] = 0.0f;
+        int E = TA_NONE;
+        int kx = scale_of(0, page_of(0)), pg = page_of(1);
+        for (int j = 0; j < nt; j++) {
+            const int kx_next = scale_of(j + 1, pg);
+            pg = page_of(j + 2);
+            const bool valid = kx >= 0;
+            const int draft = (tb + j) * TA_KEYS + key - ctx;
+            const bool drafts = (tb + j + 1) * TA_KEYS > ctx;     // the tile holds drafted rows
+            // NaN rows have NaN scores and weights
+            const float ks = kx == 255 ? __int_as_float(0x7FC00000) : pow2i(kx - 127);
+            const bool ok = warp_wait(&sh.s_full[j & 1], (j >> 1) & 1, dead);
+            tc::fence_after();
+            float x[NC];
+            float over;
+            auto load = [&]() {     // exponents (log2) of the weights against the references
+#pragma unroll
+                for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + s_col + (j & 1) * NR + c0 + i, x + i);
+                tc::tmem_wait_ld(x);
+                over = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    const float2 cm = sh.cm[c0 + i];
+                    const bool see = valid && (!drafts || draft < 0 || ((sh.rowmask[c0 + i] >> draft) & 1));
+                    x[i] = see ? fmaf(x[i] * ks, cm.x, -cm.y) : -INFINITY;
+                    over = fmaxf(over, x[i]);
+                }
+            };
+            load();
+            const bool raise = over > TA_RAISE || (valid && kx < 255 && kx - E > 7);
+            if (soft_any(raise || !ok)) {
+                if (soft_any(!ok)) break;
+                // raise the references: the rows' maxima over the tile
+#pragma unroll
+                for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + s_col + (j & 1) * NR + c0 + i, x + i);
+                tc::tmem_wait_ld(x);
+                float mine = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    const bool see = valid && (!drafts || draft < 0 || ((sh.rowmask[c0 + i] >> draft) & 1));
+                    const float t = warp_max_f(see ? x[i] * ks * sh.cm[c0 + i].x : -INFINITY);
+                    if (lane == i) mine = t;
+                }
+                if (lane < NC) sh.wmax[warp & 3][c0 + lane] = mine;
+                const int kw = __reduce_max_sync(0xffffffffu, valid && kx < 255 ? kx : TA_NONE);
+                if (lane == 0) sh.wk[warp] = kw;
+                soft_sync();
+                int En = E;
+#pragma unroll
+                for (int w = 0; w < 4; w++) En = max(En, sh.wk[w]);
+                if (tid < NR) {
+                    const float mo = sh.cm[tid].y;
+                    const float mn = fmaxf(fmaxf(mo, fmaxf(sh.wmax[0][tid], sh.wmax[1][tid])), fmaxf(sh.wmax[2][tid], sh.wmax[3][tid]));
+                    const float f = mo == -INFINITY ? 0.0f : ex2(mo - mn);
+                    sh.fl[tid] = f;
+                    sh.fo[tid] = f * pow2i(E - En);
+                    sh.cm[tid].y = mn;
+                }
+                soft_sync();
+                E = En;
+#pragma unroll
+                for (int i = 0; i < NC; i++) l[i] *= sh.fl[c0 + i];
+                if (j > 0 && warp_wait(&sh.pv_done, (j - 1) & 1, dead)) {
+                    tc::fence_after();
+                    for (int p = 0; p < nblk; p++) {
+#pragma unroll
+                        for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
+                        tc::tmem_wait_ld(x);
+#pragma unroll
+                        for (int i = 0; i < NC; i++) x[i] *= sh.fo[c0 + i];
+#pragma unroll
+                        for (int i = 0; i < NC; i += 8) tc::tmem_st8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
+                    }
+                    tc::tmem_wait_st();
+                }
+                load();
+            }
+            // weights: sums in float, the f16 operand of the second product
+            const float w = valid && kx < 255 ? pow2i(kx - E) : 1.0f;
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const float e = ex2(x[i]);
+                l[i] += e;
+                x[i] = e * w;
+            }
+            if (j > 0) warp_wait(&sh.pv_done, (j - 1) & 1, dead);
+            const uint32_t dst = p_s + key * 128;
+#pragma unroll
+            for (int i = 0; i < NC; i += 8)
+                st_smem16(dst + ((((c0 + i) >> 3) ^ (key & 7)) << 4), pack2<DSV4B_F16>(x[i], x[i + 1]), pack2<DSV4B_F16>(x[i + 2], x[i + 3]),
+                          pack2<DSV4B_F16>(x[i + 4], x[i + 5]), pack2<DSV4B_F16>(x[i + 6], x[i + 7]));
+            tc::fence_async_smem();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.p_full));
+            kx = kx_next;
+        }
+        // row sums: the warp's 32 keys by halving exchanges (lane = row), then
+        // the four warps
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] = i < NC ? l[i < NC ? i : 0] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int i = 0; i < o; i++) {
+                const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+            }
+        }
+        if (lane < NC) sh.lsum[warp & 3][c0 + lane] = v[0];
+        soft_sync();
+        const bool done = warp_wait(&sh.pv_done, (nt - 1) & 1, dead);
+        tc::fence_after();
+        if (tid < NR && tid < nr) {
+            const float m = sh.cm[tid].y, sum = (sh.lsum[0][tid] + sh.lsum[1][tid]) + (sh.lsum[2][tid] + sh.lsum[3][tid]);
+            float den = sum;
+            if (g.nsplit > 1) {
+                g.part.ml[prow + tid] = make_float2(m, sum);
+            } else if (a.sink && m != -INFINITY) {
+                den += ex2(__ldcg(a.sink + (r0 + tid) % H) * 1.4426950408889634f - m);
+            }
+            sh.fo[tid] = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / den;
+        }
+        soft_sync();
+        if (done) {
+            const float s = pow2i(E - 127);
+            for (int p = 0; p < nblk; p++) {
+                const int e = p * 128 + key;
+                float x[NC];
+#pragma unroll
+                for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
+                tc::tmem_wait_ld(x);
+                if (e >= d) continue;
+#pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    const int r = c0 + i;
+                    if (r >= nr) break;
+                    const float f = sh.fo[r], y = f == 0.0f ? 0.0f : x[i] * f * s;
+                    if (g.nsplit > 1) {
+                        g.part.o[(prow + r) * d + e] = y;
+                    } else {
+                        const int t = (r0 + r) / H;
+                        const size_t o = ((size_t)b * a.n_tok + t) * a.o_tok + (size_t)(r0 + r - t * H) * d + e;
+                        if (a.dt == DSV4B_BF16) st_row1<DSV4B_BF16>(a.o, o, y);
+                        else st_row1<DSV4B_F16>(a.o, o, y);
+                    }
+                }
+            }
+        }
+        tc::fence_before();
+    }
+    __syncthreads();
+    if (warp == TA_WMMA) {
+        tc::fence_after();
+        tc::tmem_free(tmem, 512);
+    }
+    if (tid == 0 && sh.dead) g_gave_up = 1;
+}
+
+// One row per block: the splits' averages weighted by their sums, joined in
+// split order; the sink joins the denominator.
+__global__ void __launch_bounds__(128)
+k_tree_join(const __grid_constant__ Args g)
+{
+    pdl_trigger();
+    pdl_wait();
+    const TreeAttn &a = g.a;
+    __shared__ float wt[TA_SPLITS];
+    const int H = a.n_heads, r = blockIdx.x, b = blockIdx.y, t = r / H, d = a.c.d, tid = threadIdx.x, lane = tid & 31;
+    const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
+    if (t >= nd) return;
+    const size_t rows = (size_t)a.n_tok * H, p0 = (size_t)b * g.nsplit * rows + r;
+    if (tid < 32) {
+        float2 ml[TA_SPLITS / 32];
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < TA_SPLITS / 32; i++) {
+            const int s = lane + 32 * i;
+            ml[i] = s < g.nsplit ? __ldcg(g.part.ml + p0 + s * rows) : make_float2(-INFINITY, 0.0f);
+            M = fmaxf(M, ml[i].x);
+        }
+        M = warp_max_f(M);
+        float den = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TA_SPLITS / 32; i++) {
+            // a split with a sum but no reference holds a NaN row
+            ml[i].y = ml[i].x == -INFINITY && ml[i].y == 0.0f ? 0.0f : ml[i].y * ex2(ml[i].x - M);
+            den += ml[i].y;
+        }
+        den = warp_sum_f(den);
+        if (a.sink && M != -INFINITY) den += ex2(__ldcg(a.sink + (r - t * H)) * 1.4426950408889634f - M);
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+        for (int i = 0; i < TA_SPLITS / 32; i++)
+            if (lane + 32 * i < g.nsplit) wt[lane + 32 * i] = ml[i].y * inv;
+    }
+    __syncthreads();
+    const size_t o = ((size_t)b * a.n_tok + t) * a.o_tok + (size_t)(r - t * H) * d;
+    for (int e = 4 * tid; e < d; e += 512) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < g.nsplit; s++) {
+            const float w = wt[s];
+            if (w == 0.0f) continue;                    // nothing in it, or nothing of it left
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(g.part.o + (p0 + s * rows) * d + e));
+            acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
+        }
+        uint2 u;
+        if (a.dt == DSV4B_BF16) u = make_uint2(pack2<DSV4B_BF16>(acc.x, acc.y), pack2<DSV4B_BF16>(acc.z, acc.w));
+        else u = make_uint2(pack2<DSV4B_F16>(acc.x, acc.y), pack2<DSV4B_F16>(acc.z, acc.w));
+        *reinterpret_cast<uint2 *>(reinterpret_cast<unsigned short *>(a.o) + o + e) = u;
     }
 }
 
+// How a call is cut: rows of a tile, splits of the context, tiles of a split.
+struct Plan {
+    int nr, tiles, nsplit, per;
+};
+
+Plan plan(int n_heads, int d, int n_tok, int batch, int max_ctx)
+{
+    Plan best = {};
+    const long R = (long)n_heads * n_tok;
+    // Rows per tile: 64 while Q, P and a tile of rows fit in shared memory (d
+    // <= 512), else 48. Fewer where that leaves the number of tiles alone: an
+    // MMA costs max(N / 2, 32 + N / 4) cycles (its operands' shared-memory
+    // reads), a softmax N rows.
+    const int most = d <= 512 ? 64 : 48;
+    const long tiles = (R + most - 1) / most;
+    int nr = most;
+    while (nr > 16 && (R + nr - 17) / (nr - 16) == tiles) nr -= 16;
+    best.nr = nr;
+    best.tiles = (int)tiles;
+    const long units = tiles * batch;
+    const int kt = (max_ctx + n_tok + TA_KEYS - 1) / TA_KEYS;
+    // Splits: the fewest tile times on 148 SMs, a block costing about 1.5
+    // tiles beside its tiles and the join one round trip of the partial
+    // outputs through L2 (2.3 us a tile, 6500 bytes per ns).
+    double cost = 0.0;
+    for (int s = 1; s <= TA_SPLITS && s <= kt; s++) {
+        const int per = (kt + s - 1) / s;
+        if ((kt + per - 1) / per != s) continue;
+        const long waves = (units * s + 147) / 148;
+        double c = waves * (per + 1.5);
+        if (s > 1) c += 1.0 + (double)s * units * nr * d * 8 / (6500.0 * 2300.0);
+        if (s == 1 || c < cost) {
+            cost = c;
+            best.nsplit = s;
+            best.per = per;
+        }
+    }
+    return best;
+}
+
+template <int NR>
+int run(const Args &g, const Plan &p, size_t smem, cudaStream_t st)
+{
+    if (smem_optin(k_tree_attn<NR>, TA_SMEM)) return -2;
+    PdlChain chain;
+    launch(k_tree_attn<NR>, dim3(p.nsplit, p.tiles, g.a.batch), dim3(TA_T), smem, st, g);
+    if (p.nsplit > 1) launch(k_tree_join, dim3(g.a.n_tok * g.a.n_heads, g.a.batch), dim3(128), 0, st, g);
+    return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace
+
 size_t tree_attn_bytes(int n_heads, int d, int n_tok, int batch, int max_ctx)
 {
-    return 16;
+    const Plan p = plan(n_heads, d, n_tok, batch, max_ctx);
+    if (p.nsplit == 1) return 16;
+    return (size_t)batch * p.nsplit * n_tok * n_heads * ((size_t)d * 4 + sizeof(float2)) + 16;
 }
 
 int tree_attn(const TreeAttn &a, void *scratch, cudaStream_t st)
 {
-    const dim3 grid(a.n_tok, (a.n_heads + TA_W - 1) / TA_W, a.batch);
-    if (a.dt == DSV4B_BF16) launch(k_tree_attn_simple<DSV4B_BF16>, grid, dim3(TA_W * 32), 0, st, a);
-    else launch(k_tree_attn_simple<DSV4B_F16>, grid, dim3(TA_W * 32), 0, st, a);
-    return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
+    const Plan p = plan(a.n_heads, a.c.d, a.n_tok, a.batch, a.max_ctx);
+    Args g = {};
+    g.a = a;
+    g.nch = a.c.d / 64;
+    g.nsplit = p.nsplit;
+    g.per = p.per;
+    while ((1 << g.page_shift) < a.c.page_rows) g.page_shift++;
+    g.part.o = reinterpret_cast<float *>(scratch);
+    g.part.ml = reinterpret_cast<float2 *>(g.part.o + (size_t)a.batch * p.nsplit * a.n_tok * a.n_heads * a.c.d);
+    const int fixed = 1024 + g.nch * p.nr * 128 + TA_KEYS * 128 + (int)sizeof(Shared);
+    g.stages = (TA_SMEM - fixed) / (g.nch * TA_SLOT);
+    if (g.stages > TA_STAGES) g.stages = TA_STAGES;
+    size_t smem = (size_t)fixed + (size_t)g.stages * g.nch * TA_SLOT;
+    // one block per SM: each takes all of TMEM
+    if (smem < 120 * 1024) smem = 120 * 1024;
+    switch (p.nr) {
+    case 16: return run<16>(g, p, smem, st);
+    case 32: return run<32>(g, p, smem, st);
+    case 48: return run<48>(g, p, smem, st);
+    default: return run<64>(g, p, smem, st);
+    }
+}
+
+int tree_attn_status()
+{
+    int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_gave_up, sizeof v) == cudaSuccess ? (v ? 1 : 0) : -1;
 }
 
 }  // namespace dsv4b

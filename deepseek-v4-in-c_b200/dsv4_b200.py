@@ -105,6 +105,7 @@ def _declare(L):
         "dsv4b_kv_read": ([vp, vp, i, C.c_long, vp, i, vp], i),
         "dsv4b_tree_attn_scratch": ([i, i, i, i, i], sz),
         "dsv4b_tree_attn": ([vp, vp, i, C.c_long, C.c_long, vp, vp, i, vp, vp, vp, vp, i, i, i, i, f, vp, sz, vp], i),
+        "dsv4b_tree_attn_status": ([], i),
         "dsv4b_logits": ([vp, vp, i, C.c_long, C.c_long, vp, vp, i, i, vp], i),
         "dsv4_cuda_model_create": ([vp, vp, vp, vp, i], vp),
         "dsv4_cuda_model_begin": ([vp, vp, i], i),

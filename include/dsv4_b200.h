@@ -393,7 +393,7 @@ int dsv4b_rope(void *out, int out_dt, long out_tok, long out_head, const void *x
                int first, int inverse, void *stream);
 
 /* A paged cache of quantised rows in the caller's device memory: codes
- * [n_pages][page_rows][d + tail] bytes (16-byte aligned), scales
+ * [n_pages][page_rows][d + tail] bytes (32-byte aligned), scales
  * [n_pages][page_rows] bytes. Row = d - tail e4m3 codes, then `tail` f16
  * values; element = code * 2^(scale byte - 127). d a multiple of 64 up to
  * DSV4B_KVQ_MAX_D, tail a multiple of 64 (0 .. d), page_rows a power of two.
@@ -440,6 +440,12 @@ int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long q_tok, cons
                     const int *pages, int max_pages, const int *ctx, const int *n_draft,
                     const unsigned long long *mask, const float *sink, int n_heads, int n_tok, int batch,
                     int max_ctx, float scale, void *scratch, size_t scratch_bytes, void *stream);
+
+/* 0 while every dsv4b_tree_attn on the current device has run to its end; 1
+ * once one of its blocks gave up a wait inside the kernel (each is bounded by
+ * two seconds; its outputs are then not valid); -1 without a device. Waits for
+ * the device. */
+int dsv4b_tree_attn_status(void);
 
 /* What to do to the logits of each row; a NULL array is off. hist
  * [rows][hist_stride] holds the row's hist_len tokens, the first n_prompt of

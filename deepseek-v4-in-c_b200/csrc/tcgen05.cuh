@@ -26,13 +26,14 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar)
     asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// Suspends the thread up to about a millisecond.
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
 {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\t"
-                 "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+                 "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n\t"
                  "selp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
     return ok != 0;
 }
 
@@ -49,10 +50,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 {
     if (mbar_try(bar, parity)) return true;
     const uint64_t t0 = now_ns();
-    for (int i = 1;; i++) {
+    while (true) {
         if (mbar_try(bar, parity)) return true;
         if (*dead) return false;
-        if ((i & 63) == 0 && now_ns() - t0 > 2000000000ull) {
+        if (now_ns() - t0 > 2000000000ull) {
             *dead = 1;
             return false;
         }

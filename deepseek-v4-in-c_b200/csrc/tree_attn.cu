@@ -74,7 +74,7 @@ struct Args {
 
 struct Shared {             // behind the operand tiles
     uint64_t full[TA_STAGES * TA_PAIRS], empty[TA_STAGES * TA_PAIRS], s_full[2], p_full, pv_done;
-    uint64_t rowmask[TA_ROWS];
+    uint64_t rowmask[TA_ROWS], out_at[TA_ROWS];     // a row's tree mask, and its first output element
     float2 cm[TA_ROWS];     // score factor and reference of a row
     float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
     int wk[TA_SOFT];
@@ -232,6 +232,7 @@ k_tree_attn(const __grid_constant__ Args g)
         }
         if (lane == 0) {
             sh.cm[r] = make_float2(a.scale * 1.4426950408889634f * pow2i(kq), -INFINITY);
+            sh.out_at[r] = ((uint64_t)b * a.n_tok + t) * a.o_tok + (uint64_t)(gr - t * H) * d;
             sh.rowmask[r] = r < nr ? __ldcg(a.mask + (size_t)b * a.n_tok + t) : 0ull;
         }
     }
@@ -279,48 +280,55 @@ k_tree_attn(const __grid_constant__ Args g)
                 }
             }
         };
+        int s = 0, round = 0, c = 0, part = 0;          // where the next unit goes
+        bool ok = true;
+        auto put = [&](Unit &u) {                       // store a unit, refill it, step
+            const uint32_t dst = kv_s + (s * nch + c) * TA_SLOT + key * 128;
+            const uint64_t *empty = &sh.empty[s * TA_PAIRS + (c >> 1)];
+            const bool first = round > 0 && !(c & 1) && !part;
+            bool whole = true;
+            if (c < ndq) {
+                uint32_t h[32];                         // widened before the slot is free
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    h[2 * i] = e4m3x2_f16(u.w[i] & 0xFFFFu);
+                    h[2 * i + 1] = e4m3x2_f16(u.w[i] >> 16);
+                }
+                fetch(u);
+                if (first) ok = warp_wait(empty, (round - 1) & 1, dead);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    st_smem16(dst + ((i ^ (key & 7)) << 4), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+            } else {
+                if (first) ok = warp_wait(empty, (round - 1) & 1, dead);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    st_smem16(dst + (((4 * part + i) ^ (key & 7)) << 4), u.w[4 * i], u.w[4 * i + 1], u.w[4 * i + 2], u.w[4 * i + 3]);
+                fetch(u);
+                whole = part;
+                part ^= 1;
+            }
+            if (whole) {
+                tc::fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.full[s * TA_PAIRS + (c >> 1)]));
+                if (++c == nch) {
+                    c = 0;
+                    if (++s == ST) s = 0, round++;
+                }
+            }
+        };
+        // three units in flight, in registers of their own: a copy between them
+        // would wait for the load
+        const int units = nt * (2 * nch - ndq);
         Unit u0, u1, u2;
         fetch(u0);
         fetch(u1);
         fetch(u2);
-        auto shift_in = [&]() {
-            u0 = u1;
-            u1 = u2;
-            fetch(u2);
-        };
-        int s = 0, round = 0;
-        bool ok = true;
-        for (int j = 0; ok && j < nt; j++) {
-            for (int c = 0; ok && c < nch; c++) {
-                const uint32_t dst = kv_s + (s * nch + c) * TA_SLOT + key * 128;
-                const uint64_t *empty = &sh.empty[s * TA_PAIRS + (c >> 1)];
-                if (c < ndq) {
-                    uint32_t h[32];             // widened before the slot is free
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        h[2 * i] = e4m3x2_f16(u0.w[i] & 0xFFFFu);
-                        h[2 * i + 1] = e4m3x2_f16(u0.w[i] >> 16);
-                    }
-                    if (round > 0 && !(c & 1)) ok = warp_wait(empty, (round - 1) & 1, dead);
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        st_smem16(dst + ((i ^ (key & 7)) << 4), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-                } else {
-                    if (round > 0 && !(c & 1)) ok = warp_wait(empty, (round - 1) & 1, dead);
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            st_smem16(dst + (((4 * q + i) ^ (key & 7)) << 4), u0.w[4 * i], u0.w[4 * i + 1], u0.w[4 * i + 2], u0.w[4 * i + 3]);
-                        if (q == 0) shift_in();
-                    }
-                }
-                tc::fence_async_smem();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.full[s * TA_PAIRS + (c >> 1)]));
-                shift_in();
-            }
-            if (++s == ST) s = 0, round++;
+        for (int i = 0; ok && i < units; i += 3) {
+            put(u0);
+            if (ok && i + 1 < units) put(u1);
+            if (ok && i + 2 < units) put(u2);
         }
     } else if (warp == TA_WMMA) {
         // ------------------------------------------------------- MMA issue
@@ -404,35 +412,49 @@ k_tree_attn(const __grid_constant__ Args g)
             tc::fence_after();
             float x[NC];
             float over;
-            auto load = [&]() {     // exponents (log2) of the weights against the references
+            // scores times the row's factor and key's scale; hidden ones -inf
+            auto scores = [&](bool lift) {
+                __syncwarp();
 #pragma unroll
                 for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + s_col + (j & 1) * NR + c0 + i, x + i);
                 tc::tmem_wait_ld(x);
+#pragma unroll
+                for (int i = 0; i < NC; i += 2) {
+                    const float4 cm = *reinterpret_cast<const float4 *>(&sh.cm[c0 + i]);
+                    x[i] = fmaf(x[i] * ks, cm.x, lift ? -cm.y : 0.0f);
+                    x[i + 1] = fmaf(x[i + 1] * ks, cm.z, lift ? -cm.w : 0.0f);
+                }
+                if (drafts && draft >= 0) {
+#pragma unroll
+                    for (int i = 0; i < NC; i++)
+                        if (!((sh.rowmask[c0 + i] >> draft) & 1)) x[i] = -INFINITY;
+                }
+                if (!valid) {
+#pragma unroll
+                    for (int i = 0; i < NC; i++) x[i] = -INFINITY;
+                }
+            };
+            auto load = [&]() {     // exponents (log2) of the weights against the references
+                scores(true);
                 over = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < NC; i++) {
-                    const float2 cm = sh.cm[c0 + i];
-                    const bool see = valid && (!drafts || draft < 0 || ((sh.rowmask[c0 + i] >> draft) & 1));
-                    x[i] = see ? fmaf(x[i] * ks, cm.x, -cm.y) : -INFINITY;
-                    over = fmaxf(over, x[i]);
-                }
+                for (int i = 0; i < NC; i++) over = fmaxf(over, x[i]);
             };
             load();
             const bool raise = over > TA_RAISE || (valid && kx < 255 && kx - E > 7);
             if (soft_any(raise || !ok)) {
                 if (soft_any(!ok)) break;
-                // raise the references: the rows' maxima over the tile
-#pragma unroll
-                for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + s_col + (j & 1) * NR + c0 + i, x + i);
-                tc::tmem_wait_ld(x);
-                float mine = -INFINITY;
+                // raise the references: the rows' maxima over the tile, as
+                // integers of the same order (a NaN has none)
+                scores(false);
+                int mine = 0;
 #pragma unroll
                 for (int i = 0; i < NC; i++) {
-                    const bool see = valid && (!drafts || draft < 0 || ((sh.rowmask[c0 + i] >> draft) & 1));
-                    const float t = warp_max_f(see ? x[i] * ks * sh.cm[c0 + i].x : -INFINITY);
-                    if (lane == i) mine = t;
+                    const int k = __float_as_int(x[i] == x[i] ? x[i] : -INFINITY);
+                    const int top = __reduce_max_sync(0xffffffffu, k ^ ((k >> 31) & 0x7FFFFFFF));
+                    if (lane == i) mine = top ^ ((top >> 31) & 0x7FFFFFFF);
                 }
-                if (lane < NC) sh.wmax[warp & 3][c0 + lane] = mine;
+                if (lane < NC) sh.wmax[warp & 3][c0 + lane] = __int_as_float(mine);
                 const int kw = __reduce_max_sync(0xffffffffu, valid && kx < 255 ? kx : TA_NONE);
                 if (lane == 0) sh.wk[warp] = kw;
                 soft_sync();
@@ -524,19 +546,23 @@ k_tree_attn(const __grid_constant__ Args g)
                 for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
                 tc::tmem_wait_ld(x);
                 if (e >= d) continue;
+                if (g.nsplit > 1) {
+                    float *o = g.part.o + (prow + c0) * d + e;
 #pragma unroll
-                for (int i = 0; i < NC; i++) {
-                    const int r = c0 + i;
-                    if (r >= nr) break;
-                    const float f = sh.fo[r], y = f == 0.0f ? 0.0f : x[i] * f * s;
-                    if (g.nsplit > 1) {
-                        g.part.o[(prow + r) * d + e] = y;
-                    } else {
-                        const int t = (r0 + r) / H;
-                        const size_t o = ((size_t)b * a.n_tok + t) * a.o_tok + (size_t)(r0 + r - t * H) * d + e;
-                        if (a.dt == DSV4B_BF16) st_row1<DSV4B_BF16>(a.o, o, y);
-                        else st_row1<DSV4B_F16>(a.o, o, y);
-                    }
+                    for (int i = 0; i < NC; i++)
+                        if (c0 + i < nr) {
+                            const float f = sh.fo[c0 + i];
+                            o[(size_t)i * d] = f == 0.0f ? 0.0f : x[i] * f * s;
+                        }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NC; i++)
+                        if (c0 + i < nr) {
+                            const float f = sh.fo[c0 + i], y = f == 0.0f ? 0.0f : x[i] * f * s;
+                            const size_t o = sh.out_at[c0 + i] + e;
+                            if (a.dt == DSV4B_BF16) st_row1<DSV4B_BF16>(a.o, o, y);
+                            else st_row1<DSV4B_F16>(a.o, o, y);
+                        }
                 }
             }
         }

@@ -18,18 +18,29 @@
 //   S^T [128 keys][rows] = V Q^T      A = V  (K-major),  B = Q  (K-major)
 //   O^T [128 dims][rows] += V^T P^T   A = V^T (M-major), B = P^T (N-major)
 //
-// rows = up to 64 (token, head) pairs. Both products read one f16 copy of the
-// 128 rows in shared memory (V^T is the same bytes, described M-major), and
-// all of O stays in TMEM: d/128 blocks of `rows` columns (the other way
-// round, with queries on the M side, O [128][512] alone would fill TMEM).
+// rows = up to 64 (token, head) pairs. All of O stays in TMEM: d/128 blocks
+// of `rows` columns (the other way round, with queries on the M side, O
+// [128][512] alone would fill TMEM).
 //
-// A block takes one tile of rows and a run of 128-key tiles:
-//   4 loader warps   thread = one key: read its codes (64-byte units, three in
-//                    flight), widen e4m3 to f16 -- exact, the row scale stays
-//                    outside -- and store 64-element chunks in the 128-byte
-//                    swizzle; tail chunks are f16 already;
-//   1 MMA thread     issues both products, chunk by chunk as they arrive, and
-//                    frees chunk pairs as their part of O^T is done;
+// What bounds it is shared memory: an MMA with both operands there reads
+// 128 x 16 + rows x 16 f16, at 128 bytes a cycle 48 cycles for 64 rows where
+// the tensor core needs 32 (measured: 48.5; with A in TMEM 32.5). So the first
+// product takes V from TMEM, and the second -- whose A is V transposed, which
+// only a shared-memory descriptor can express -- from shared memory. The
+// TMEM copy also lets the first product run ahead of the second by more than
+// a tile while shared memory holds one tile (128 rows of 512 f16 are 128 KB),
+// which hides the softmax.
+//
+// A block takes one tile of rows and a run of 128-key tiles, cut into chunk
+// pairs of 128 elements:
+//   8 loader warps   thread = one key and every other 64-element chunk: read
+//                    its codes (64-byte units, two in flight), widen e4m3 to
+//                    f16 -- exact, the row scale stays outside -- into a TMEM
+//                    ring of 3 or 4 pairs; later, when the second product has
+//                    freed the pair's place, from there to shared memory
+//                    (128-byte swizzle; V^T is the same bytes, M-major);
+//   1 MMA warp       issues S of pair v, then O of the pair one tile and one
+//                    pair behind it;
 //   8 softmax warps  thread = one key and half of the rows.
 //
 // Numbers. With s_j = 2^e_j the row scale, score = S (scale 2^e_j) in float
@@ -50,9 +61,15 @@ namespace dsv4b {
 namespace {
 
 constexpr int TA_KEYS = 128;                        // keys of a tile (M of S^T)
-constexpr int TA_SOFT = 8, TA_LOAD = 4;             // softmax and loader warps (13 warps: 128 registers each)
-constexpr int TA_WMMA = TA_SOFT;                    // the MMA warp
-constexpr int TA_T = 32 * (TA_SOFT + 1 + TA_LOAD);
+constexpr int TA_SOFT = 8, TA_LOAD = 8;             // softmax and loader warps
+constexpr int TA_LAG = 1;                           // pairs, beyond a tile, that O runs behind S
+constexpr int TA_RING = 4;                          // most pairs of the TMEM ring
+constexpr int TA_WMMA = TA_SOFT + TA_LOAD;          // the MMA warp, in a warpgroup of its own
+constexpr int TA_T = 32 * (TA_SOFT + TA_LOAD + 4);
+// registers: 640 threads are launched with 96 each; the MMA warpgroup gives 64
+// away, 24 to each softmax and 8 to each loader warpgroup
+constexpr int TA_REG_SOFT = 120, TA_REG_LOAD = 104, TA_REG_MMA = 32;
+static_assert(2 * (TA_REG_SOFT + TA_REG_LOAD) + TA_REG_MMA <= 5 * 96, "more registers than the block is launched with");
 constexpr int TA_ROWS = 64;                         // most rows of a tile (N)
 constexpr int TA_STAGES = 4, TA_PAIRS = 5;
 constexpr int TA_SLOT = TA_KEYS * 128;              // bytes of one 64-element chunk
@@ -69,11 +86,12 @@ struct Parts {              // one entry per (sequence, split, row)
 struct Args {
     TreeAttn a;
     Parts part;
-    int nch, stages, page_shift, nsplit, per;       // chunks of a row; tiles of a split
+    int nch, stages, ring, page_shift, nsplit, per; // chunks of a row; TMEM pairs; tiles of a split
 };
 
 struct Shared {             // behind the operand tiles
-    uint64_t full[TA_STAGES * TA_PAIRS], empty[TA_STAGES * TA_PAIRS], s_full[2], p_full, pv_done;
+    uint64_t v_full[TA_STAGES * TA_PAIRS], v_empty[TA_STAGES * TA_PAIRS], k_full[TA_RING], k_done[TA_RING];
+    uint64_t s_full, s_free, p_full, pv_done;
     uint64_t rowmask[TA_ROWS], out_at[TA_ROWS];     // a row's tree mask, and its first output element
     float2 cm[TA_ROWS];     // score factor and reference of a row
     float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
@@ -82,6 +100,7 @@ struct Shared {             // behind the operand tiles
     int dead;
 };
 
+__device__ __align__(64) unsigned char g_zero_row[2 * DSV4B_KVQ_MAX_D];  // a position that is not there
 __device__ int g_gave_up;   // a bounded wait ran out (dsv4b_tree_attn_status)
 
 __device__ __forceinline__ float ex2(float x)
@@ -143,7 +162,7 @@ __device__ __forceinline__ bool warp_wait(const uint64_t *bar, uint32_t parity, 
 // a tail chunk (128 bytes), which half.
 struct Cursor {
     int j, c, part;
-    const unsigned char *row;       // null: a position that is not there
+    const unsigned char *row;
 };
 
 template <int NR>
@@ -155,7 +174,7 @@ k_tree_attn(const __grid_constant__ Args g)
     constexpr int NC = NR / 2;                  // rows of a softmax thread
     const TreeAttn &a = g.a;
     extern __shared__ unsigned char ta_raw[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int split = blockIdx.x, b = blockIdx.z, H = a.n_heads, d = a.c.d, nch = g.nch, ST = g.stages;
     const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
     const int r0 = blockIdx.y * NR, R = nd * H;
@@ -176,13 +195,18 @@ k_tree_attn(const __grid_constant__ Args g)
 
     if (warp == TA_WMMA) tc::tmem_alloc(tc::smem_u32(&sh.tmem), 512);
     if (tid == 0) {
-        for (int s = 0; s < ST; s++)
-            for (int p = 0; p < npair; p++) {
-                tc::mbar_init(tc::smem_u32(&sh.full[s * TA_PAIRS + p]), 2 * p + 1 < nch ? 2 * TA_LOAD : TA_LOAD);
-                tc::mbar_init(tc::smem_u32(&sh.empty[s * TA_PAIRS + p]), 1);
+        for (int p = 0; p < npair; p++)
+            for (int s = 0; s < ST; s++) {
+                tc::mbar_init(tc::smem_u32(&sh.v_full[s * TA_PAIRS + p]), 2 * p + 1 < nch ? TA_LOAD : TA_LOAD / 2);
+                tc::mbar_init(tc::smem_u32(&sh.v_empty[s * TA_PAIRS + p]), 1);
             }
-        tc::mbar_init(tc::smem_u32(&sh.s_full[0]), 1);
-        tc::mbar_init(tc::smem_u32(&sh.s_full[1]), 1);
+        // a pair of a single chunk has half the arrivals, so they count per chunk
+        for (int r = 0; r < g.ring; r++) {
+            tc::mbar_init(tc::smem_u32(&sh.k_full[r]), TA_LOAD);
+            tc::mbar_init(tc::smem_u32(&sh.k_done[r]), 1);
+        }
+        tc::mbar_init(tc::smem_u32(&sh.s_full), 1);
+        tc::mbar_init(tc::smem_u32(&sh.s_free), TA_SOFT);
         tc::mbar_init(tc::smem_u32(&sh.p_full), TA_SOFT);
         tc::mbar_init(tc::smem_u32(&sh.pv_done), 1);
         tc::mbar_init_fence();
@@ -242,145 +266,190 @@ k_tree_attn(const __grid_constant__ Args g)
     tc::fence_after();
     const uint32_t tmem = sh.tmem;
     const int nblk = npair;                             // 128-element blocks of O^T
-    const uint32_t o_col = 0, s_col = nblk * NR;        // TMEM columns
+    const uint32_t o_col = 0, s_col = nblk * NR, k_col = s_col + NR;    // TMEM columns
+    const int KR = g.ring;
 
-    if (warp > TA_WMMA) {
+    if (warp >= TA_SOFT && warp < TA_WMMA) {
         // ---------------------------------------------------------- loaders
-        const int key = (warp - TA_WMMA - 1) * 32 + lane;
+        tc::reg_inc<TA_REG_LOAD>();
+        const int quad = warp & 3, half = (warp - TA_SOFT) >> 2, key = quad * 32 + lane;
         const int ndq = (d - a.c.tail) >> 6, shift = g.page_shift, rm = a.c.page_rows - 1;
         const int *pages = a.pages + (size_t)b * a.max_pages;
-        const size_t row_bytes = d + a.c.tail;
+        const int row_bytes = d + a.c.tail;
         auto page_of = [&](int j) {
             const int pos = (tb + j) * TA_KEYS + key;
             return j < nt && pos < n ? __ldcg(pages + (pos >> shift)) : -1;
         };
-        auto row_of = [&](int j, int pg) -> const unsigned char * {
+        auto row_of = [&](int j, int pg) {
             const int pos = (tb + j) * TA_KEYS + key;
-            if ((unsigned)pg >= (unsigned)a.c.n_pages) return nullptr;
-            return reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (pos & rm)) * row_bytes;
+            return (unsigned)pg < (unsigned)a.c.n_pages
+                       ? reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (pos & rm)) * row_bytes
+                       : g_zero_row;
         };
         int pg_next = page_of(0);
-        Cursor at = {0, 0, 0, row_of(0, pg_next)};
+        Cursor at = {half < nch ? 0 : nt, half, 0, row_of(0, pg_next)};
         pg_next = page_of(1);
         auto fetch = [&](Unit &u) {                     // the cursor's unit, then step
-            if (at.j < nt) {
-                if (at.row) ld64(u, at.row + (at.c < ndq ? at.c * 64 : ndq * 64 + (at.c - ndq) * 128 + at.part * 64));
-                else
-#pragma unroll
-                    for (int i = 0; i < 16; i++) u.w[i] = 0;
-                if (at.c >= ndq && !at.part) at.part = 1;
-                else {
-                    at.part = 0;
-                    if (++at.c == nch) {
-                        at.c = 0;
-                        at.j++;
-                        at.row = row_of(at.j, pg_next);
-                        pg_next = page_of(at.j + 1);
-                    }
-                }
+            if (at.j >= nt) return;
+            ld64(u, at.row + (at.c < ndq ? at.c * 64 : at.c * 128 - ndq * 64 + at.part * 64));
+            if (at.c >= ndq && !at.part) {
+                at.part = 1;
+                return;
+            }
+            at.part = 0;
+            at.c += 2;
+            if (at.c >= nch) {
+                at.c = half;
+                at.j++;
+                at.row = row_of(at.j, pg_next);
+                pg_next = page_of(at.j + 1);
             }
         };
-        int s = 0, round = 0, c = 0, part = 0;          // where the next unit goes
+        const uint32_t k_mine = tmem + ((uint32_t)quad << 21) + k_col + 32 * half;
+        const int pairs = nt * npair;
         bool ok = true;
-        auto put = [&](Unit &u) {                       // store a unit, refill it, step
-            const uint32_t dst = kv_s + (s * nch + c) * TA_SLOT + key * 128;
-            const uint64_t *empty = &sh.empty[s * TA_PAIRS + (c >> 1)];
-            const bool first = round > 0 && !(c & 1) && !part;
-            bool whole = true;
-            if (c < ndq) {
-                uint32_t h[32];                         // widened before the slot is free
+        // pairs are numbered through the tiles: ku is the next one to widen
+        // into the ring, vu the next one to copy from there to shared memory
+        int ku = 0, kp = 0, kslot = 0, kround = 0, part = 0;
+        int vu = 0, vp = 0, vslot = 0, vstage = 0, vround = 0;
+        auto copy = [&]() {                             // pair vu: TMEM to shared memory
+            if (2 * vp + half < nch) {
+                if (vround > 0) ok = warp_wait(&sh.v_empty[vstage * TA_PAIRS + vp], (vround - 1) & 1, dead);
+                if (!ok) return;
+                uint32_t h[32];
+                tc::tmem_ld32(k_mine + 64 * vslot, h);
+                tc::tmem_wait_ld(h);
+                const uint32_t dst = kv_s + (vstage * nch + 2 * vp + half) * TA_SLOT + key * 128;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    st_smem16(dst + ((i ^ (key & 7)) << 4), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+                tc::fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.v_full[vstage * TA_PAIRS + vp]));
+            }
+            vu++;
+            if (++vslot == KR) vslot = 0;
+            if (++vp == npair) {
+                vp = 0;
+                if (++vstage == ST) vstage = 0, vround++;
+            }
+        };
+        auto k_step = [&]() {
+            ku++;
+            if (++kp == npair) kp = 0;
+            if (++kslot == KR) kslot = 0, kround++;
+        };
+        auto put = [&](Unit &u) {                       // widen a unit into the ring, refill it
+            const uint32_t dst = k_mine + 64 * kslot;
+            if (!part && kround > 0) {
+                ok = warp_wait(&sh.k_done[kslot], (kround - 1) & 1, dead);
+                tc::fence_after();
+                if (!ok) return;
+            }
+            if (2 * kp + half < ndq) {
+                uint32_t h[32];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     h[2 * i] = e4m3x2_f16(u.w[i] & 0xFFFFu);
                     h[2 * i + 1] = e4m3x2_f16(u.w[i] >> 16);
                 }
                 fetch(u);
-                if (first) ok = warp_wait(empty, (round - 1) & 1, dead);
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    st_smem16(dst + ((i ^ (key & 7)) << 4), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+                tc::tmem_st32(dst, h);
             } else {
-                if (first) ok = warp_wait(empty, (round - 1) & 1, dead);
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    st_smem16(dst + (((4 * part + i) ^ (key & 7)) << 4), u.w[4 * i], u.w[4 * i + 1], u.w[4 * i + 2], u.w[4 * i + 3]);
+                tc::tmem_st16(dst + 16 * part, u.w);
                 fetch(u);
-                whole = part;
                 part ^= 1;
+                if (part) return;
             }
-            if (whole) {
-                tc::fence_async_smem();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.full[s * TA_PAIRS + (c >> 1)]));
-                if (++c == nch) {
-                    c = 0;
-                    if (++s == ST) s = 0, round++;
-                }
+            tc::tmem_wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                tc::mbar_arrive(tc::smem_u32(&sh.k_full[kslot]));
+                // a single last chunk arrives for the warps that have none
+                if (2 * kp + 1 >= nch) tc::mbar_arrive(tc::smem_u32(&sh.k_full[kslot]));
             }
+            k_step();
+            if (2 * kp + half >= nch) k_step();         // the pair's chunk is another warp's
+            while (ok && vu <= ku - KR && vu < pairs) copy();
         };
-        // three units in flight, in registers of their own: a copy between them
+        // two units in flight, in registers of their own: a copy between them
         // would wait for the load
-        const int units = nt * (2 * nch - ndq);
-        Unit u0, u1, u2;
+        int units = 0;
+        for (int c = half; c < nch; c += 2) units += c < ndq ? nt : 2 * nt;
+        Unit u0, u1;
         fetch(u0);
         fetch(u1);
-        fetch(u2);
-        for (int i = 0; ok && i < units; i += 3) {
+        for (int i = 0; ok && i < units; i += 2) {
             put(u0);
             if (ok && i + 1 < units) put(u1);
-            if (ok && i + 2 < units) put(u2);
         }
-    } else if (warp == TA_WMMA) {
+        while (ok && vu < pairs) copy();
+    } else if (warp >= TA_WMMA) {
         // ------------------------------------------------------- MMA issue
-        if (lane == 0) {
-            constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false), id_o = tc::idesc_f16(128, NR, true, true);
-            bool ok = true;
-            auto scores = [&](int j) {
-                const int s = j % ST;
-                for (int p = 0; ok && p < npair; p++) {
-                    ok = tc::mbar_wait(tc::smem_u32(&sh.full[s * TA_PAIRS + p]), (j / ST) & 1, dead);
-                    tc::fence_after();
-                    for (int c = 2 * p; ok && c < min(2 * p + 2, nch); c++) {
-                        const uint32_t ka = kv_s + (s * nch + c) * TA_SLOT, qa = q_s + c * NR * 128;
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tc::mma_f16(tmem + s_col + (j & 1) * NR, tc::sdesc(ka + 32 * k, 16, 1024), tc::sdesc(qa + 32 * k, 16, 1024),
-                                        id_s, c > 0 || k > 0);
-                    }
-                }
-                if (ok) tc::mma_commit(tc::smem_u32(&sh.s_full[j & 1]));
-            };
-            scores(0);
-            for (int j = 0; ok && j < nt; j++) {
-                if (ST > 1 && j + 1 < nt) scores(j + 1);
-                if (!ok) break;
-                ok = tc::mbar_wait(tc::smem_u32(&sh.p_full), j & 1, dead);
+        tc::reg_dec<TA_REG_MMA>();
+        if (warp == TA_WMMA) {
+        constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false), id_o = tc::idesc_f16(128, NR, true, true);
+        const int pairs = nt * npair;
+        const uint64_t q_d = tc::sdesc(q_s, 16, 1024), p_d = tc::sdesc(p_s, 16, 1024);
+        // a last single chunk: its second half repeats the first, into TMEM
+        // lanes that nothing reads
+        const uint64_t v_d2 = tc::sdesc(kv_s, TA_SLOT, 1024), v_d1 = tc::sdesc(kv_s, 0, 1024);
+        bool ok = true;
+        int p = 0, j = 0, slot = 0, round = 0;                      // of S
+        int op = 0, oj = 0, stage = 0, oround = 0;                  // of O
+        for (int v = 0; v < pairs + npair + TA_LAG; v++) {
+            if (v < pairs) {
+                if (p == 0 && j > 0) ok = warp_wait(&sh.s_free, (j - 1) & 1, dead);
+                if (ok) ok = warp_wait(&sh.k_full[slot], round & 1, dead);
                 if (!ok) break;
                 tc::fence_after();
-                const int s = j % ST;
-                for (int p = 0; p < npair; p++) {
-                    const uint32_t va = kv_s + (s * nch + 2 * p) * TA_SLOT;
-                    // a last single chunk: its second half repeats the first,
-                    // into TMEM lanes that nothing reads
-                    const uint32_t lbo = 2 * p + 1 < nch ? TA_SLOT : 0;
+                if (tc::elect_one()) {
+                    const uint32_t ka = tmem + k_col + 64 * slot;
+                    const uint64_t qb = q_d + (uint64_t)(2 * p * NR * 8);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tc::mma_f16_ta(tmem + s_col, ka + 8 * k, qb + 2 * k, id_s, p > 0 || k > 0);
+                    if (2 * p + 1 < nch) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) tc::mma_f16_ta(tmem + s_col, ka + 32 + 8 * k, qb + NR * 8 + 2 * k, id_s, true);
+                    }
+                    tc::mma_commit(tc::smem_u32(&sh.k_done[slot]));
+                    if (p == npair - 1) tc::mma_commit(tc::smem_u32(&sh.s_full));
+                }
+                __syncwarp();
+                if (++slot == KR) slot = 0, round++;
+                if (++p == npair) p = 0, j++;
+            }
+            if (v >= npair + TA_LAG) {
+                if (op == 0) ok = warp_wait(&sh.p_full, oj & 1, dead);
+                if (ok) ok = warp_wait(&sh.v_full[stage * TA_PAIRS + op], oround & 1, dead);
+                if (!ok) break;
+                tc::fence_after();
+                if (tc::elect_one()) {
+                    const uint64_t va = (2 * op + 1 < nch ? v_d2 : v_d1) + (uint64_t)((stage * nch + 2 * op) * (TA_SLOT >> 4));
 #pragma unroll
                     for (int k = 0; k < 8; k++)
-                        tc::mma_f16(tmem + o_col + p * NR, tc::sdesc(va + 2048 * k, lbo, 1024), tc::sdesc(p_s + 2048 * k, 16, 1024), id_o,
-                                    j > 0 || k > 0);
-                    tc::mma_commit(tc::smem_u32(&sh.empty[s * TA_PAIRS + p]));
+                        tc::mma_f16(tmem + o_col + op * NR, va + 128 * k, p_d + 128 * k, id_o, oj > 0 || k > 0);
+                    tc::mma_commit(tc::smem_u32(&sh.v_empty[stage * TA_PAIRS + op]));
+                    if (op == npair - 1) tc::mma_commit(tc::smem_u32(&sh.pv_done));
                 }
-                tc::mma_commit(tc::smem_u32(&sh.pv_done));
-                if (ST == 1 && j + 1 < nt) scores(j + 1);
-            }
-            if (!ok) {          // drain what was issued before TMEM is freed
-                tc::mma_commit(tc::smem_u32(&sh.s_full[0]));
-                const uint64_t t0 = tc::now_ns();
-                while (tc::now_ns() - t0 < 1000000ull) {}
+                __syncwarp();
+                if (++op == npair) {
+                    op = 0;
+                    oj++;
+                    if (++stage == ST) stage = 0, oround++;
+                }
             }
         }
+        if (!ok) {              // let what was issued finish before TMEM is freed
+            const uint64_t t0 = tc::now_ns();
+            while (tc::now_ns() - t0 < 1000000ull) {}
+        }
         __syncwarp();
+        }
     } else {
         // --------------------------------------------------------- softmax
+        tc::reg_inc<TA_REG_SOFT>();
         const int wg = warp >> 2, key = (warp & 3) * 32 + lane, c0 = wg * NC;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const int shift = g.page_shift, rm = a.c.page_rows - 1;
@@ -408,7 +477,7 @@ k_tree_attn(const __grid_constant__ Args g)
             const bool drafts = (tb + j + 1) * TA_KEYS > ctx;     // the tile holds drafted rows
             // NaN rows have NaN scores and weights
             const float ks = kx == 255 ? __int_as_float(0x7FC00000) : pow2i(kx - 127);
-            const bool ok = warp_wait(&sh.s_full[j & 1], (j >> 1) & 1, dead);
+            const bool ok = warp_wait(&sh.s_full, j & 1, dead);
             tc::fence_after();
             float x[NC];
             float over;
@@ -416,7 +485,7 @@ k_tree_attn(const __grid_constant__ Args g)
             auto scores = [&](bool lift) {
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + s_col + (j & 1) * NR + c0 + i, x + i);
+                for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + s_col + c0 + i, x + i);
                 tc::tmem_wait_ld(x);
 #pragma unroll
                 for (int i = 0; i < NC; i += 2) {
@@ -440,6 +509,13 @@ k_tree_attn(const __grid_constant__ Args g)
 #pragma unroll
                 for (int i = 0; i < NC; i++) over = fmaxf(over, x[i]);
             };
+            // S is in registers: its columns are free. Before any wait for the
+            // second product, which the MMA warp issues behind the next S.
+            auto free_s = [&]() {
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.s_free));
+            };
             load();
             const bool raise = over > TA_RAISE || (valid && kx < 255 && kx - E > 7);
             if (soft_any(raise || !ok)) {
@@ -447,6 +523,7 @@ k_tree_attn(const __grid_constant__ Args g)
                 // raise the references: the rows' maxima over the tile, as
                 // integers of the same order (a NaN has none)
                 scores(false);
+                free_s();
                 int mine = 0;
 #pragma unroll
                 for (int i = 0; i < NC; i++) {
@@ -475,18 +552,22 @@ k_tree_attn(const __grid_constant__ Args g)
                 for (int i = 0; i < NC; i++) l[i] *= sh.fl[c0 + i];
                 if (j > 0 && warp_wait(&sh.pv_done, (j - 1) & 1, dead)) {
                     tc::fence_after();
-                    for (int p = 0; p < nblk; p++) {
+                    for (int p = 0; p < nblk; p++)
 #pragma unroll
-                        for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
-                        tc::tmem_wait_ld(x);
+                        for (int i = 0; i < NC; i += 8) {
+                            float y[8];
+                            tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, y);
+                            tc::tmem_wait_ld(y);
 #pragma unroll
-                        for (int i = 0; i < NC; i++) x[i] *= sh.fo[c0 + i];
-#pragma unroll
-                        for (int i = 0; i < NC; i += 8) tc::tmem_st8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
-                    }
+                            for (int k = 0; k < 8; k++) y[k] *= sh.fo[c0 + i + k];
+                            tc::tmem_st8(tmem + lanes + o_col + p * NR + c0 + i, y);
+                        }
                     tc::tmem_wait_st();
                 }
-                load();
+#pragma unroll
+                for (int i = 0; i < NC; i++) x[i] = x[i] == -INFINITY ? x[i] : x[i] - sh.cm[c0 + i].y;
+            } else {
+                free_s();
             }
             // weights: sums in float, the f16 operand of the second product
             const float w = valid && kx < 255 ? pow2i(kx - E) : 1.0f;
@@ -703,6 +784,9 @@ int tree_attn(const TreeAttn &a, void *scratch, cudaStream_t st)
     const int fixed = 1024 + g.nch * p.nr * 128 + TA_KEYS * 128 + (int)sizeof(Shared);
     g.stages = (TA_SMEM - fixed) / (g.nch * TA_SLOT);
     if (g.stages > TA_STAGES) g.stages = TA_STAGES;
+    // at least 3 pairs: d <= 512 has 4 blocks of up to 64 columns, else 5 of 48
+    g.ring = (512 - ((g.nch + 1) / 2 + 1) * p.nr) / 64;
+    if (g.ring > TA_RING) g.ring = TA_RING;
     size_t smem = (size_t)fixed + (size_t)g.stages * g.nch * TA_SLOT;
     // one block per SM: each takes all of TMEM
     if (smem < 120 * 1024) smem = 120 * 1024;

@@ -33,12 +33,13 @@
 //
 // A block takes one tile of rows and a run of 128-key tiles, cut into chunk
 // pairs of 128 elements:
-//   8 loader warps   thread = one key and every other 64-element chunk: read
-//                    its codes (64-byte units, two in flight), widen e4m3 to
-//                    f16 -- exact, the row scale stays outside -- into a TMEM
-//                    ring of 3 or 4 pairs; later, when the second product has
-//                    freed the pair's place, from there to shared memory
-//                    (128-byte swizzle; V^T is the same bytes, M-major);
+//   8 widening warps thread = one key and every other 64-element chunk: read
+//                    its codes (64 bytes, two chunks in flight), widen e4m3
+//                    to f16 -- exact, the row scale stays outside -- into a
+//                    TMEM ring of 3 or 4 pairs;
+//   8 copying warps  from there to shared memory once the second product has
+//                    freed the pair's place (128-byte swizzle; V^T is the
+//                    same bytes, M-major);
 //   1 MMA warp       issues S of pair v, then O of the pair one tile and one
 //                    pair behind it;
 //   8 softmax warps  thread = one key and half of the rows.
@@ -61,15 +62,15 @@ namespace dsv4b {
 namespace {
 
 constexpr int TA_KEYS = 128;                        // keys of a tile (M of S^T)
-constexpr int TA_SOFT = 8, TA_LOAD = 8;             // softmax and loader warps
+constexpr int TA_SOFT = 8, TA_LOAD = 8, TA_COPY = 8;    // softmax, widening and copying warps
 constexpr int TA_LAG = 1;                           // pairs, beyond a tile, that O runs behind S
 constexpr int TA_RING = 4;                          // most pairs of the TMEM ring
-constexpr int TA_WMMA = TA_SOFT + TA_LOAD;          // the MMA warp, in a warpgroup of its own
-constexpr int TA_T = 32 * (TA_SOFT + TA_LOAD + 4);
-// registers: 640 threads are launched with 96 each; the MMA warpgroup gives 64
-// away, 24 to each softmax and 8 to each loader warpgroup
-constexpr int TA_REG_SOFT = 120, TA_REG_LOAD = 104, TA_REG_MMA = 32;
-static_assert(2 * (TA_REG_SOFT + TA_REG_LOAD) + TA_REG_MMA <= 5 * 96, "more registers than the block is launched with");
+constexpr int TA_WCOPY = TA_SOFT + TA_LOAD, TA_WMMA = TA_WCOPY + TA_COPY;   // the MMA warp, in a warpgroup of its own
+constexpr int TA_T = 32 * (TA_WMMA + 4);
+// registers: 896 threads are launched with 72 each; the other warpgroups give
+// theirs to the softmax ones
+constexpr int TA_REG_SOFT = 128, TA_REG_LOAD = 64, TA_REG_COPY = 48, TA_REG_MMA = 24;
+static_assert(2 * (TA_REG_SOFT + TA_REG_LOAD + TA_REG_COPY) + TA_REG_MMA <= 7 * 72, "more registers than the block is launched with");
 constexpr int TA_ROWS = 64;                         // most rows of a tile (N)
 constexpr int TA_STAGES = 4, TA_PAIRS = 5;
 constexpr int TA_SLOT = TA_KEYS * 128;              // bytes of one 64-element chunk
@@ -130,15 +131,16 @@ __device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 1, 
 // 64 bytes of a row.
 struct Unit {
     uint32_t w[16];
+    const unsigned char *src;
 };
-__device__ __forceinline__ void ld64(Unit &u, const unsigned char *p)
+__device__ __forceinline__ void ld64(Unit &u)
 {
 #pragma unroll
     for (int i = 0; i < 2; i++)
         asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(u.w[8 * i]), "=r"(u.w[8 * i + 1]), "=r"(u.w[8 * i + 2]), "=r"(u.w[8 * i + 3]),
                        "=r"(u.w[8 * i + 4]), "=r"(u.w[8 * i + 5]), "=r"(u.w[8 * i + 6]), "=r"(u.w[8 * i + 7])
-                     : "l"(p + 32 * i));
+                     : "l"(u.src + 32 * i));
 }
 
 __device__ __forceinline__ uint32_t e4m3x2_f16(uint32_t v)
@@ -152,18 +154,17 @@ __device__ __forceinline__ void st_smem16(uint32_t a, uint32_t x, uint32_t y, ui
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// mbar_wait by a whole warp: one answer for all lanes.
-__device__ __forceinline__ bool warp_wait(const uint64_t *bar, uint32_t parity, volatile int *dead)
+// mbar_wait by a whole warp.
+__device__ __forceinline__ void warp_wait(const uint64_t *bar, uint32_t parity, volatile int *dead)
 {
-    return __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(bar), parity, dead));
+    tc::mbar_wait(tc::smem_u32(bar), parity, dead);
+    __syncwarp();
 }
-
-// A loader thread's place in its stream of 64-byte units: tile, chunk and, in
-// a tail chunk (128 bytes), which half.
-struct Cursor {
-    int j, c, part;
-    const unsigned char *row;
-};
+__device__ __forceinline__ void warp_arrive(const uint64_t *bar, int lane)
+{
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(tc::smem_u32(bar));
+}
 
 template <int NR>
 __global__ void __launch_bounds__(TA_T, 1)
@@ -197,13 +198,12 @@ k_tree_attn(const __grid_constant__ Args g)
     if (tid == 0) {
         for (int p = 0; p < npair; p++)
             for (int s = 0; s < ST; s++) {
-                tc::mbar_init(tc::smem_u32(&sh.v_full[s * TA_PAIRS + p]), 2 * p + 1 < nch ? TA_LOAD : TA_LOAD / 2);
+                tc::mbar_init(tc::smem_u32(&sh.v_full[s * TA_PAIRS + p]), TA_COPY);
                 tc::mbar_init(tc::smem_u32(&sh.v_empty[s * TA_PAIRS + p]), 1);
             }
-        // a pair of a single chunk has half the arrivals, so they count per chunk
         for (int r = 0; r < g.ring; r++) {
             tc::mbar_init(tc::smem_u32(&sh.k_full[r]), TA_LOAD);
-            tc::mbar_init(tc::smem_u32(&sh.k_done[r]), 1);
+            tc::mbar_init(tc::smem_u32(&sh.k_done[r]), 1 + TA_COPY);
         }
         tc::mbar_init(tc::smem_u32(&sh.s_full), 1);
         tc::mbar_init(tc::smem_u32(&sh.s_free), TA_SOFT);
@@ -269,183 +269,190 @@ k_tree_attn(const __grid_constant__ Args g)
     const uint32_t o_col = 0, s_col = nblk * NR, k_col = s_col + NR;    // TMEM columns
     const int KR = g.ring;
 
-    if (warp >= TA_SOFT && warp < TA_WMMA) {
-        // ---------------------------------------------------------- loaders
-        tc::reg_inc<TA_REG_LOAD>();
+    if (warp >= TA_SOFT && warp < TA_WCOPY) {
+        // --------------------------------------------------------- widening
+        tc::reg_dec<TA_REG_LOAD>();
         const int quad = warp & 3, half = (warp - TA_SOFT) >> 2, key = quad * 32 + lane;
         const int ndq = (d - a.c.tail) >> 6, shift = g.page_shift, rm = a.c.page_rows - 1;
         const int *pages = a.pages + (size_t)b * a.max_pages;
         const int row_bytes = d + a.c.tail;
-        auto page_of = [&](int j) {
-            const int pos = (tb + j) * TA_KEYS + key;
-            return j < nt && pos < n ? __ldcg(pages + (pos >> shift)) : -1;
+        int pos = tb * TA_KEYS + key;                   // of the next row to look up
+        auto page_at = [&](int q) { return q < n ? __ldcg(pages + (q >> shift)) : -1; };
+        int pg = page_at(pos);
+        const unsigned char *row;
+        auto next_row = [&]() {
+            row = (unsigned)pg < (unsigned)a.c.n_pages
+                      ? reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (pos & rm)) * row_bytes
+                      : g_zero_row;
+            pos += TA_KEYS;
+            pg = page_at(pos);
         };
-        auto row_of = [&](int j, int pg) {
-            const int pos = (tb + j) * TA_KEYS + key;
-            return (unsigned)pg < (unsigned)a.c.n_pages
-                       ? reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (pos & rm)) * row_bytes
-                       : g_zero_row;
-        };
-        int pg_next = page_of(0);
-        Cursor at = {half < nch ? 0 : nt, half, 0, row_of(0, pg_next)};
-        pg_next = page_of(1);
-        auto fetch = [&](Unit &u) {                     // the cursor's unit, then step
-            if (at.j >= nt) return;
-            ld64(u, at.row + (at.c < ndq ? at.c * 64 : at.c * 128 - ndq * 64 + at.part * 64));
-            if (at.c >= ndq && !at.part) {
-                at.part = 1;
-                return;
-            }
-            at.part = 0;
-            at.c += 2;
-            if (at.c >= nch) {
-                at.c = half;
-                at.j++;
-                at.row = row_of(at.j, pg_next);
-                pg_next = page_of(at.j + 1);
+        next_row();
+        int fc = half, left = half < nch ? nt : 0;      // chunk to fetch; tiles left
+        auto fetch = [&](Unit &u) {
+            if (left == 0) return;
+            u.src = row + (fc < ndq ? fc * 64 : fc * 128 - ndq * 64);
+            ld64(u);
+            fc += 2;
+            if (fc >= nch) {
+                fc = half;
+                left--;
+                next_row();
             }
         };
         const uint32_t k_mine = tmem + ((uint32_t)quad << 21) + k_col + 32 * half;
         const int pairs = nt * npair;
-        bool ok = true;
-        // pairs are numbered through the tiles: ku is the next one to widen
-        // into the ring, vu the next one to copy from there to shared memory
-        int ku = 0, kp = 0, kslot = 0, kround = 0, part = 0;
-        int vu = 0, vp = 0, vslot = 0, vstage = 0, vround = 0;
-        auto copy = [&]() {                             // pair vu: TMEM to shared memory
-            if (2 * vp + half < nch) {
-                if (vround > 0) ok = warp_wait(&sh.v_empty[vstage * TA_PAIRS + vp], (vround - 1) & 1, dead);
-                if (!ok) return;
-                uint32_t h[32];
-                tc::tmem_ld32(k_mine + 64 * vslot, h);
-                tc::tmem_wait_ld(h);
-                const uint32_t dst = kv_s + (vstage * nch + 2 * vp + half) * TA_SLOT + key * 128;
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    st_smem16(dst + ((i ^ (key & 7)) << 4), h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-                tc::fence_async_smem();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.v_full[vstage * TA_PAIRS + vp]));
-            }
-            vu++;
-            if (++vslot == KR) vslot = 0;
-            if (++vp == npair) {
-                vp = 0;
-                if (++vstage == ST) vstage = 0, vround++;
-            }
+        int i = 0, c = half, slot = 0, par = 1;         // pair, chunk, ring place, parity of its last use
+        auto open = [&]() {
+            if (i >= KR) warp_wait(&sh.k_done[slot], par, dead);
+            tc::fence_after();
         };
-        auto k_step = [&]() {
-            ku++;
-            if (++kp == npair) kp = 0;
-            if (++kslot == KR) kslot = 0, kround++;
+        auto close = [&]() {
+            warp_arrive(&sh.k_full[slot], lane);
+            i++;
+            c += 2;
+            if (c >= 2 * npair) c = half;
+            if (++slot == KR) slot = 0, par ^= 1;
         };
-        auto put = [&](Unit &u) {                       // widen a unit into the ring, refill it
-            const uint32_t dst = k_mine + 64 * kslot;
-            if (!part && kround > 0) {
-                ok = warp_wait(&sh.k_done[kslot], (kround - 1) & 1, dead);
-                tc::fence_after();
-                if (!ok) return;
-            }
-            if (2 * kp + half < ndq) {
-                uint32_t h[32];
+        auto put = [&](Unit &u) {
+            const uint32_t dst = k_mine + 64 * slot;
+            if (c < ndq) {
+                open();
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    h[2 * i] = e4m3x2_f16(u.w[i] & 0xFFFFu);
-                    h[2 * i + 1] = e4m3x2_f16(u.w[i] >> 16);
+                for (int s = 0; s < 2; s++) {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        h[2 * k] = e4m3x2_f16(u.w[8 * s + k] & 0xFFFFu);
+                        h[2 * k + 1] = e4m3x2_f16(u.w[8 * s + k] >> 16);
+                    }
+                    tc::tmem_st16(dst + 16 * s, h);
                 }
-                fetch(u);
-                tc::tmem_st32(dst, h);
             } else {
-                tc::tmem_st16(dst + 16 * part, u.w);
-                fetch(u);
-                part ^= 1;
-                if (part) return;
+                Unit t;
+                t.src = u.src + 64;
+                ld64(t);
+                open();
+                tc::tmem_st16(dst, u.w);
+                tc::tmem_st16(dst + 16, t.w);
             }
+            fetch(u);
             tc::tmem_wait_st();
             tc::fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                tc::mbar_arrive(tc::smem_u32(&sh.k_full[kslot]));
-                // a single last chunk arrives for the warps that have none
-                if (2 * kp + 1 >= nch) tc::mbar_arrive(tc::smem_u32(&sh.k_full[kslot]));
+            close();
+            if (c >= nch && i < pairs) {                // a pair without a chunk for this warp
+                open();
+                close();
             }
-            k_step();
-            if (2 * kp + half >= nch) k_step();         // the pair's chunk is another warp's
-            while (ok && vu <= ku - KR && vu < pairs) copy();
         };
-        // two units in flight, in registers of their own: a copy between them
+        // two chunks in flight, in registers of their own: a copy between them
         // would wait for the load
-        int units = 0;
-        for (int c = half; c < nch; c += 2) units += c < ndq ? nt : 2 * nt;
         Unit u0, u1;
         fetch(u0);
         fetch(u1);
-        for (int i = 0; ok && i < units; i += 2) {
-            put(u0);
-            if (ok && i + 1 < units) put(u1);
+        if (half < nch) {
+            while (i < pairs) {
+                put(u0);
+                if (i < pairs) put(u1);
+            }
+        } else {
+            while (i < pairs) {
+                open();
+                close();
+            }
         }
-        while (ok && vu < pairs) copy();
+    } else if (warp >= TA_WCOPY && warp < TA_WMMA) {
+        // ---------------------------------------------------------- copying
+        tc::reg_dec<TA_REG_COPY>();
+        const int quad = warp & 3, half = (warp - TA_WCOPY) >> 2, key = quad * 32 + lane;
+        const uint32_t k_mine = tmem + ((uint32_t)quad << 21) + k_col + 32 * half, sw = key & 7;
+        const int pairs = nt * npair;
+        int p = 0, slot = 0, kpar = 0, stage = 0, vpar = 1;
+        for (int i = 0; i < pairs; i++) {
+            const int c = 2 * p + half;
+            warp_wait(&sh.k_full[slot], kpar, dead);
+            if (i >= ST * npair) warp_wait(&sh.v_empty[stage * TA_PAIRS + p], vpar, dead);
+            tc::fence_after();
+            if (c < nch) {
+                const uint32_t dst = kv_s + (stage * nch + c) * TA_SLOT + key * 128;
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint32_t h[16];
+                    tc::tmem_ld16(k_mine + 64 * slot + 16 * s, h);
+                    tc::tmem_wait_ld(h);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        st_smem16(dst + (((4 * s + k) ^ sw) << 4), h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+                }
+                tc::fence_before();
+                tc::fence_async_smem();
+            }
+            warp_arrive(&sh.k_done[slot], lane);
+            warp_arrive(&sh.v_full[stage * TA_PAIRS + p], lane);
+            if (++slot == KR) slot = 0, kpar ^= 1;
+            if (++p == npair) {
+                p = 0;
+                if (++stage == ST) stage = 0, vpar ^= 1;
+            }
+        }
     } else if (warp >= TA_WMMA) {
         // ------------------------------------------------------- MMA issue
         tc::reg_dec<TA_REG_MMA>();
         if (warp == TA_WMMA) {
-        constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false), id_o = tc::idesc_f16(128, NR, true, true);
-        const int pairs = nt * npair;
-        const uint64_t q_d = tc::sdesc(q_s, 16, 1024), p_d = tc::sdesc(p_s, 16, 1024);
-        // a last single chunk: its second half repeats the first, into TMEM
-        // lanes that nothing reads
-        const uint64_t v_d2 = tc::sdesc(kv_s, TA_SLOT, 1024), v_d1 = tc::sdesc(kv_s, 0, 1024);
-        bool ok = true;
-        int p = 0, j = 0, slot = 0, round = 0;                      // of S
-        int op = 0, oj = 0, stage = 0, oround = 0;                  // of O
-        for (int v = 0; v < pairs + npair + TA_LAG; v++) {
-            if (v < pairs) {
-                if (p == 0 && j > 0) ok = warp_wait(&sh.s_free, (j - 1) & 1, dead);
-                if (ok) ok = warp_wait(&sh.k_full[slot], round & 1, dead);
-                if (!ok) break;
-                tc::fence_after();
-                if (tc::elect_one()) {
-                    const uint32_t ka = tmem + k_col + 64 * slot;
-                    const uint64_t qb = q_d + (uint64_t)(2 * p * NR * 8);
+            constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false), id_o = tc::idesc_f16(128, NR, true, true);
+            const int pairs = nt * npair, behind = npair + TA_LAG;
+            const uint64_t q_d = tc::sdesc(q_s, 16, 1024), p_d = tc::sdesc(p_s, 16, 1024);
+            // a last single chunk: its second half repeats the first, into
+            // TMEM lanes that nothing reads
+            const uint64_t v_d2 = tc::sdesc(kv_s, TA_SLOT, 1024), v_d1 = tc::sdesc(kv_s, 0, 1024);
+            int p = 0, j = 0, slot = 0, kpar = 0;                       // of S
+            int op = 0, oj = 0, stage = 0, vpar = 0;                    // of O
+            for (int v = 0; v < pairs + behind; v++) {
+                if (v < pairs) {
+                    if (p == 0 && j > 0) warp_wait(&sh.s_free, (j - 1) & 1, dead);
+                    warp_wait(&sh.k_full[slot], kpar, dead);
+                    tc::fence_after();
+                    if (tc::elect_one()) {
+                        const uint32_t ka = tmem + k_col + 64 * slot;
+                        const uint64_t qb = q_d + (uint64_t)(2 * p * NR * 8);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) tc::mma_f16_ta(tmem + s_col, ka + 8 * k, qb + 2 * k, id_s, p > 0 || k > 0);
-                    if (2 * p + 1 < nch) {
+                        for (int k = 0; k < 4; k++) tc::mma_f16_ta(tmem + s_col, ka + 8 * k, qb + 2 * k, id_s, p > 0 || k > 0);
+                        if (2 * p + 1 < nch) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) tc::mma_f16_ta(tmem + s_col, ka + 32 + 8 * k, qb + NR * 8 + 2 * k, id_s, true);
+                            for (int k = 0; k < 4; k++)
+                                tc::mma_f16_ta(tmem + s_col, ka + 32 + 8 * k, qb + NR * 8 + 2 * k, id_s, true);
+                        }
+                        tc::mma_commit(tc::smem_u32(&sh.k_done[slot]));
+                        if (p == npair - 1) tc::mma_commit(tc::smem_u32(&sh.s_full));
                     }
-                    tc::mma_commit(tc::smem_u32(&sh.k_done[slot]));
-                    if (p == npair - 1) tc::mma_commit(tc::smem_u32(&sh.s_full));
+                    __syncwarp();
+                    if (++slot == KR) slot = 0, kpar ^= 1;
+                    if (++p == npair) p = 0, j++;
                 }
-                __syncwarp();
-                if (++slot == KR) slot = 0, round++;
-                if (++p == npair) p = 0, j++;
-            }
-            if (v >= npair + TA_LAG) {
-                if (op == 0) ok = warp_wait(&sh.p_full, oj & 1, dead);
-                if (ok) ok = warp_wait(&sh.v_full[stage * TA_PAIRS + op], oround & 1, dead);
-                if (!ok) break;
-                tc::fence_after();
-                if (tc::elect_one()) {
-                    const uint64_t va = (2 * op + 1 < nch ? v_d2 : v_d1) + (uint64_t)((stage * nch + 2 * op) * (TA_SLOT >> 4));
+                if (v >= behind) {
+                    if (op == 0) warp_wait(&sh.p_full, oj & 1, dead);
+                    warp_wait(&sh.v_full[stage * TA_PAIRS + op], vpar, dead);
+                    tc::fence_after();
+                    if (tc::elect_one()) {
+                        const uint64_t va = (2 * op + 1 < nch ? v_d2 : v_d1) + (uint64_t)((stage * nch + 2 * op) * (TA_SLOT >> 4));
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        tc::mma_f16(tmem + o_col + op * NR, va + 128 * k, p_d + 128 * k, id_o, oj > 0 || k > 0);
-                    tc::mma_commit(tc::smem_u32(&sh.v_empty[stage * TA_PAIRS + op]));
-                    if (op == npair - 1) tc::mma_commit(tc::smem_u32(&sh.pv_done));
-                }
-                __syncwarp();
-                if (++op == npair) {
-                    op = 0;
-                    oj++;
-                    if (++stage == ST) stage = 0, oround++;
+                        for (int k = 0; k < 8; k++)
+                            tc::mma_f16(tmem + o_col + op * NR, va + 128 * k, p_d + 128 * k, id_o, oj > 0 || k > 0);
+                        tc::mma_commit(tc::smem_u32(&sh.v_empty[stage * TA_PAIRS + op]));
+                        if (op == npair - 1) tc::mma_commit(tc::smem_u32(&sh.pv_done));
+                    }
+                    __syncwarp();
+                    if (++op == npair) {
+                        op = 0;
+                        oj++;
+                        if (++stage == ST) stage = 0, vpar ^= 1;
+                    }
                 }
             }
-        }
-        if (!ok) {              // let what was issued finish before TMEM is freed
-            const uint64_t t0 = tc::now_ns();
-            while (tc::now_ns() - t0 < 1000000ull) {}
-        }
-        __syncwarp();
+            if (*dead) {        // let what was issued finish before TMEM is freed
+                const uint64_t t0 = tc::now_ns();
+                while (tc::now_ns() - t0 < 1000000ull) {}
+            }
         }
     } else {
         // --------------------------------------------------------- softmax
@@ -477,7 +484,7 @@ k_tree_attn(const __grid_constant__ Args g)
             const bool drafts = (tb + j + 1) * TA_KEYS > ctx;     // the tile holds drafted rows
             // NaN rows have NaN scores and weights
             const float ks = kx == 255 ? __int_as_float(0x7FC00000) : pow2i(kx - 127);
-            const bool ok = warp_wait(&sh.s_full, j & 1, dead);
+            warp_wait(&sh.s_full, j & 1, dead);
             tc::fence_after();
             float x[NC];
             float over;
@@ -518,8 +525,7 @@ k_tree_attn(const __grid_constant__ Args g)
             };
             load();
             const bool raise = over > TA_RAISE || (valid && kx < 255 && kx - E > 7);
-            if (soft_any(raise || !ok)) {
-                if (soft_any(!ok)) break;
+            if (soft_any(raise)) {
                 // raise the references: the rows' maxima over the tile, as
                 // integers of the same order (a NaN has none)
                 scores(false);
@@ -550,7 +556,8 @@ k_tree_attn(const __grid_constant__ Args g)
                 E = En;
 #pragma unroll
                 for (int i = 0; i < NC; i++) l[i] *= sh.fl[c0 + i];
-                if (j > 0 && warp_wait(&sh.pv_done, (j - 1) & 1, dead)) {
+                if (j > 0) {
+                    warp_wait(&sh.pv_done, (j - 1) & 1, dead);
                     tc::fence_after();
                     for (int p = 0; p < nblk; p++)
 #pragma unroll
@@ -605,7 +612,7 @@ k_tree_attn(const __grid_constant__ Args g)
         }
         if (lane < NC) sh.lsum[warp & 3][c0 + lane] = v[0];
         soft_sync();
-        const bool done = warp_wait(&sh.pv_done, (nt - 1) & 1, dead);
+        warp_wait(&sh.pv_done, (nt - 1) & 1, dead);
         tc::fence_after();
         if (tid < NR && tid < nr) {
             const float m = sh.cm[tid].y, sum = (sh.lsum[0][tid] + sh.lsum[1][tid]) + (sh.lsum[2][tid] + sh.lsum[3][tid]);
@@ -618,33 +625,31 @@ k_tree_attn(const __grid_constant__ Args g)
             sh.fo[tid] = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / den;
         }
         soft_sync();
-        if (done) {
-            const float s = pow2i(E - 127);
-            for (int p = 0; p < nblk; p++) {
-                const int e = p * 128 + key;
-                float x[NC];
+        const float s = pow2i(E - 127);
+        for (int p = 0; p < nblk; p++) {
+            const int e = p * 128 + key;
+            float x[NC];
 #pragma unroll
-                for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
-                tc::tmem_wait_ld(x);
-                if (e >= d) continue;
-                if (g.nsplit > 1) {
-                    float *o = g.part.o + (prow + c0) * d + e;
+            for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
+            tc::tmem_wait_ld(x);
+            if (e >= d) continue;
+            if (g.nsplit > 1) {
+                float *o = g.part.o + (prow + c0) * d + e;
 #pragma unroll
-                    for (int i = 0; i < NC; i++)
-                        if (c0 + i < nr) {
-                            const float f = sh.fo[c0 + i];
-                            o[(size_t)i * d] = f == 0.0f ? 0.0f : x[i] * f * s;
-                        }
-                } else {
+                for (int i = 0; i < NC; i++)
+                    if (c0 + i < nr) {
+                        const float f = sh.fo[c0 + i];
+                        o[(size_t)i * d] = f == 0.0f ? 0.0f : x[i] * f * s;
+                    }
+            } else {
 #pragma unroll
-                    for (int i = 0; i < NC; i++)
-                        if (c0 + i < nr) {
-                            const float f = sh.fo[c0 + i], y = f == 0.0f ? 0.0f : x[i] * f * s;
-                            const size_t o = sh.out_at[c0 + i] + e;
-                            if (a.dt == DSV4B_BF16) st_row1<DSV4B_BF16>(a.o, o, y);
-                            else st_row1<DSV4B_F16>(a.o, o, y);
-                        }
-                }
+                for (int i = 0; i < NC; i++)
+                    if (c0 + i < nr) {
+                        const float f = sh.fo[c0 + i], y = f == 0.0f ? 0.0f : x[i] * f * s;
+                        const size_t o = sh.out_at[c0 + i] + e;
+                        if (a.dt == DSV4B_BF16) st_row1<DSV4B_BF16>(a.o, o, y);
+                        else st_row1<DSV4B_F16>(a.o, o, y);
+                    }
             }
         }
         tc::fence_before();

@@ -50,19 +50,21 @@ __device__ __forceinline__ uint64_t now_ns()
     return t;
 }
 
-// Wait for the phase of `parity` to complete. A wait of more than two seconds
-// sets *dead, and once that is set every wait returns: the block runs to its
-// end with results that are not valid.
-// (The clock is read once in 256 tries: a wait's instructions take issue slots
-// from the warps that work.)
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead)
+// A whole warp waits for the phase of `parity` to complete. A wait of more
+// than two seconds sets *dead, and once that is set every wait returns: the
+// block runs to its end with results that are not valid. The votes keep the
+// control flow uniform, so that loop counters, barrier addresses and operand
+// descriptors around a wait can live in uniform registers: without them an
+// MMA's issue took 80 cycles instead of 27. (The clock is read once in 256
+// tries: a wait's instructions take issue slots from the warps that work.)
+__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatile int *dead)
 {
     uint64_t t0 = 0;
     while (true) {
 #pragma unroll 1
         for (int i = 0; i < 256; i++)
-            if (mbar_try(bar, parity)) return;
-        if (*dead) return;
+            if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
+        if (__any_sync(0xffffffffu, *dead)) return;
         const uint64_t t = now_ns();
         if (t0 == 0) t0 = t;
         if (t - t0 > 2000000000ull) *dead = 1;
@@ -160,22 +162,22 @@ __device__ __forceinline__ void tmem_wait_ld(float (&v)[N])
 #pragma unroll
     for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r)
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r)
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
-// 16 columns, as words.
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16])
+// 32 columns, as words.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32])
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16])
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32])
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; i++) asm volatile("" : "+r"(r[i]));
+    for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 

@@ -34,14 +34,13 @@
 // A block takes one tile of rows and a run of 128-key tiles, cut into chunk
 // pairs of 128 elements:
 //   8 widening warps thread = one key and every other 64-element chunk: read
-//                    its codes (64 bytes, two chunks in flight), widen e4m3
+//                    its codes (64 bytes; one chunk in flight while one is widened), widen e4m3
 //                    to f16 -- exact, the row scale stays outside -- into a
 //                    TMEM ring of 3 or 4 pairs;
 //   8 copying warps  from there to shared memory once the second product has
 //                    freed the pair's place (128-byte swizzle; V^T is the
 //                    same bytes, M-major);
-//   1 MMA warp       issues S of pair v, then O of the pair one tile and one
-//                    pair behind it;
+//   2 MMA warps      one issues S pair by pair, one O;
 //   8 softmax warps  thread = one key and half of the rows.
 //
 // Numbers. With s_j = 2^e_j the row scale, score = S (scale 2^e_j) in float
@@ -63,7 +62,6 @@ namespace {
 
 constexpr int TA_KEYS = 128;                        // keys of a tile (M of S^T)
 constexpr int TA_SOFT = 8, TA_LOAD = 8, TA_COPY = 8;    // softmax, widening and copying warps
-constexpr int TA_LAG = 1;                           // pairs, beyond a tile, that O runs behind S
 constexpr int TA_RING = 4;                          // most pairs of the TMEM ring
 constexpr int TA_WCOPY = TA_SOFT + TA_LOAD, TA_WMMA = TA_WCOPY + TA_COPY;   // the MMA warp, in a warpgroup of its own
 constexpr int TA_T = 32 * (TA_WMMA + 4);
@@ -117,16 +115,17 @@ __device__ __forceinline__ float pow2i(int e)
     return __uint_as_float(e < -126 ? 0u : e > 127 ? 0x7F800000u : (uint32_t)(e + 127) << 23);
 }
 
-// Votes among the 8 softmax warps.
-__device__ __forceinline__ bool soft_any(bool p)
+// Among the 4 softmax warps of a half of the rows (named barriers 1 and 2):
+// a vote, and a barrier.
+__device__ __forceinline__ bool soft_any(bool p, int wg)
 {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-                 "barrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"((uint32_t)p) : "memory");
+                 "barrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"((uint32_t)p), "r"(wg + 1) : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void soft_sync(int wg) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(wg + 1) : "memory"); }
 
 // 64 bytes of a row.
 struct Unit {
@@ -145,8 +144,9 @@ __device__ __forceinline__ void ld64(Unit &u)
 
 __device__ __forceinline__ uint32_t e4m3x2_f16(uint32_t v)
 {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)v));
+    return r;
 }
 
 __device__ __forceinline__ void st_smem16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
@@ -154,11 +154,9 @@ __device__ __forceinline__ void st_smem16(uint32_t a, uint32_t x, uint32_t y, ui
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// mbar_wait by a whole warp.
 __device__ __forceinline__ void warp_wait(const uint64_t *bar, uint32_t parity, volatile int *dead)
 {
-    tc::mbar_wait(tc::smem_u32(bar), parity, dead);
-    __syncwarp();
+    tc::warp_wait(tc::smem_u32(bar), parity, dead);
 }
 __device__ __forceinline__ void warp_arrive(const uint64_t *bar, int lane)
 {
@@ -302,64 +300,41 @@ k_tree_attn(const __grid_constant__ Args g)
         };
         const uint32_t k_mine = tmem + ((uint32_t)quad << 21) + k_col + 32 * half;
         const int pairs = nt * npair;
-        int i = 0, c = half, slot = 0, par = 1;         // pair, chunk, ring place, parity of its last use
-        auto open = [&]() {
-            if (i >= KR) warp_wait(&sh.k_done[slot], par, dead);
-            tc::fence_after();
-        };
-        auto close = [&]() {
+        int slot = 0, par = 1, c = half;                // ring place, parity of its last use, chunk
+        Unit u;
+        fetch(u);
+        for (int i = 0; i < pairs; i++) {
+            if (c < nch) {
+                uint32_t h[32];                         // widened before the place is free
+                if (c < ndq) {
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        h[2 * k] = e4m3x2_f16(u.w[k] & 0xFFFFu);
+                        h[2 * k + 1] = e4m3x2_f16(u.w[k] >> 16);
+                    }
+                } else {
+                    Unit t;
+                    t.src = u.src + 64;
+                    ld64(t);
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        h[k] = u.w[k];
+                        h[16 + k] = t.w[k];
+                    }
+                }
+                fetch(u);
+                if (i >= KR) warp_wait(&sh.k_done[slot], par, dead);
+                tc::fence_after();
+                tc::tmem_st32(k_mine + 64 * slot, h);
+                tc::tmem_wait_st();
+            } else if (i >= KR) {
+                warp_wait(&sh.k_done[slot], par, dead);
+            }
+            tc::fence_before();
             warp_arrive(&sh.k_full[slot], lane);
-            i++;
             c += 2;
             if (c >= 2 * npair) c = half;
             if (++slot == KR) slot = 0, par ^= 1;
-        };
-        auto put = [&](Unit &u) {
-            const uint32_t dst = k_mine + 64 * slot;
-            if (c < ndq) {
-                open();
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    uint32_t h[16];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        h[2 * k] = e4m3x2_f16(u.w[8 * s + k] & 0xFFFFu);
-                        h[2 * k + 1] = e4m3x2_f16(u.w[8 * s + k] >> 16);
-                    }
-                    tc::tmem_st16(dst + 16 * s, h);
-                }
-            } else {
-                Unit t;
-                t.src = u.src + 64;
-                ld64(t);
-                open();
-                tc::tmem_st16(dst, u.w);
-                tc::tmem_st16(dst + 16, t.w);
-            }
-            fetch(u);
-            tc::tmem_wait_st();
-            tc::fence_before();
-            close();
-            if (c >= nch && i < pairs) {                // a pair without a chunk for this warp
-                open();
-                close();
-            }
-        };
-        // two chunks in flight, in registers of their own: a copy between them
-        // would wait for the load
-        Unit u0, u1;
-        fetch(u0);
-        fetch(u1);
-        if (half < nch) {
-            while (i < pairs) {
-                put(u0);
-                if (i < pairs) put(u1);
-            }
-        } else {
-            while (i < pairs) {
-                open();
-                close();
-            }
         }
     } else if (warp >= TA_WCOPY && warp < TA_WMMA) {
         // ---------------------------------------------------------- copying
@@ -370,24 +345,23 @@ k_tree_attn(const __grid_constant__ Args g)
         int p = 0, slot = 0, kpar = 0, stage = 0, vpar = 1;
         for (int i = 0; i < pairs; i++) {
             const int c = 2 * p + half;
+            uint32_t h[32];
             warp_wait(&sh.k_full[slot], kpar, dead);
-            if (i >= ST * npair) warp_wait(&sh.v_empty[stage * TA_PAIRS + p], vpar, dead);
             tc::fence_after();
+            if (c < nch) {
+                tc::tmem_ld32(k_mine + 64 * slot, h);
+                tc::tmem_wait_ld(h);
+                tc::fence_before();
+            }
+            warp_arrive(&sh.k_done[slot], lane);
+            if (i >= ST * npair) warp_wait(&sh.v_empty[stage * TA_PAIRS + p], vpar, dead);
             if (c < nch) {
                 const uint32_t dst = kv_s + (stage * nch + c) * TA_SLOT + key * 128;
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    uint32_t h[16];
-                    tc::tmem_ld16(k_mine + 64 * slot + 16 * s, h);
-                    tc::tmem_wait_ld(h);
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        st_smem16(dst + (((4 * s + k) ^ sw) << 4), h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
-                }
-                tc::fence_before();
+                for (int k = 0; k < 8; k++)
+                    st_smem16(dst + ((k ^ sw) << 4), h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
                 tc::fence_async_smem();
             }
-            warp_arrive(&sh.k_done[slot], lane);
             warp_arrive(&sh.v_full[stage * TA_PAIRS + p], lane);
             if (++slot == KR) slot = 0, kpar ^= 1;
             if (++p == npair) {
@@ -398,57 +372,62 @@ k_tree_attn(const __grid_constant__ Args g)
     } else if (warp >= TA_WMMA) {
         // ------------------------------------------------------- MMA issue
         tc::reg_dec<TA_REG_MMA>();
+        // Two warps, one for each product, each in the order of the pairs: the
+        // tensor core takes what is ready of either.
+        const int pairs = nt * npair;
         if (warp == TA_WMMA) {
-            constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false), id_o = tc::idesc_f16(128, NR, true, true);
-            const int pairs = nt * npair, behind = npair + TA_LAG;
-            const uint64_t q_d = tc::sdesc(q_s, 16, 1024), p_d = tc::sdesc(p_s, 16, 1024);
+            constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false);
+            const uint64_t q_d = tc::sdesc(q_s, 16, 1024);
+            int p = 0, j = 0, slot = 0, kpar = 0;
+            for (int v = 0; v < pairs; v++) {
+                if (p == 0 && j > 0) warp_wait(&sh.s_free, (j - 1) & 1, dead);
+                warp_wait(&sh.k_full[slot], kpar, dead);
+                tc::fence_after();
+                if (tc::elect_one()) {
+                    const uint32_t ka = tmem + k_col + 64 * slot;
+                    const uint64_t qb = q_d + (uint64_t)(2 * p * NR * 8);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tc::mma_f16_ta(tmem + s_col, ka + 8 * k, qb + 2 * k, id_s, p > 0 || k > 0);
+                    if (2 * p + 1 < nch) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            tc::mma_f16_ta(tmem + s_col, ka + 32 + 8 * k, qb + NR * 8 + 2 * k, id_s, true);
+                    }
+                    tc::mma_commit(tc::smem_u32(&sh.k_done[slot]));
+                    if (p == npair - 1) tc::mma_commit(tc::smem_u32(&sh.s_full));
+                }
+                __syncwarp();
+                if (++slot == KR) slot = 0, kpar ^= 1;
+                if (++p == npair) p = 0, j++;
+            }
+        } else if (warp == TA_WMMA + 1) {
+            constexpr uint32_t id_o = tc::idesc_f16(128, NR, true, true);
+            const uint64_t p_d = tc::sdesc(p_s, 16, 1024);
             // a last single chunk: its second half repeats the first, into
             // TMEM lanes that nothing reads
             const uint64_t v_d2 = tc::sdesc(kv_s, TA_SLOT, 1024), v_d1 = tc::sdesc(kv_s, 0, 1024);
-            int p = 0, j = 0, slot = 0, kpar = 0;                       // of S
-            int op = 0, oj = 0, stage = 0, vpar = 0;                    // of O
-            for (int v = 0; v < pairs + behind; v++) {
-                if (v < pairs) {
-                    if (p == 0 && j > 0) warp_wait(&sh.s_free, (j - 1) & 1, dead);
-                    warp_wait(&sh.k_full[slot], kpar, dead);
-                    tc::fence_after();
-                    if (tc::elect_one()) {
-                        const uint32_t ka = tmem + k_col + 64 * slot;
-                        const uint64_t qb = q_d + (uint64_t)(2 * p * NR * 8);
+            int p = 0, j = 0, stage = 0, vpar = 0;
+            for (int v = 0; v < pairs; v++) {
+                if (p == 0) warp_wait(&sh.p_full, j & 1, dead);
+                warp_wait(&sh.v_full[stage * TA_PAIRS + p], vpar, dead);
+                tc::fence_after();
+                if (tc::elect_one()) {
+                    const uint64_t va = (2 * p + 1 < nch ? v_d2 : v_d1) + (uint64_t)((stage * nch + 2 * p) * (TA_SLOT >> 4));
 #pragma unroll
-                        for (int k = 0; k < 4; k++) tc::mma_f16_ta(tmem + s_col, ka + 8 * k, qb + 2 * k, id_s, p > 0 || k > 0);
-                        if (2 * p + 1 < nch) {
-#pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                tc::mma_f16_ta(tmem + s_col, ka + 32 + 8 * k, qb + NR * 8 + 2 * k, id_s, true);
-                        }
-                        tc::mma_commit(tc::smem_u32(&sh.k_done[slot]));
-                        if (p == npair - 1) tc::mma_commit(tc::smem_u32(&sh.s_full));
-                    }
-                    __syncwarp();
-                    if (++slot == KR) slot = 0, kpar ^= 1;
-                    if (++p == npair) p = 0, j++;
+                    for (int k = 0; k < 8; k++)
+                        tc::mma_f16(tmem + o_col + p * NR, va + 128 * k, p_d + 128 * k, id_o, j > 0 || k > 0);
+                    tc::mma_commit(tc::smem_u32(&sh.v_empty[stage * TA_PAIRS + p]));
+                    if (p == npair - 1) tc::mma_commit(tc::smem_u32(&sh.pv_done));
                 }
-                if (v >= behind) {
-                    if (op == 0) warp_wait(&sh.p_full, oj & 1, dead);
-                    warp_wait(&sh.v_full[stage * TA_PAIRS + op], vpar, dead);
-                    tc::fence_after();
-                    if (tc::elect_one()) {
-                        const uint64_t va = (2 * op + 1 < nch ? v_d2 : v_d1) + (uint64_t)((stage * nch + 2 * op) * (TA_SLOT >> 4));
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            tc::mma_f16(tmem + o_col + op * NR, va + 128 * k, p_d + 128 * k, id_o, oj > 0 || k > 0);
-                        tc::mma_commit(tc::smem_u32(&sh.v_empty[stage * TA_PAIRS + op]));
-                        if (op == npair - 1) tc::mma_commit(tc::smem_u32(&sh.pv_done));
-                    }
-                    __syncwarp();
-                    if (++op == npair) {
-                        op = 0;
-                        oj++;
-                        if (++stage == ST) stage = 0, vpar ^= 1;
-                    }
+                __syncwarp();
+                if (++p == npair) {
+                    p = 0;
+                    j++;
+                    if (++stage == ST) stage = 0, vpar ^= 1;
                 }
             }
+        }
+        if (warp <= TA_WMMA + 1) {
             if (*dead) {        // let what was issued finish before TMEM is freed
                 const uint64_t t0 = tc::now_ns();
                 while (tc::now_ns() - t0 < 1000000ull) {}
@@ -525,7 +504,7 @@ k_tree_attn(const __grid_constant__ Args g)
             };
             load();
             const bool raise = over > TA_RAISE || (valid && kx < 255 && kx - E > 7);
-            if (soft_any(raise)) {
+            if (soft_any(raise, wg)) {
                 // raise the references: the rows' maxima over the tile, as
                 // integers of the same order (a NaN has none)
                 scores(false);
@@ -540,19 +519,20 @@ k_tree_attn(const __grid_constant__ Args g)
                 if (lane < NC) sh.wmax[warp & 3][c0 + lane] = __int_as_float(mine);
                 const int kw = __reduce_max_sync(0xffffffffu, valid && kx < 255 ? kx : TA_NONE);
                 if (lane == 0) sh.wk[warp] = kw;
-                soft_sync();
+                soft_sync(wg);
                 int En = E;
 #pragma unroll
-                for (int w = 0; w < 4; w++) En = max(En, sh.wk[w]);
-                if (tid < NR) {
-                    const float mo = sh.cm[tid].y;
-                    const float mn = fmaxf(fmaxf(mo, fmaxf(sh.wmax[0][tid], sh.wmax[1][tid])), fmaxf(sh.wmax[2][tid], sh.wmax[3][tid]));
+                for (int w = 0; w < 4; w++) En = max(En, sh.wk[4 * wg + w]);
+                if (key < NC) {
+                    const int r = c0 + key;
+                    const float mo = sh.cm[r].y;
+                    const float mn = fmaxf(fmaxf(mo, fmaxf(sh.wmax[0][r], sh.wmax[1][r])), fmaxf(sh.wmax[2][r], sh.wmax[3][r]));
                     const float f = mo == -INFINITY ? 0.0f : ex2(mo - mn);
-                    sh.fl[tid] = f;
-                    sh.fo[tid] = f * pow2i(E - En);
-                    sh.cm[tid].y = mn;
+                    sh.fl[r] = f;
+                    sh.fo[r] = f * pow2i(E - En);
+                    sh.cm[r].y = mn;
                 }
-                soft_sync();
+                soft_sync(wg);
                 E = En;
 #pragma unroll
                 for (int i = 0; i < NC; i++) l[i] *= sh.fl[c0 + i];
@@ -611,20 +591,21 @@ k_tree_attn(const __grid_constant__ Args g)
             }
         }
         if (lane < NC) sh.lsum[warp & 3][c0 + lane] = v[0];
-        soft_sync();
+        soft_sync(wg);
         warp_wait(&sh.pv_done, (nt - 1) & 1, dead);
         tc::fence_after();
-        if (tid < NR && tid < nr) {
-            const float m = sh.cm[tid].y, sum = (sh.lsum[0][tid] + sh.lsum[1][tid]) + (sh.lsum[2][tid] + sh.lsum[3][tid]);
+        if (key < NC && c0 + key < nr) {
+            const int r = c0 + key;
+            const float m = sh.cm[r].y, sum = (sh.lsum[0][r] + sh.lsum[1][r]) + (sh.lsum[2][r] + sh.lsum[3][r]);
             float den = sum;
             if (g.nsplit > 1) {
-                g.part.ml[prow + tid] = make_float2(m, sum);
+                g.part.ml[prow + r] = make_float2(m, sum);
             } else if (a.sink && m != -INFINITY) {
-                den += ex2(__ldcg(a.sink + (r0 + tid) % H) * 1.4426950408889634f - m);
+                den += ex2(__ldcg(a.sink + (r0 + r) % H) * 1.4426950408889634f - m);
             }
-            sh.fo[tid] = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / den;
+            sh.fo[r] = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / den;
         }
-        soft_sync();
+        soft_sync(wg);
         const float s = pow2i(E - 127);
         for (int p = 0; p < nblk; p++) {
             const int e = p * 128 + key;

@@ -90,9 +90,9 @@ struct Args {
 
 struct Shared {             // behind the operand tiles
     uint64_t v_full[TA_STAGES * TA_PAIRS], v_empty[TA_STAGES * TA_PAIRS], k_full[TA_RING], k_done[TA_RING];
-    uint64_t s_full, s_free, p_full, pv_done;
+    uint64_t q_full, s_full, s_free, p_full, pv_done;
     uint64_t rowmask[TA_ROWS], out_at[TA_ROWS];     // a row's tree mask, and its first output element
-    float2 cm[TA_ROWS];     // score factor and reference of a row
+    float cq[TA_ROWS], nm[TA_ROWS];     // score factor of a row, and its negated reference
     float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
     int wk[TA_SOFT];
     uint32_t tmem;
@@ -107,6 +107,21 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
 }
 
 // 2^e for an integer e, 0 below the normal range and infinity above it.
@@ -203,6 +218,7 @@ k_tree_attn(const __grid_constant__ Args g)
             tc::mbar_init(tc::smem_u32(&sh.k_full[r]), TA_LOAD);
             tc::mbar_init(tc::smem_u32(&sh.k_done[r]), 1 + TA_COPY);
         }
+        tc::mbar_init(tc::smem_u32(&sh.q_full), TA_SOFT);
         tc::mbar_init(tc::smem_u32(&sh.s_full), 1);
         tc::mbar_init(tc::smem_u32(&sh.s_free), TA_SOFT);
         tc::mbar_init(tc::smem_u32(&sh.p_full), TA_SOFT);
@@ -210,55 +226,6 @@ k_tree_attn(const __grid_constant__ Args g)
         tc::mbar_init_fence();
         sh.dead = 0;
     }
-    // q rows to f16, one warp a row: scaled so that the largest magnitude
-    // lies in [2^14, 2^15) (f16 rows are taken as they are)
-    for (int r = warp; r < NR; r += TA_T / 32) {
-        const int gr = r0 + r, t = gr / H;
-        const uint32_t dst = q_s + r * 128;
-        uint4 w[3];
-        uint32_t top = 0;
-        int kq = 0;
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-            const int e = i * 256 + lane * 8;
-            w[i] = make_uint4(0, 0, 0, 0);
-            if (r < nr && e < d)
-                w[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const unsigned short *>(a.q) +
-                                                              ((size_t)b * a.n_tok + t) * a.q_tok + (size_t)(gr - t * H) * d + e));
-        }
-        if (a.dt == DSV4B_BF16) {
-            float v[3][8];
-#pragma unroll
-            for (int i = 0; i < 3; i++) {
-                Raw8<DSV4B_BF16> x;
-                x.w[0] = w[i];
-                widen8<DSV4B_BF16>(x, v[i]);
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const uint32_t m = __float_as_uint(v[i][k]) & 0x7FFFFFFFu;
-                    if (m < 0x7F800000u) top = max(top, m);
-                }
-            }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (top) kq = max((int)(top >> 23) - 127 - 14, -112);
-            const float f = pow2i(-kq);
-#pragma unroll
-            for (int i = 0; i < 3; i++)
-                w[i] = make_uint4(pack2<DSV4B_F16>(v[i][0] * f, v[i][1] * f), pack2<DSV4B_F16>(v[i][2] * f, v[i][3] * f),
-                                  pack2<DSV4B_F16>(v[i][4] * f, v[i][5] * f), pack2<DSV4B_F16>(v[i][6] * f, v[i][7] * f));
-        }
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-            const int e = i * 256 + lane * 8;
-            if (e < d) st_smem16(dst + (e >> 6) * (NR * 128) + ((((e >> 3) & 7) ^ (r & 7)) << 4), w[i].x, w[i].y, w[i].z, w[i].w);
-        }
-        if (lane == 0) {
-            sh.cm[r] = make_float2(a.scale * 1.4426950408889634f * pow2i(kq), -INFINITY);
-            sh.out_at[r] = ((uint64_t)b * a.n_tok + t) * a.o_tok + (uint64_t)(gr - t * H) * d;
-            sh.rowmask[r] = r < nr ? __ldcg(a.mask + (size_t)b * a.n_tok + t) : 0ull;
-        }
-    }
-    tc::fence_async_smem();
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -304,32 +271,29 @@ k_tree_attn(const __grid_constant__ Args g)
         Unit u;
         fetch(u);
         for (int i = 0; i < pairs; i++) {
-            if (c < nch) {
-                uint32_t h[32];                         // widened before the place is free
-                if (c < ndq) {
+            const uint32_t dst = k_mine + 64 * slot;
+            if (i >= KR) warp_wait(&sh.k_done[slot], par, dead);
+            tc::fence_after();
+            if (c < ndq) {
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        h[2 * k] = e4m3x2_f16(u.w[k] & 0xFFFFu);
-                        h[2 * k + 1] = e4m3x2_f16(u.w[k] >> 16);
-                    }
-                } else {
-                    Unit t;
-                    t.src = u.src + 64;
-                    ld64(t);
+                for (int s = 0; s < 2; s++) {
+                    uint32_t h[16];
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        h[k] = u.w[k];
-                        h[16 + k] = t.w[k];
+                    for (int k = 0; k < 8; k++) {
+                        h[2 * k] = e4m3x2_f16(u.w[8 * s + k] & 0xFFFFu);
+                        h[2 * k + 1] = e4m3x2_f16(u.w[8 * s + k] >> 16);
                     }
+                    tc::tmem_st16(dst + 16 * s, h);
                 }
                 fetch(u);
-                if (i >= KR) warp_wait(&sh.k_done[slot], par, dead);
-                tc::fence_after();
-                tc::tmem_st32(k_mine + 64 * slot, h);
-                tc::tmem_wait_st();
-            } else if (i >= KR) {
-                warp_wait(&sh.k_done[slot], par, dead);
+            } else if (c < nch) {
+                tc::tmem_st16(dst, u.w);
+                u.src += 64;
+                ld64(u);
+                tc::tmem_st16(dst + 16, u.w);
+                fetch(u);
             }
+            tc::tmem_wait_st();
             tc::fence_before();
             warp_arrive(&sh.k_full[slot], lane);
             c += 2;
@@ -379,6 +343,7 @@ k_tree_attn(const __grid_constant__ Args g)
             constexpr uint32_t id_s = tc::idesc_f16(128, NR, false, false);
             const uint64_t q_d = tc::sdesc(q_s, 16, 1024);
             int p = 0, j = 0, slot = 0, kpar = 0;
+            warp_wait(&sh.q_full, 0, dead);
             for (int v = 0; v < pairs; v++) {
                 if (p == 0 && j > 0) warp_wait(&sh.s_free, (j - 1) & 1, dead);
                 warp_wait(&sh.k_full[slot], kpar, dead);
@@ -438,6 +403,75 @@ k_tree_attn(const __grid_constant__ Args g)
         tc::reg_inc<TA_REG_SOFT>();
         const int wg = warp >> 2, key = (warp & 3) * 32 + lane, c0 = wg * NC;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        // q rows to f16, one warp a row, two in flight: scaled so that the
+        // largest magnitude lies in [2^14, 2^15) (f16 rows are taken as they
+        // are)
+#pragma unroll 1
+        for (int r1 = warp; r1 < NR; r1 += 2 * TA_SOFT) {
+            uint4 w[2][3];
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const int r = r1 + s * TA_SOFT, t = (r0 + r) / H;
+                const unsigned short *q = reinterpret_cast<const unsigned short *>(a.q) +
+                                          ((size_t)b * a.n_tok + t) * a.q_tok + (size_t)(r0 + r - t * H) * d;
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+                    const int e = i * 256 + lane * 8;
+                    w[s][i] = make_uint4(0, 0, 0, 0);
+                    if (r < nr && e < d) w[s][i] = __ldcg(reinterpret_cast<const uint4 *>(q + e));
+                }
+                if (lane == 0 && r < NR) {
+                    sh.out_at[r] = ((uint64_t)b * a.n_tok + t) * a.o_tok + (uint64_t)(r0 + r - t * H) * d;
+                    sh.rowmask[r] = r < nr ? __ldcg(a.mask + (size_t)b * a.n_tok + t) : 0ull;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const int r = r1 + s * TA_SOFT;
+                if (r >= NR) break;
+                int kq = 0;
+                if (a.dt == DSV4B_BF16) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        const uint32_t u[4] = {w[s][i].x, w[s][i].y, w[s][i].z, w[s][i].w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t lo = u[k] & 0x7FFFu, hi = (u[k] >> 16) & 0x7FFFu;
+                            if (lo < 0x7F80u) top = max(top, lo);
+                            if (hi < 0x7F80u) top = max(top, hi);
+                        }
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    if (top) kq = max((int)(top >> 7) - 127 - 14, -112);
+                    const float f = pow2i(-kq);
+#pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        uint32_t u[4] = {w[s][i].x, w[s][i].y, w[s][i].z, w[s][i].w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float2 v = bf16x2(u[k]);
+                            u[k] = pack2<DSV4B_F16>(v.x * f, v.y * f);
+                        }
+                        w[s][i] = make_uint4(u[0], u[1], u[2], u[3]);
+                    }
+                }
+                const uint32_t dst = q_s + r * 128;
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+                    const int e = i * 256 + lane * 8;
+                    if (e < d)
+                        st_smem16(dst + (e >> 6) * (NR * 128) + ((((e >> 3) & 7) ^ (r & 7)) << 4), w[s][i].x, w[s][i].y, w[s][i].z, w[s][i].w);
+                }
+                if (lane == 0) {
+                    sh.cq[r] = a.scale * 1.4426950408889634f * pow2i(kq);
+                    sh.nm[r] = INFINITY;
+                }
+            }
+        }
+        tc::fence_async_smem();
+        warp_arrive(&sh.q_full, lane);
+        warp_wait(&sh.q_full, 0, dead);
         const int shift = g.page_shift, rm = a.c.page_rows - 1;
         const int *pages = a.pages + (size_t)b * a.max_pages;
         const unsigned char *scales = reinterpret_cast<const unsigned char *>(a.c.scales);
@@ -461,8 +495,7 @@ k_tree_attn(const __grid_constant__ Args g)
             const bool valid = kx >= 0;
             const int draft = (tb + j) * TA_KEYS + key - ctx;
             const bool drafts = (tb + j + 1) * TA_KEYS > ctx;     // the tile holds drafted rows
-            // NaN rows have NaN scores and weights
-            const float ks = kx == 255 ? __int_as_float(0x7FC00000) : pow2i(kx - 127);
+            const float ks = e8m0((uint8_t)kx);         // NaN for a NaN row: so are its scores and weights
             warp_wait(&sh.s_full, j & 1, dead);
             tc::fence_after();
             float x[NC];
@@ -474,10 +507,12 @@ k_tree_attn(const __grid_constant__ Args g)
                 for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + s_col + c0 + i, x + i);
                 tc::tmem_wait_ld(x);
 #pragma unroll
-                for (int i = 0; i < NC; i += 2) {
-                    const float4 cm = *reinterpret_cast<const float4 *>(&sh.cm[c0 + i]);
-                    x[i] = fmaf(x[i] * ks, cm.x, lift ? -cm.y : 0.0f);
-                    x[i + 1] = fmaf(x[i + 1] * ks, cm.z, lift ? -cm.w : 0.0f);
+                for (int i = 0; i < NC; i += 4) {
+                    const float4 cq = *reinterpret_cast<const float4 *>(&sh.cq[c0 + i]);
+                    const float4 nm = lift ? *reinterpret_cast<const float4 *>(&sh.nm[c0 + i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const float2 u = fma2(mul2(make_float2(x[i], x[i + 1]), make_float2(ks, ks)), make_float2(cq.x, cq.y), make_float2(nm.x, nm.y));
+                    const float2 v = fma2(mul2(make_float2(x[i + 2], x[i + 3]), make_float2(ks, ks)), make_float2(cq.z, cq.w), make_float2(nm.z, nm.w));
+                    x[i] = u.x, x[i + 1] = u.y, x[i + 2] = v.x, x[i + 3] = v.y;
                 }
                 if (drafts && draft >= 0) {
 #pragma unroll
@@ -525,12 +560,12 @@ k_tree_attn(const __grid_constant__ Args g)
                 for (int w = 0; w < 4; w++) En = max(En, sh.wk[4 * wg + w]);
                 if (key < NC) {
                     const int r = c0 + key;
-                    const float mo = sh.cm[r].y;
+                    const float mo = -sh.nm[r];
                     const float mn = fmaxf(fmaxf(mo, fmaxf(sh.wmax[0][r], sh.wmax[1][r])), fmaxf(sh.wmax[2][r], sh.wmax[3][r]));
                     const float f = mo == -INFINITY ? 0.0f : ex2(mo - mn);
                     sh.fl[r] = f;
                     sh.fo[r] = f * pow2i(E - En);
-                    sh.cm[r].y = mn;
+                    sh.nm[r] = -mn;
                 }
                 soft_sync(wg);
                 E = En;
@@ -552,24 +587,26 @@ k_tree_attn(const __grid_constant__ Args g)
                     tc::tmem_wait_st();
                 }
 #pragma unroll
-                for (int i = 0; i < NC; i++) x[i] = x[i] == -INFINITY ? x[i] : x[i] - sh.cm[c0 + i].y;
+                for (int i = 0; i < NC; i++) x[i] = x[i] == -INFINITY ? x[i] : x[i] + sh.nm[c0 + i];
             } else {
                 free_s();
             }
             // weights: sums in float, the f16 operand of the second product
-            const float w = valid && kx < 255 ? pow2i(kx - E) : 1.0f;
+            const __half2 w = __float2half2_rn(valid && kx < 255 ? pow2i(kx - E) : 1.0f);
+            uint32_t pw[NC / 2];
 #pragma unroll
-            for (int i = 0; i < NC; i++) {
-                const float e = ex2(x[i]);
-                l[i] += e;
-                x[i] = e * w;
+            for (int i = 0; i < NC; i += 2) {
+                const float2 e = make_float2(ex2(x[i]), ex2(x[i + 1]));
+                const float2 s = add2(make_float2(l[i], l[i + 1]), e);
+                l[i] = s.x, l[i + 1] = s.y;
+                const __half2 h = __hmul2(__floats2half2_rn(e.x, e.y), w);
+                pw[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
             }
             if (j > 0) warp_wait(&sh.pv_done, (j - 1) & 1, dead);
             const uint32_t dst = p_s + key * 128;
 #pragma unroll
             for (int i = 0; i < NC; i += 8)
-                st_smem16(dst + ((((c0 + i) >> 3) ^ (key & 7)) << 4), pack2<DSV4B_F16>(x[i], x[i + 1]), pack2<DSV4B_F16>(x[i + 2], x[i + 3]),
-                          pack2<DSV4B_F16>(x[i + 4], x[i + 5]), pack2<DSV4B_F16>(x[i + 6], x[i + 7]));
+                st_smem16(dst + ((((c0 + i) >> 3) ^ (key & 7)) << 4), pw[i / 2], pw[i / 2 + 1], pw[i / 2 + 2], pw[i / 2 + 3]);
             tc::fence_async_smem();
             tc::fence_before();
             __syncwarp();
@@ -596,17 +633,19 @@ k_tree_attn(const __grid_constant__ Args g)
         tc::fence_after();
         if (key < NC && c0 + key < nr) {
             const int r = c0 + key;
-            const float m = sh.cm[r].y, sum = (sh.lsum[0][r] + sh.lsum[1][r]) + (sh.lsum[2][r] + sh.lsum[3][r]);
+            const float m = -sh.nm[r], sum = (sh.lsum[0][r] + sh.lsum[1][r]) + (sh.lsum[2][r] + sh.lsum[3][r]);
             float den = sum;
             if (g.nsplit > 1) {
                 g.part.ml[prow + r] = make_float2(m, sum);
             } else if (a.sink && m != -INFINITY) {
                 den += ex2(__ldcg(a.sink + (r0 + r) % H) * 1.4426950408889634f - m);
             }
+            // the row scales' reference goes with it; 0 where nothing was seen
             sh.fo[r] = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / den;
         }
         soft_sync(wg);
-        const float s = pow2i(E - 127);
+        const float s = E == TA_NONE ? 0.0f : e8m0((uint8_t)E);
+#pragma unroll 1
         for (int p = 0; p < nblk; p++) {
             const int e = p * 128 + key;
             float x[NC];
@@ -617,20 +656,18 @@ k_tree_attn(const __grid_constant__ Args g)
             if (g.nsplit > 1) {
                 float *o = g.part.o + (prow + c0) * d + e;
 #pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    if (c0 + i < nr) *o = x[i] * sh.fo[c0 + i] * s;
+                    o += d;
+                }
+            } else if (a.dt == DSV4B_BF16) {
+#pragma unroll
                 for (int i = 0; i < NC; i++)
-                    if (c0 + i < nr) {
-                        const float f = sh.fo[c0 + i];
-                        o[(size_t)i * d] = f == 0.0f ? 0.0f : x[i] * f * s;
-                    }
+                    if (c0 + i < nr) st_row1<DSV4B_BF16>(a.o, sh.out_at[c0 + i] + e, x[i] * sh.fo[c0 + i] * s);
             } else {
 #pragma unroll
                 for (int i = 0; i < NC; i++)
-                    if (c0 + i < nr) {
-                        const float f = sh.fo[c0 + i], y = f == 0.0f ? 0.0f : x[i] * f * s;
-                        const size_t o = sh.out_at[c0 + i] + e;
-                        if (a.dt == DSV4B_BF16) st_row1<DSV4B_BF16>(a.o, o, y);
-                        else st_row1<DSV4B_F16>(a.o, o, y);
-                    }
+                    if (c0 + i < nr) st_row1<DSV4B_F16>(a.o, sh.out_at[c0 + i] + e, x[i] * sh.fo[c0 + i] * s);
             }
         }
         tc::fence_before();

@@ -16,7 +16,7 @@ bool row_dt(int dt) { return dt == DSV4B_F32 || dt == DSV4B_BF16 || dt == DSV4B_
 
 bool cache_ok(const dsv4b_kvq *c)
 {
-    if (!c || !c->codes || !c->scales || ((uintptr_t)c->codes & 31)) return false;
+    if (!c || !c->codes || !c->scales || ((uintptr_t)c->codes & 15)) return false;
     if (c->d < 64 || c->d > DSV4B_KVQ_MAX_D || (c->d & 63) || c->tail < 0 || c->tail > c->d || (c->tail & 63)) return false;
     if (c->page_rows < 1 || c->page_rows > 65536 || (c->page_rows & (c->page_rows - 1))) return false;
     return c->n_pages > 0 && c->n_pages <= 0x7fffffffL;

@@ -162,9 +162,12 @@ __device__ __forceinline__ void tmem_wait_ld(float (&v)[N])
 #pragma unroll
     for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r)
+// 32 columns of 16 lanes: thread 4r + q holds, for i < 4, columns 8i + 2q and
+// 8i + 2q + 1 of lane r in registers 4i and 4i + 1 and those of lane r + 8 in
+// registers 4i + 2 and 4i + 3.
+__device__ __forceinline__ void tmem_st_16x256(uint32_t addr, const uint32_t (&r)[16])
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 // 32 columns, as words.

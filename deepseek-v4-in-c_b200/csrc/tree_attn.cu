@@ -33,10 +33,10 @@
 //
 // A block takes one tile of rows and a run of 128-key tiles, cut into chunk
 // pairs of 128 elements:
-//   8 widening warps thread = one key and every other 64-element chunk: read
-//                    its codes (64 bytes; one chunk in flight while one is widened), widen e4m3
-//                    to f16 -- exact, the row scale stays outside -- into a
-//                    TMEM ring of 3 or 4 pairs;
+//   8 widening warps four threads to a key: read the codes (64-byte runs, one
+//                    pair in flight while one is widened), widen e4m3 to f16
+//                    -- exact, the row scale stays outside -- into a TMEM
+//                    ring of 3 or 4 pairs;
 //   8 copying warps  from there to shared memory once the second product has
 //                    freed the pair's place (128-byte swizzle; V^T is the
 //                    same bytes, M-major);
@@ -95,6 +95,7 @@ struct Shared {             // behind the operand tiles
     float cq[TA_ROWS], nm[TA_ROWS];     // score factor of a row, and its negated reference
     float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
     int wk[TA_SOFT];
+    float scale[2];         // 2^E of each half of the rows
     uint32_t tmem;
     int dead;
 };
@@ -142,19 +143,15 @@ __device__ __forceinline__ bool soft_any(bool p, int wg)
 }
 __device__ __forceinline__ void soft_sync(int wg) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(wg + 1) : "memory"); }
 
-// 64 bytes of a row.
+// A widening thread's codes of a chunk pair (16 of each chunk for two keys),
+// and the two rows.
 struct Unit {
     uint32_t w[16];
-    const unsigned char *src;
+    const unsigned char *r0, *r1;
 };
-__device__ __forceinline__ void ld64(Unit &u)
+__device__ __forceinline__ void ld16(uint32_t *w, const unsigned char *p)
 {
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(u.w[8 * i]), "=r"(u.w[8 * i + 1]), "=r"(u.w[8 * i + 2]), "=r"(u.w[8 * i + 3]),
-                       "=r"(u.w[8 * i + 4]), "=r"(u.w[8 * i + 5]), "=r"(u.w[8 * i + 6]), "=r"(u.w[8 * i + 7])
-                     : "l"(u.src + 32 * i));
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
 }
 
 __device__ __forceinline__ uint32_t e4m3x2_f16(uint32_t v)
@@ -164,6 +161,10 @@ __device__ __forceinline__ uint32_t e4m3x2_f16(uint32_t v)
     return r;
 }
 
+__device__ __forceinline__ void st_smem8(uint32_t a, uint32_t x, uint32_t y)
+{
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void st_smem16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -177,6 +178,86 @@ __device__ __forceinline__ void warp_arrive(const uint64_t *bar, int lane)
 {
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(tc::smem_u32(bar));
+}
+
+// q rows to f16 for warp w of the 16 that share the work: one warp a row,
+// scaled so that the largest magnitude lies in [2^14, 2^15) (f16 rows are
+// taken as they are).
+template <int NR>
+__device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t q_s, int r0, int nr, int b, int w, int lane)
+{
+    const int H = a.n_heads, d = a.c.d;
+#pragma unroll 1
+    for (int r = w; r < NR; r += TA_SOFT + TA_COPY) {
+        const int t = (r0 + r) / H;
+        const unsigned short *q = reinterpret_cast<const unsigned short *>(a.q) +
+                                  ((size_t)b * a.n_tok + t) * a.q_tok + (size_t)(r0 + r - t * H) * d;
+        uint4 v[3];
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            const int e = i * 256 + lane * 8;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (r < nr && e < d) v[i] = __ldcg(reinterpret_cast<const uint4 *>(q + e));
+        }
+        int kq = 0;
+        if (a.dt == DSV4B_BF16) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+                const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t lo = u[k] & 0x7FFFu, hi = (u[k] >> 16) & 0x7FFFu;
+                    if (lo < 0x7F80u) top = max(top, lo);
+                    if (hi < 0x7F80u) top = max(top, hi);
+                }
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (top) kq = max((int)(top >> 7) - 127 - 14, -112);
+            const float f = pow2i(-kq);
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+                uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float2 x = bf16x2(u[k]);
+                    u[k] = pack2<DSV4B_F16>(x.x * f, x.y * f);
+                }
+                v[i] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
+        const uint32_t dst = q_s + r * 128;
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            const int e = i * 256 + lane * 8;
+            if (e >= d) continue;
+            // elements 16 q + 4 i go to place 16 i + 4 q of the chunk
+            const uint32_t chunk = dst + (e >> 6) * (NR * 128), q4 = (e >> 4) & 3, i4 = (e >> 2) & 3, sw = (r & 7) << 4;
+            st_smem8(chunk + ((32 * i4 + 8 * q4) ^ sw), v[i].x, v[i].y);
+            st_smem8(chunk + ((32 * (i4 + 1) + 8 * q4) ^ sw), v[i].z, v[i].w);
+        }
+        if (lane == 0) sh.cq[r] = a.scale * 1.4426950408889634f * pow2i(kq);
+    }
+}
+
+// Combine N values per lane over the 32 lanes of a warp: lane i gets the
+// result of value i (N <= 32), by halving exchanges.
+template <int N, typename F>
+__device__ __forceinline__ float across(const float (&x)[N], float none, int lane, F op)
+{
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = i < N ? x[i < N ? i : 0] : none;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; i++) {
+            const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+            v[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, o));
+        }
+    }
+    return v[0];
 }
 
 template <int NR>
@@ -218,7 +299,7 @@ k_tree_attn(const __grid_constant__ Args g)
             tc::mbar_init(tc::smem_u32(&sh.k_full[r]), TA_LOAD);
             tc::mbar_init(tc::smem_u32(&sh.k_done[r]), 1 + TA_COPY);
         }
-        tc::mbar_init(tc::smem_u32(&sh.q_full), TA_SOFT);
+        tc::mbar_init(tc::smem_u32(&sh.q_full), TA_SOFT + TA_COPY);
         tc::mbar_init(tc::smem_u32(&sh.s_full), 1);
         tc::mbar_init(tc::smem_u32(&sh.s_free), TA_SOFT);
         tc::mbar_init(tc::smem_u32(&sh.p_full), TA_SOFT);
@@ -237,72 +318,103 @@ k_tree_attn(const __grid_constant__ Args g)
     if (warp >= TA_SOFT && warp < TA_WCOPY) {
         // --------------------------------------------------------- widening
         tc::reg_dec<TA_REG_LOAD>();
-        const int quad = warp & 3, half = (warp - TA_SOFT) >> 2, key = quad * 32 + lane;
+        // Four lanes share a key: lane 4r + q holds elements 16q .. 16q + 15 of
+        // a chunk for keys r and r + 8 of the warp's 16, so that a load reads
+        // whole 64-byte runs of 8 rows (with a key per lane it took 4 times
+        // the shared-memory cycles). The 16x256b store puts them 4 elements at
+        // a time at places 16 i + 4 q of the chunk, i < 4: TMEM holds each
+        // chunk in that order, which q follows and the copy undoes.
+        const int lane0 = (warp & 3) * 32 + ((warp - TA_SOFT) >> 2) * 16, q4 = lane & 3;
         const int ndq = (d - a.c.tail) >> 6, shift = g.page_shift, rm = a.c.page_rows - 1;
         const int *pages = a.pages + (size_t)b * a.max_pages;
         const int row_bytes = d + a.c.tail;
-        int pos = tb * TA_KEYS + key;                   // of the next row to look up
+        int pos = tb * TA_KEYS + lane0 + (lane >> 2);   // of the next rows to look up
         auto page_at = [&](int q) { return q < n ? __ldcg(pages + (q >> shift)) : -1; };
-        int pg = page_at(pos);
-        const unsigned char *row;
-        auto next_row = [&]() {
-            row = (unsigned)pg < (unsigned)a.c.n_pages
-                      ? reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (pos & rm)) * row_bytes
-                      : g_zero_row;
-            pos += TA_KEYS;
-            pg = page_at(pos);
+        auto row_at = [&](int pg, int q) {
+            return (unsigned)pg < (unsigned)a.c.n_pages
+                       ? reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (q & rm)) * row_bytes
+                       : g_zero_row;
         };
-        next_row();
-        int fc = half, left = half < nch ? nt : 0;      // chunk to fetch; tiles left
-        auto fetch = [&](Unit &u) {
+        int pg0 = page_at(pos), pg1 = page_at(pos + 8);
+        const unsigned char *row0, *row1;
+        auto next_rows = [&]() {
+            row0 = row_at(pg0, pos);
+            row1 = row_at(pg1, pos + 8);
+            pos += TA_KEYS;
+            pg0 = page_at(pos);
+            pg1 = page_at(pos + 8);
+        };
+        next_rows();
+        Unit u;
+        int fp = 0, left = nt;                          // pair to fetch; tiles left
+        auto fetch = [&]() {
             if (left == 0) return;
-            u.src = row + (fc < ndq ? fc * 64 : fc * 128 - ndq * 64);
-            ld64(u);
-            fc += 2;
-            if (fc >= nch) {
-                fc = half;
+            u.r0 = row0 + 16 * q4;
+            u.r1 = row1 + 16 * q4;
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+                if (2 * fp + s < ndq) {
+                    ld16(u.w + 8 * s, u.r0 + (2 * fp + s) * 64);
+                    ld16(u.w + 8 * s + 4, u.r1 + (2 * fp + s) * 64);
+                }
+            if (++fp == npair) {
+                fp = 0;
                 left--;
-                next_row();
+                next_rows();
             }
         };
-        const uint32_t k_mine = tmem + ((uint32_t)quad << 21) + k_col + 32 * half;
+        const uint32_t k_mine = tmem + ((uint32_t)lane0 << 16) + k_col;
         const int pairs = nt * npair;
-        int slot = 0, par = 1, c = half;                // ring place, parity of its last use, chunk
-        Unit u;
-        fetch(u);
+        int slot = 0, par = 1, p = 0;                   // ring place, parity of its last use, pair of the tile
+        fetch();
         for (int i = 0; i < pairs; i++) {
             const uint32_t dst = k_mine + 64 * slot;
             if (i >= KR) warp_wait(&sh.k_done[slot], par, dead);
             tc::fence_after();
-            if (c < ndq) {
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    uint32_t h[16];
+            for (int s = 0; s < 2; s++) {
+                const int c = 2 * p + s;
+                uint32_t h[16];
+                if (c < ndq) {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        h[2 * k] = e4m3x2_f16(u.w[8 * s + k] & 0xFFFFu);
-                        h[2 * k + 1] = e4m3x2_f16(u.w[8 * s + k] >> 16);
+                    for (int k = 0; k < 4; k++) {
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            h[4 * k + 2 * r] = e4m3x2_f16(u.w[8 * s + 4 * r + k] & 0xFFFFu);
+                            h[4 * k + 2 * r + 1] = e4m3x2_f16(u.w[8 * s + 4 * r + k] >> 16);
+                        }
                     }
-                    tc::tmem_st16(dst + 16 * s, h);
+                    tc::tmem_st_16x256(dst + 32 * s, h);
+                } else if (c < nch) {
+                    const int at = ndq * 64 + (c - ndq) * 128 + 16 * q4;
+                    uint32_t t[16];
+                    ld16(t, u.r0 + at);
+                    ld16(t + 4, u.r0 + at + 16);
+                    ld16(t + 8, u.r1 + at);
+                    ld16(t + 12, u.r1 + at + 16);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            h[4 * k + 2 * r] = t[8 * r + 2 * k];
+                            h[4 * k + 2 * r + 1] = t[8 * r + 2 * k + 1];
+                        }
+                    tc::tmem_st_16x256(dst + 32 * s, h);
                 }
-                fetch(u);
-            } else if (c < nch) {
-                tc::tmem_st16(dst, u.w);
-                u.src += 64;
-                ld64(u);
-                tc::tmem_st16(dst + 16, u.w);
-                fetch(u);
             }
+            fetch();
             tc::tmem_wait_st();
             tc::fence_before();
             warp_arrive(&sh.k_full[slot], lane);
-            c += 2;
-            if (c >= 2 * npair) c = half;
+            if (++p == npair) p = 0;
             if (++slot == KR) slot = 0, par ^= 1;
         }
     } else if (warp >= TA_WCOPY && warp < TA_WMMA) {
         // ---------------------------------------------------------- copying
         tc::reg_dec<TA_REG_COPY>();
+        widen_q<NR>(a, sh, q_s, r0, nr, b, TA_SOFT + warp - TA_WCOPY, lane);
+        tc::fence_async_smem();
+        warp_arrive(&sh.q_full, lane);
         const int quad = warp & 3, half = (warp - TA_WCOPY) >> 2, key = quad * 32 + lane;
         const uint32_t k_mine = tmem + ((uint32_t)quad << 21) + k_col + 32 * half, sw = key & 7;
         const int pairs = nt * npair;
@@ -322,8 +434,10 @@ k_tree_attn(const __grid_constant__ Args g)
             if (c < nch) {
                 const uint32_t dst = kv_s + (stage * nch + c) * TA_SLOT + key * 128;
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    st_smem16(dst + ((k ^ sw) << 4), h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+                for (int k = 0; k < 8; k++) {           // elements 8k .. 8k + 7 are at places 32 (k % 2) + 4 (k / 2)
+                    const int r = 16 * (k & 1) + 2 * (k >> 1);
+                    st_smem16(dst + ((k ^ sw) << 4), h[r], h[r + 1], h[r + 8], h[r + 9]);
+                }
                 tc::fence_async_smem();
             }
             warp_arrive(&sh.v_full[stage * TA_PAIRS + p], lane);
@@ -403,71 +517,12 @@ k_tree_attn(const __grid_constant__ Args g)
         tc::reg_inc<TA_REG_SOFT>();
         const int wg = warp >> 2, key = (warp & 3) * 32 + lane, c0 = wg * NC;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        // q rows to f16, one warp a row, two in flight: scaled so that the
-        // largest magnitude lies in [2^14, 2^15) (f16 rows are taken as they
-        // are)
-#pragma unroll 1
-        for (int r1 = warp; r1 < NR; r1 += 2 * TA_SOFT) {
-            uint4 w[2][3];
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                const int r = r1 + s * TA_SOFT, t = (r0 + r) / H;
-                const unsigned short *q = reinterpret_cast<const unsigned short *>(a.q) +
-                                          ((size_t)b * a.n_tok + t) * a.q_tok + (size_t)(r0 + r - t * H) * d;
-#pragma unroll
-                for (int i = 0; i < 3; i++) {
-                    const int e = i * 256 + lane * 8;
-                    w[s][i] = make_uint4(0, 0, 0, 0);
-                    if (r < nr && e < d) w[s][i] = __ldcg(reinterpret_cast<const uint4 *>(q + e));
-                }
-                if (lane == 0 && r < NR) {
-                    sh.out_at[r] = ((uint64_t)b * a.n_tok + t) * a.o_tok + (uint64_t)(r0 + r - t * H) * d;
-                    sh.rowmask[r] = r < nr ? __ldcg(a.mask + (size_t)b * a.n_tok + t) : 0ull;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                const int r = r1 + s * TA_SOFT;
-                if (r >= NR) break;
-                int kq = 0;
-                if (a.dt == DSV4B_BF16) {
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int i = 0; i < 3; i++) {
-                        const uint32_t u[4] = {w[s][i].x, w[s][i].y, w[s][i].z, w[s][i].w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t lo = u[k] & 0x7FFFu, hi = (u[k] >> 16) & 0x7FFFu;
-                            if (lo < 0x7F80u) top = max(top, lo);
-                            if (hi < 0x7F80u) top = max(top, hi);
-                        }
-                    }
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    if (top) kq = max((int)(top >> 7) - 127 - 14, -112);
-                    const float f = pow2i(-kq);
-#pragma unroll
-                    for (int i = 0; i < 3; i++) {
-                        uint32_t u[4] = {w[s][i].x, w[s][i].y, w[s][i].z, w[s][i].w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const float2 v = bf16x2(u[k]);
-                            u[k] = pack2<DSV4B_F16>(v.x * f, v.y * f);
-                        }
-                        w[s][i] = make_uint4(u[0], u[1], u[2], u[3]);
-                    }
-                }
-                const uint32_t dst = q_s + r * 128;
-#pragma unroll
-                for (int i = 0; i < 3; i++) {
-                    const int e = i * 256 + lane * 8;
-                    if (e < d)
-                        st_smem16(dst + (e >> 6) * (NR * 128) + ((((e >> 3) & 7) ^ (r & 7)) << 4), w[s][i].x, w[s][i].y, w[s][i].z, w[s][i].w);
-                }
-                if (lane == 0) {
-                    sh.cq[r] = a.scale * 1.4426950408889634f * pow2i(kq);
-                    sh.nm[r] = INFINITY;
-                }
-            }
+        widen_q<NR>(a, sh, q_s, r0, nr, b, warp, lane);
+        if (tid < NR) {
+            const int r = tid, t = (r0 + r) / H;
+            sh.nm[r] = INFINITY;
+            sh.out_at[r] = ((uint64_t)b * a.n_tok + t) * a.o_tok + (uint64_t)(r0 + r - t * H) * d;
+            sh.rowmask[r] = r < nr ? __ldcg(a.mask + (size_t)b * a.n_tok + t) : 0ull;
         }
         tc::fence_async_smem();
         warp_arrive(&sh.q_full, lane);
@@ -540,18 +595,12 @@ k_tree_attn(const __grid_constant__ Args g)
             load();
             const bool raise = over > TA_RAISE || (valid && kx < 255 && kx - E > 7);
             if (soft_any(raise, wg)) {
-                // raise the references: the rows' maxima over the tile, as
-                // integers of the same order (a NaN has none)
+                // raise the references: the rows' maxima over the tile (fmaxf
+                // takes no NaN)
                 scores(false);
                 free_s();
-                int mine = 0;
-#pragma unroll
-                for (int i = 0; i < NC; i++) {
-                    const int k = __float_as_int(x[i] == x[i] ? x[i] : -INFINITY);
-                    const int top = __reduce_max_sync(0xffffffffu, k ^ ((k >> 31) & 0x7FFFFFFF));
-                    if (lane == i) mine = top ^ ((top >> 31) & 0x7FFFFFFF);
-                }
-                if (lane < NC) sh.wmax[warp & 3][c0 + lane] = __int_as_float(mine);
+                const float mine = across<NC>(x, -INFINITY, lane, [](float p, float q) { return fmaxf(p, q); });
+                if (lane < NC) sh.wmax[warp & 3][c0 + lane] = fmaxf(mine, -INFINITY);
                 const int kw = __reduce_max_sync(0xffffffffu, valid && kx < 255 ? kx : TA_NONE);
                 if (lane == 0) sh.wk[warp] = kw;
                 soft_sync(wg);
@@ -613,21 +662,9 @@ k_tree_attn(const __grid_constant__ Args g)
             if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.p_full));
             kx = kx_next;
         }
-        // row sums: the warp's 32 keys by halving exchanges (lane = row), then
-        // the four warps
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; i++) v[i] = i < NC ? l[i < NC ? i : 0] : 0.0f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const bool up = lane & o;
-#pragma unroll
-            for (int i = 0; i < o; i++) {
-                const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
-                v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-            }
-        }
-        if (lane < NC) sh.lsum[warp & 3][c0 + lane] = v[0];
+        // row sums: the warp's 32 keys (lane = row), then the four warps
+        const float mine = across<NC>(l, 0.0f, lane, [](float p, float q) { return p + q; });
+        if (lane < NC) sh.lsum[warp & 3][c0 + lane] = mine;
         soft_sync(wg);
         warp_wait(&sh.pv_done, (nt - 1) & 1, dead);
         tc::fence_after();
@@ -643,31 +680,44 @@ k_tree_attn(const __grid_constant__ Args g)
             // the row scales' reference goes with it; 0 where nothing was seen
             sh.fo[r] = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / den;
         }
-        soft_sync(wg);
-        const float s = E == TA_NONE ? 0.0f : e8m0((uint8_t)E);
+        if (key == 0) sh.scale[wg] = E == TA_NONE ? 0.0f : e8m0((uint8_t)E);
+        tc::fence_before();
+    }
+    __syncthreads();
+    tc::fence_after();
+    // O out of TMEM by six groups of four warps, 16 rows at a time: lane = an
+    // element of the output
+    if (warp < TA_WMMA) {
+        const int key = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        constexpr int NQ = NR / 16;
 #pragma unroll 1
-        for (int p = 0; p < nblk; p++) {
-            const int e = p * 128 + key;
-            float x[NC];
-#pragma unroll
-            for (int i = 0; i < NC; i += 8) tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + i, x + i);
+        for (int w = warp >> 2; w < npair * NQ; w += TA_WMMA / 4) {
+            const int p = w / NQ, c0 = (w - p * NQ) * 16, e = p * 128 + key;
+            if (c0 >= nr) continue;
+            float x[16];
+            tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0, x);
+            tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + 8, x + 8);
             tc::tmem_wait_ld(x);
             if (e >= d) continue;
+            const float s0 = sh.scale[c0 >= NC], s1 = sh.scale[c0 + 8 >= NC];
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = x[i] * sh.fo[c0 + i] * (i < 8 ? s0 : s1);
             if (g.nsplit > 1) {
                 float *o = g.part.o + (prow + c0) * d + e;
 #pragma unroll
-                for (int i = 0; i < NC; i++) {
-                    if (c0 + i < nr) *o = x[i] * sh.fo[c0 + i] * s;
+                for (int i = 0; i < 16; i++) {
+                    if (c0 + i < nr) *o = x[i];
                     o += d;
                 }
             } else if (a.dt == DSV4B_BF16) {
 #pragma unroll
-                for (int i = 0; i < NC; i++)
-                    if (c0 + i < nr) st_row1<DSV4B_BF16>(a.o, sh.out_at[c0 + i] + e, x[i] * sh.fo[c0 + i] * s);
+                for (int i = 0; i < 16; i++)
+                    if (c0 + i < nr) st_row1<DSV4B_BF16>(a.o, sh.out_at[c0 + i] + e, x[i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < NC; i++)
-                    if (c0 + i < nr) st_row1<DSV4B_F16>(a.o, sh.out_at[c0 + i] + e, x[i] * sh.fo[c0 + i] * s);
+                for (int i = 0; i < 16; i++)
+                    if (c0 + i < nr) st_row1<DSV4B_F16>(a.o, sh.out_at[c0 + i] + e, x[i]);
             }
         }
         tc::fence_before();

@@ -393,7 +393,7 @@ int dsv4b_rope(void *out, int out_dt, long out_tok, long out_head, const void *x
                int first, int inverse, void *stream);
 
 /* A paged cache of quantised rows in the caller's device memory: codes
- * [n_pages][page_rows][d + tail] bytes (32-byte aligned), scales
+ * [n_pages][page_rows][d + tail] bytes (16-byte aligned), scales
  * [n_pages][page_rows] bytes. Row = d - tail e4m3 codes, then `tail` f16
  * values; element = code * 2^(scale byte - 127). d a multiple of 64 up to
  * DSV4B_KVQ_MAX_D, tail a multiple of 64 (0 .. d), page_rows a power of two.

@@ -33,14 +33,15 @@
 //
 // A block takes one tile of rows and a run of 128-key tiles, cut into chunk
 // pairs of 128 elements:
-//   8 widening warps four threads to a key: read the codes (64-byte runs, one
-//                    pair in flight while one is widened), widen e4m3 to f16
+//   8 widening warps four threads to a key: read the codes (64-byte runs, two
+//                    pairs in flight), widen e4m3 to f16
 //                    -- exact, the row scale stays outside -- into a TMEM
 //                    ring of 3 or 4 pairs;
 //   8 copying warps  from there to shared memory once the second product has
 //                    freed the pair's place (128-byte swizzle; V^T is the
 //                    same bytes, M-major);
 //   2 MMA warps      one issues S pair by pair, one O;
+//   2 look-up warps  the next tile's row scales;
 //   8 softmax warps  thread = one key and half of the rows.
 //
 // Numbers. With s_j = 2^e_j the row scale, score = S (scale 2^e_j) in float
@@ -67,7 +68,7 @@ constexpr int TA_WCOPY = TA_SOFT + TA_LOAD, TA_WMMA = TA_WCOPY + TA_COPY;   // t
 constexpr int TA_T = 32 * (TA_WMMA + 4);
 // registers: 896 threads are launched with 72 each; the other warpgroups give
 // theirs to the softmax ones
-constexpr int TA_REG_SOFT = 128, TA_REG_LOAD = 64, TA_REG_COPY = 48, TA_REG_MMA = 24;
+constexpr int TA_REG_SOFT = 112, TA_REG_LOAD = 72, TA_REG_COPY = 48, TA_REG_MMA = 40;
 static_assert(2 * (TA_REG_SOFT + TA_REG_LOAD + TA_REG_COPY) + TA_REG_MMA <= 7 * 72, "more registers than the block is launched with");
 constexpr int TA_ROWS = 64;                         // most rows of a tile (N)
 constexpr int TA_STAGES = 4, TA_PAIRS = 5;
@@ -90,11 +91,11 @@ struct Args {
 
 struct Shared {             // behind the operand tiles
     uint64_t v_full[TA_STAGES * TA_PAIRS], v_empty[TA_STAGES * TA_PAIRS], k_full[TA_RING], k_done[TA_RING];
-    uint64_t q_full, s_full, s_free, p_full, pv_done;
+    uint64_t q_full, key_full, s_full, s_free, p_full, pv_done;
     uint64_t rowmask[TA_ROWS], out_at[TA_ROWS];     // a row's tree mask, and its first output element
     float cq[TA_ROWS], nm[TA_ROWS];     // score factor of a row, and its negated reference
     float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
-    int wk[TA_SOFT];
+    int wk[TA_SOFT], kx[TA_KEYS];       // (raises); scale byte of each key of the tile, -1: not there
     float scale[2];         // 2^E of each half of the rows
     uint32_t tmem;
     int dead;
@@ -146,9 +147,9 @@ __device__ __forceinline__ void soft_sync(int wg) { asm volatile("barrier.cta.sy
 // A widening thread's codes of a chunk pair (16 of each chunk for two keys),
 // and the two rows.
 struct Unit {
-    uint32_t w[16];
-    const unsigned char *r0, *r1;
+    uint32_t w[16], r0, r1;         // rows as 64-byte steps from the cache's start; TA_NOROW
 };
+constexpr uint32_t TA_NOROW = 0xFFFFFFFFu;
 __device__ __forceinline__ void ld16(uint32_t *w, const unsigned char *p)
 {
     asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
@@ -201,27 +202,32 @@ __device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t 
         }
         int kq = 0;
         if (a.dt == DSV4B_BF16) {
-            uint32_t top = 0;
+            uint32_t top2 = 0;          // magnitudes order as 16-bit integers
 #pragma unroll
             for (int i = 0; i < 3; i++) {
-                const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const uint32_t lo = u[k] & 0x7FFFu, hi = (u[k] >> 16) & 0x7FFFu;
-                    if (lo < 0x7F80u) top = max(top, lo);
-                    if (hi < 0x7F80u) top = max(top, hi);
-                }
+                if (i * 256 >= d) break;
+                top2 = __vmaxs2(top2, __vmaxs2(__vmaxs2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu), __vmaxs2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
             }
-            top = __reduce_max_sync(0xffffffffu, top);
+            uint32_t top = __reduce_max_sync(0xffffffffu, max(top2 & 0xFFFFu, top2 >> 16));
+            if (top >= 0x7F80u) {       // infinities and NaN set no scale
+                top = 0;
+#pragma unroll 1
+                for (int i = 0; i < d / 32; i++) {
+                    const uint32_t m = r < nr ? __ldcg(q + i * 32 + lane) & 0x7FFFu : 0u;
+                    if (m < 0x7F80u) top = max(top, m);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+            }
             if (top) kq = max((int)(top >> 7) - 127 - 14, -112);
             const float f = pow2i(-kq);
 #pragma unroll
             for (int i = 0; i < 3; i++) {
+                if (i * 256 >= d) break;
                 uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const float2 x = bf16x2(u[k]);
-                    u[k] = pack2<DSV4B_F16>(x.x * f, x.y * f);
+                    const float2 x = mul2(bf16x2(u[k]), make_float2(f, f));
+                    u[k] = pack2<DSV4B_F16>(x.x, x.y);
                 }
                 v[i] = make_uint4(u[0], u[1], u[2], u[3]);
             }
@@ -300,6 +306,7 @@ k_tree_attn(const __grid_constant__ Args g)
             tc::mbar_init(tc::smem_u32(&sh.k_done[r]), 1 + TA_COPY);
         }
         tc::mbar_init(tc::smem_u32(&sh.q_full), TA_SOFT + TA_COPY);
+        tc::mbar_init(tc::smem_u32(&sh.key_full), 2);
         tc::mbar_init(tc::smem_u32(&sh.s_full), 1);
         tc::mbar_init(tc::smem_u32(&sh.s_free), TA_SOFT);
         tc::mbar_init(tc::smem_u32(&sh.p_full), TA_SOFT);
@@ -317,7 +324,6 @@ k_tree_attn(const __grid_constant__ Args g)
 
     if (warp >= TA_SOFT && warp < TA_WCOPY) {
         // --------------------------------------------------------- widening
-        tc::reg_dec<TA_REG_LOAD>();
         // Four lanes share a key: lane 4r + q holds elements 16q .. 16q + 15 of
         // a chunk for keys r and r + 8 of the warp's 16, so that a load reads
         // whole 64-byte runs of 8 rows (with a key per lane it took 4 times
@@ -327,16 +333,17 @@ k_tree_attn(const __grid_constant__ Args g)
         const int lane0 = (warp & 3) * 32 + ((warp - TA_SOFT) >> 2) * 16, q4 = lane & 3;
         const int ndq = (d - a.c.tail) >> 6, shift = g.page_shift, rm = a.c.page_rows - 1;
         const int *pages = a.pages + (size_t)b * a.max_pages;
-        const int row_bytes = d + a.c.tail;
+        const uint32_t row_steps = (d + a.c.tail) >> 6;
         int pos = tb * TA_KEYS + lane0 + (lane >> 2);   // of the next rows to look up
         auto page_at = [&](int q) { return q < n ? __ldcg(pages + (q >> shift)) : -1; };
         auto row_at = [&](int pg, int q) {
-            return (unsigned)pg < (unsigned)a.c.n_pages
-                       ? reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (q & rm)) * row_bytes
-                       : g_zero_row;
+            return (unsigned)pg < (unsigned)a.c.n_pages ? (uint32_t)((((size_t)pg << shift) + (q & rm)) * row_steps) : TA_NOROW;
+        };
+        auto at_row = [&](uint32_t r) {
+            return (r == TA_NOROW ? g_zero_row : reinterpret_cast<const unsigned char *>(a.c.codes) + ((size_t)r << 6)) + 16 * q4;
         };
         int pg0 = page_at(pos), pg1 = page_at(pos + 8);
-        const unsigned char *row0, *row1;
+        uint32_t row0, row1;
         auto next_rows = [&]() {
             row0 = row_at(pg0, pos);
             row1 = row_at(pg1, pos + 8);
@@ -345,18 +352,18 @@ k_tree_attn(const __grid_constant__ Args g)
             pg1 = page_at(pos + 8);
         };
         next_rows();
-        Unit u;
         int fp = 0, left = nt;                          // pair to fetch; tiles left
-        auto fetch = [&]() {
+        auto fetch = [&](Unit &u) {
             if (left == 0) return;
-            u.r0 = row0 + 16 * q4;
-            u.r1 = row1 + 16 * q4;
+            u.r0 = row0;
+            u.r1 = row1;
 #pragma unroll
-            for (int s = 0; s < 2; s++)
-                if (2 * fp + s < ndq) {
-                    ld16(u.w + 8 * s, u.r0 + (2 * fp + s) * 64);
-                    ld16(u.w + 8 * s + 4, u.r1 + (2 * fp + s) * 64);
-                }
+            for (int r = 0; r < 2; r++) {
+                const unsigned char *at = at_row(r ? row1 : row0) + 128 * fp;
+#pragma unroll
+                for (int s = 0; s < 2; s++)
+                    if (2 * fp + s < ndq) ld16(u.w + 8 * s + 4 * r, at + 64 * s);
+            }
             if (++fp == npair) {
                 fp = 0;
                 left--;
@@ -366,8 +373,8 @@ k_tree_attn(const __grid_constant__ Args g)
         const uint32_t k_mine = tmem + ((uint32_t)lane0 << 16) + k_col;
         const int pairs = nt * npair;
         int slot = 0, par = 1, p = 0;                   // ring place, parity of its last use, pair of the tile
-        fetch();
-        for (int i = 0; i < pairs; i++) {
+        int i = 0;
+        auto put = [&](Unit &u) {
             const uint32_t dst = k_mine + 64 * slot;
             if (i >= KR) warp_wait(&sh.k_done[slot], par, dead);
             tc::fence_after();
@@ -386,28 +393,36 @@ k_tree_attn(const __grid_constant__ Args g)
                     }
                     tc::tmem_st_16x256(dst + 32 * s, h);
                 } else if (c < nch) {
-                    const int at = ndq * 64 + (c - ndq) * 128 + 16 * q4;
-                    uint32_t t[16];
-                    ld16(t, u.r0 + at);
-                    ld16(t + 4, u.r0 + at + 16);
-                    ld16(t + 8, u.r1 + at);
-                    ld16(t + 12, u.r1 + at + 16);
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
+                    for (int r = 0; r < 2; r++) {
+                        const unsigned char *at = at_row(r ? u.r1 : u.r0) + ndq * 64 + (c - ndq) * 128 + 16 * q4;
 #pragma unroll
-                        for (int r = 0; r < 2; r++) {
-                            h[4 * k + 2 * r] = t[8 * r + 2 * k];
-                            h[4 * k + 2 * r + 1] = t[8 * r + 2 * k + 1];
+                        for (int k = 0; k < 2; k++) {
+                            uint32_t t[4];
+                            ld16(t, at + 16 * k);
+                            h[8 * k + 2 * r] = t[0], h[8 * k + 2 * r + 1] = t[1];
+                            h[8 * k + 4 + 2 * r] = t[2], h[8 * k + 4 + 2 * r + 1] = t[3];
                         }
+                    }
                     tc::tmem_st_16x256(dst + 32 * s, h);
                 }
             }
-            fetch();
+            fetch(u);
             tc::tmem_wait_st();
             tc::fence_before();
             warp_arrive(&sh.k_full[slot], lane);
+            i++;
             if (++p == npair) p = 0;
             if (++slot == KR) slot = 0, par ^= 1;
+        };
+        // two pairs in flight, in registers of their own: a copy between them
+        // would wait for the load
+        Unit u0, u1;
+        fetch(u0);
+        fetch(u1);
+        while (i < pairs) {
+            put(u0);
+            if (i < pairs) put(u1);
         }
     } else if (warp >= TA_WCOPY && warp < TA_WMMA) {
         // ---------------------------------------------------------- copying
@@ -506,6 +521,46 @@ k_tree_attn(const __grid_constant__ Args g)
                 }
             }
         }
+        if (warp > TA_WMMA + 1) {
+            // Two warps look up, for the softmax, the scale bytes of each tile's
+            // rows, and ask the L2 for the rows two tiles ahead. A tile's
+            // loads are all sent before any is used.
+            const int key = (warp - TA_WMMA - 2) * 64 + lane, shift = g.page_shift, rm = a.c.page_rows - 1;
+            const int *pages = a.pages + (size_t)b * a.max_pages;
+            int pos = tb * TA_KEYS + key;               // of tile j, key 0 of the thread's two
+            auto page_at = [&](int q) { return q < n ? __ldcg(pages + (q >> shift)) : -1; };
+            auto scale_at = [&](int pg, int q) {
+                return (unsigned)pg < (unsigned)a.c.n_pages
+                           ? (int)__ldcg(reinterpret_cast<const unsigned char *>(a.c.scales) + ((size_t)pg << shift) + (q & rm))
+                           : -1;
+            };
+            auto ask = [&](int pg, int q) {
+                if ((unsigned)pg < (unsigned)a.c.n_pages)
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                        reinterpret_cast<const unsigned char *>(a.c.codes) + (((size_t)pg << shift) + (q & rm)) * (d + a.c.tail)),
+                        "r"(d + a.c.tail));
+            };
+            int pa = page_at(pos), pb = page_at(pos + 32);
+            int pa1 = page_at(pos + TA_KEYS), pb1 = page_at(pos + TA_KEYS + 32);
+            int ka = scale_at(pa, pos), kb = scale_at(pb, pos + 32);
+            pa = page_at(pos + 2 * TA_KEYS);
+            pb = page_at(pos + 2 * TA_KEYS + 32);
+            for (int j = 0; j < nt; j++) {              // pa1, pb1: tile j + 1; pa, pb: tile j + 2
+                const int ka1 = scale_at(pa1, pos + TA_KEYS), kb1 = scale_at(pb1, pos + TA_KEYS + 32);
+                if (j + 2 < nt) {
+                    ask(pa, pos + 2 * TA_KEYS);
+                    ask(pb, pos + 2 * TA_KEYS + 32);
+                }
+                pa1 = pa, pb1 = pb;
+                pa = page_at(pos + 3 * TA_KEYS), pb = page_at(pos + 3 * TA_KEYS + 32);
+                if (j > 0) warp_wait(&sh.s_free, (j - 1) & 1, dead);
+                sh.kx[key] = ka;
+                sh.kx[key + 32] = kb;
+                warp_arrive(&sh.key_full, lane);
+                ka = ka1, kb = kb1;
+                pos += TA_KEYS;
+            }
+        }
         if (warp <= TA_WMMA + 1) {
             if (*dead) {        // let what was issued finish before TMEM is freed
                 const uint64_t t0 = tc::now_ns();
@@ -527,26 +582,13 @@ k_tree_attn(const __grid_constant__ Args g)
         tc::fence_async_smem();
         warp_arrive(&sh.q_full, lane);
         warp_wait(&sh.q_full, 0, dead);
-        const int shift = g.page_shift, rm = a.c.page_rows - 1;
-        const int *pages = a.pages + (size_t)b * a.max_pages;
-        const unsigned char *scales = reinterpret_cast<const unsigned char *>(a.c.scales);
-        auto page_of = [&](int j) {
-            const int pos = (tb + j) * TA_KEYS + key;
-            return j < nt && pos < n ? __ldcg(pages + (pos >> shift)) : -1;
-        };
-        auto scale_of = [&](int j, int pg) -> int {     // E8M0 byte of the key's row, -1: not there
-            const int pos = (tb + j) * TA_KEYS + key;
-            if ((unsigned)pg >= (unsigned)a.c.n_pages) return -1;
-            return __ldcg(scales + ((size_t)pg << shift) + (pos & rm));
-        };
         float l[NC];
 #pragma unroll
         for (int i = 0; i < NC; i++) l[i] = 0.0f;
         int E = TA_NONE;
-        int kx = scale_of(0, page_of(0)), pg = page_of(1);
         for (int j = 0; j < nt; j++) {
-            const int kx_next = scale_of(j + 1, pg);
-            pg = page_of(j + 2);
+            warp_wait(&sh.key_full, j & 1, dead);
+            const int kx = sh.kx[key];
             const bool valid = kx >= 0;
             const int draft = (tb + j) * TA_KEYS + key - ctx;
             const bool drafts = (tb + j + 1) * TA_KEYS > ctx;     // the tile holds drafted rows
@@ -660,7 +702,6 @@ k_tree_attn(const __grid_constant__ Args g)
             tc::fence_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.p_full));
-            kx = kx_next;
         }
         // row sums: the warp's 32 keys (lane = row), then the four warps
         const float mine = across<NC>(l, 0.0f, lane, [](float p, float q) { return p + q; });
@@ -797,7 +838,7 @@ Plan plan(int n_heads, int d, int n_tok, int batch, int max_ctx)
     // <= 512), else 48. Fewer where that leaves the number of tiles alone: an
     // MMA costs max(N / 2, 32 + N / 4) cycles (its operands' shared-memory
     // reads), a softmax N rows.
-    const int most = d <= 512 ? 64 : 48;
+    const int most = 48;
     const long tiles = (R + most - 1) / most;
     int nr = most;
     while (nr > 16 && (R + nr - 17) / (nr - 16) == tiles) nr -= 16;

@@ -59,6 +59,7 @@ __device__ __forceinline__ uint64_t now_ns()
 // tries: a wait's instructions take issue slots from the warps that work.)
 __device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatile int *dead)
 {
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
     uint64_t t0 = 0;
     while (true) {
 #pragma unroll 1

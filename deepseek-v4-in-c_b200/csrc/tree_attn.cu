@@ -66,10 +66,16 @@ constexpr int TA_SOFT = 8, TA_LOAD = 8, TA_COPY = 8;    // softmax, widening and
 constexpr int TA_RING = 4;                          // most pairs of the TMEM ring
 constexpr int TA_WCOPY = TA_SOFT + TA_LOAD, TA_WMMA = TA_WCOPY + TA_COPY;   // the MMA warp, in a warpgroup of its own
 constexpr int TA_T = 32 * (TA_WMMA + 4);
-// registers: 896 threads are launched with 72 each; the other warpgroups give
-// theirs to the softmax ones
-constexpr int TA_REG_SOFT = 112, TA_REG_LOAD = 72, TA_REG_COPY = 48, TA_REG_MMA = 40;
-static_assert(2 * (TA_REG_SOFT + TA_REG_LOAD + TA_REG_COPY) + TA_REG_MMA <= 7 * 72, "more registers than the block is launched with");
+// Registers: 896 threads are launched with 72 each. A softmax thread holds two
+// floats for each of its NR / 2 rows, a widening one the codes of the pairs in
+// flight (two, one at 64 rows); no role may spill in its loop (shared memory
+// leaves next to no L1, so a spilled register comes back from L2).
+template <int NR>
+struct Regs {
+    static constexpr int soft = NR == 64 ? 128 : NR == 48 ? 112 : 88, load = NR == 64 ? 64 : 72;
+    static constexpr int copy = NR >= 48 ? 48 : 56, mma = NR == 64 ? 24 : 40;
+    static_assert(2 * (soft + load + copy) + mma <= 7 * 72, "more registers than the block is launched with");
+};
 constexpr int TA_ROWS = 64;                         // most rows of a tile (N)
 constexpr int TA_STAGES = 4, TA_PAIRS = 5;
 constexpr int TA_SLOT = TA_KEYS * 128;              // bytes of one 64-element chunk
@@ -324,6 +330,7 @@ k_tree_attn(const __grid_constant__ Args g)
 
     if (warp >= TA_SOFT && warp < TA_WCOPY) {
         // --------------------------------------------------------- widening
+        if (Regs<NR>::load < 72) tc::reg_dec<Regs<NR>::load>();
         // Four lanes share a key: lane 4r + q holds elements 16q .. 16q + 15 of
         // a chunk for keys r and r + 8 of the warp's 16, so that a load reads
         // whole 64-byte runs of 8 rows (with a key per lane it took 4 times
@@ -417,16 +424,21 @@ k_tree_attn(const __grid_constant__ Args g)
         };
         // two pairs in flight, in registers of their own: a copy between them
         // would wait for the load
-        Unit u0, u1;
+        Unit u0;
         fetch(u0);
-        fetch(u1);
-        while (i < pairs) {
-            put(u0);
-            if (i < pairs) put(u1);
+        if constexpr (NR < 64) {
+            Unit u1;
+            fetch(u1);
+            while (i < pairs) {
+                put(u0);
+                if (i < pairs) put(u1);
+            }
+        } else {
+            while (i < pairs) put(u0);
         }
     } else if (warp >= TA_WCOPY && warp < TA_WMMA) {
         // ---------------------------------------------------------- copying
-        tc::reg_dec<TA_REG_COPY>();
+        tc::reg_dec<Regs<NR>::copy>();
         widen_q<NR>(a, sh, q_s, r0, nr, b, TA_SOFT + warp - TA_WCOPY, lane);
         tc::fence_async_smem();
         warp_arrive(&sh.q_full, lane);
@@ -464,7 +476,7 @@ k_tree_attn(const __grid_constant__ Args g)
         }
     } else if (warp >= TA_WMMA) {
         // ------------------------------------------------------- MMA issue
-        tc::reg_dec<TA_REG_MMA>();
+        tc::reg_dec<Regs<NR>::mma>();
         // Two warps, one for each product, each in the order of the pairs: the
         // tensor core takes what is ready of either.
         const int pairs = nt * npair;
@@ -569,7 +581,7 @@ k_tree_attn(const __grid_constant__ Args g)
         }
     } else {
         // --------------------------------------------------------- softmax
-        tc::reg_inc<TA_REG_SOFT>();
+        tc::reg_inc<Regs<NR>::soft>();
         const int wg = warp >> 2, key = (warp & 3) * 32 + lane, c0 = wg * NC;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         widen_q<NR>(a, sh, q_s, r0, nr, b, warp, lane);
@@ -830,36 +842,33 @@ struct Plan {
     int nr, tiles, nsplit, per;
 };
 
+// The pair (rows of a tile, splits) of least time on 148 SMs, one block each,
+// by what a block costs: microseconds per tile and beside its tiles, measured
+// at d = 512 over 700 to 32768 positions. A tile's time hardly depends on its
+// rows (the 128 keys are widened all the same), so many rows win once the
+// blocks fill the machine, and few rows before that. At 64 rows Q, P and the
+// keys fit in shared memory up to d = 512.
 Plan plan(int n_heads, int d, int n_tok, int batch, int max_ctx)
 {
+    static const double tile_us[4] = {2.9, 3.1, 3.2, 3.4}, block_us[4] = {9.0, 11.0, 12.5, 15.0};
     Plan best = {};
-    const long R = (long)n_heads * n_tok;
-    // Rows per tile: 64 while Q, P and a tile of rows fit in shared memory (d
-    // <= 512), else 48. Fewer where that leaves the number of tiles alone: an
-    // MMA costs max(N / 2, 32 + N / 4) cycles (its operands' shared-memory
-    // reads), a softmax N rows.
-    const int most = 48;
-    const long tiles = (R + most - 1) / most;
-    int nr = most;
-    while (nr > 16 && (R + nr - 17) / (nr - 16) == tiles) nr -= 16;
-    best.nr = nr;
-    best.tiles = (int)tiles;
-    const long units = tiles * batch;
-    const int kt = (max_ctx + n_tok + TA_KEYS - 1) / TA_KEYS;
-    // Splits: the fewest tile times on 148 SMs, a block costing about 1.5
-    // tiles beside its tiles and the join one round trip of the partial
-    // outputs through L2 (2.3 us a tile, 6500 bytes per ns).
     double cost = 0.0;
-    for (int s = 1; s <= TA_SPLITS && s <= kt; s++) {
-        const int per = (kt + s - 1) / s;
-        if ((kt + per - 1) / per != s) continue;
-        const long waves = (units * s + 147) / 148;
-        double c = waves * (per + 1.5);
-        if (s > 1) c += 1.0 + (double)s * units * nr * d * 8 / (6500.0 * 2300.0);
-        if (s == 1 || c < cost) {
-            cost = c;
-            best.nsplit = s;
-            best.per = per;
+    const long R = (long)n_heads * n_tok;
+    const int kt = (max_ctx + n_tok + TA_KEYS - 1) / TA_KEYS;
+    for (int i = d <= 512 ? 3 : 2; i >= 0; i--) {
+        const int nr = 16 * (i + 1);
+        const long tiles = (R + nr - 1) / nr, units = tiles * batch;
+        if (tiles > 65535) continue;
+        for (int s = 1; s <= TA_SPLITS && s <= kt; s++) {
+            const int per = (kt + s - 1) / s;
+            if ((kt + per - 1) / per != s) continue;
+            double c = (double)((units * s + 147) / 148) * (per * tile_us[i] + block_us[i]);
+            // the join: a launch, and the partial outputs once through L2
+            if (s > 1) c += 3.0 + (double)s * batch * R * d * 8 / 6.5e6;
+            if (best.nr == 0 || c < cost) {
+                cost = c;
+                best = {nr, (int)tiles, s, per};
+            }
         }
     }
     return best;

@@ -163,7 +163,7 @@ extern "C" int dsv4b_logits(void *out, const void *x, int dt, long out_stride, l
     if (!row_dt(dt) || rows < 0 || vocab < 1 || vocab > (1 << 30)) return -1;
     const dsv4b_logit_adjust none = {};
     const dsv4b_logit_adjust a = adj ? *adj : none;
-    if (a.hist && (!a.hist_len || a.hist_stride < 0)) return -1;
+    if (a.hist && (!a.hist_len || a.hist_stride < 0 || a.hist_stride > (1 << 30))) return -1;
     if (!a.hist && (a.rep || a.freq || a.pres || a.n_prompt)) return -1;
     if (a.bias && (!a.bias_ids || !a.bias_len || a.bias_stride < 0 || a.bias_stride > (1 << 30))) return -1;
     if (!a.bias && a.bias_ids) return -1;

@@ -12,12 +12,28 @@
 // value), -1 when no x is above -inf; a NaN is never chosen.
 //
 // Bound by HBM at many rows (2 * vocab * size a row) and by latency at one. A
-// cluster of 8 blocks owns a row: each block takes runs of the vocabulary,
-// counts the history that falls into its run in shared memory (integer
-// atomics, so the order of arrival cannot show), and makes one pass over the
-// logits; the blocks' best (value, index) pairs meet in the first block's
-// shared memory, so the greedy token needs neither scratch nor a second
-// launch.
+// cluster of 4 or 8 blocks owns a row; chunks of 64 tokens are dealt to the
+// blocks in turn, as the frequent tokens of a text lie together at the low end
+// of a vocabulary. Few of a block's tokens are in the history or the bias
+// list, so these are settled apart, and the pass over the logits only looks
+// up what they became:
+//
+//   mark     a bitmap of the block's named tokens, and a list of the history
+//            that falls to the block
+//   place    a slot for each marked token, by prefix sums of the bitmap
+//   count    its occurrences and its first bias, by integer atomics, so the
+//            order of arrival cannot show
+//   settle   its adjusted value, one thread a slot, kept in the slot
+//   stream   all its tokens, eight logits a thread at a time: a marked one is
+//            taken from its slot; mask, rounding, best value
+//
+// The blocks' best (value, index) pairs meet in the first block's shared
+// memory, so the greedy token needs neither scratch nor a second launch.
+//
+// Measured at 129280 floats a row: 9.4 us for one row with 600 tokens of
+// history, 31 us for 64 rows with up to 8192 (16.5 us without history and
+// biases, where the traffic alone takes 10.5); the rest is the latency of the
+// five steps, which two blocks a multiprocessor overlap only in part.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -29,16 +45,25 @@ namespace cg = cooperative_groups;
 
 namespace dsv4b {
 
-constexpr int LG_C = 8;                 // blocks of a row (a portable cluster)
+// Threads of a block, two blocks a multiprocessor. At 64 rows 512 threads take
+// 31 us, 256 take 44 (fewer loads in flight) and 1024, one block, 40.
 constexpr int LG_T = 512;
-constexpr int LG_RUN = 8192;            // tokens handled at once: 32 KB of counters, 32 KB of bias links
+constexpr int LG_CHUNK = 64;            // tokens dealt to a block at a time
+constexpr int LG_RUN = 65536;           // tokens of a block at a time: 16 bits number them
+constexpr int LG_SLOTS = 2048;          // named tokens settled at once; a run with more is cut into parts this long
+constexpr int LG_LIST = 4096;           // history entries kept; a longer list is read again
 
-// A history word in shared memory: the count of generated occurrences, and
-// the top bit when the token occurs in the prompt.
+// A slot's count: the generated occurrences, and the top bit when the token
+// occurs in the prompt. The same bit of a list entry marks the prompt's.
 constexpr unsigned LG_SEEN = 0x80000000u;
-// A bias link: the first list entry of the token, and a bit when there are
-// more.
-constexpr unsigned LG_NONE = 0xFFFFFFFFu, LG_MORE = 0x80000000u;
+constexpr unsigned LG_NONE = 0xFFFFFFFFu;       // a slot without a bias
+
+// Rows that get 8 blocks each; more get 4, which read the history half as
+// often. Measured at 129280 floats, 2000 tokens of history, 50 biases, a mask
+// (us by 8 / by 4 blocks a row): 1 row 10.6 / 13.5, 16 rows 14.1 / 14.0,
+// 32 rows 16.3 / 18.3, 48 rows 30.8 / 22.7, 64 rows 31.5 / 24.1: the step
+// comes where the blocks no longer all fit on the device at once.
+constexpr int LG_FEW = 36;
 
 struct LogitsCall {
     void *out;
@@ -58,122 +83,241 @@ __device__ __forceinline__ void better(float &v, int &i, float ov, int oi)
     }
 }
 
-template <int DT, bool VEC>
-__global__ void __cluster_dims__(LG_C, 1, 1) __launch_bounds__(LG_T)
+// Dynamic shared memory of a run of `run` tokens (a multiple of 64).
+__host__ __device__ inline size_t lg_smem(int run, bool named, bool bias)
+{
+    if (!named) return 0;
+    return LG_LIST * 4 + LG_SLOTS * (4 + 2) + (bias ? LG_SLOTS * 4 + LG_SLOTS / 8 : 0) + (size_t)run / 32 * (4 + 2);
+}
+
+// LG_C blocks a row.
+template <int DT, bool VEC, int LG_C>
+__global__ void __cluster_dims__(LG_C, 1, 1) __launch_bounds__(LG_T, 2)
 k_logits(LogitsCall c)
 {
     pdl_trigger();
     pdl_wait();
-    extern __shared__ unsigned cnt[];           // [run]
-    unsigned *link = cnt + c.run;               // [run] when there are biases
+    extern __shared__ unsigned sm[];
     __shared__ float sv[LG_T / 32], best_v[LG_C];
     __shared__ int si[LG_T / 32], best_i[LG_C];
-    const int row = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x;
+    __shared__ unsigned n_list, n_slots;
+    const int row = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
     const dsv4b_logit_adjust &a = c.a;
     const char *x = reinterpret_cast<const char *>(c.x) + (size_t)row * c.x_stride * row_dt_size(DT);
     char *out = c.out ? reinterpret_cast<char *>(c.out) + (size_t)row * c.out_stride * row_dt_size(DT) : nullptr;
     const int *hist = a.hist ? a.hist + (size_t)row * a.hist_stride : nullptr;
-    const int hl = hist ? min(__ldcg(a.hist_len + row), (int)min(a.hist_stride, 0x7fffffffL)) : 0;
-    const int np = hist && a.n_prompt ? __ldcg(a.n_prompt + row) : 0;
     const int *bid = a.bias ? a.bias_ids + (size_t)row * a.bias_stride : nullptr;
     const float *bias = a.bias ? a.bias + (size_t)row * a.bias_stride : nullptr;
-    const int bl = bias ? min(__ldcg(a.bias_len + row), (int)min(a.bias_stride, 0x7fffffffL)) : 0;
     const unsigned *mask = a.mask ? a.mask + (size_t)row * a.mask_stride : nullptr;
-    const float rep = a.rep ? __ldcg(a.rep + row) : 1.0f, freq = a.freq ? __ldcg(a.freq + row) : 0.0f;
-    const float pres = a.pres ? __ldcg(a.pres + row) : 0.0f;
+    const bool named = hist || bias;
+    unsigned *list = sm, *cnt = list + LG_LIST, *link = cnt + LG_SLOTS, *many = link + (bias ? LG_SLOTS : 0);
+    unsigned *bits = many + (bias ? LG_SLOTS / 32 : 0);
+    unsigned short *tok = reinterpret_cast<unsigned short *>(bits + c.run / 32), *base = tok + LG_SLOTS;
+
+    // Number k of the block's run in the run of the cluster that starts at r0.
+    auto token_of = [&](int r0, int k) { return r0 + ((k / LG_CHUNK) * LG_C + rank) * LG_CHUNK + k % LG_CHUNK; };
+    // eight logits and their mask bits, asked for ahead of their use
+    Raw8<DT> nx;
+    unsigned nm = 0xFFu;
+    auto ask = [&](int r0, int k, int end) {
+        const int t0 = token_of(r0, k);
+        if (k >= end || t0 >= c.vocab) return;
+        if (t0 + 8 <= c.vocab) nx = ld_raw8<DT, VEC>(x, (size_t)t0);
+        if (mask) nm = __ldcg(mask + (t0 >> 5)) >> (t0 & 31);
+    };
+    ask(0, tid * 8, c.run);
+
+    const int hl = hist ? min(__ldcg(a.hist_len + row), (int)min(a.hist_stride, 0x7fffffffL)) : 0;
+    const int np = hist && a.n_prompt ? __ldcg(a.n_prompt + row) : 0;
+    const int bl = bias ? min(__ldcg(a.bias_len + row), (int)min(a.bias_stride, 0x7fffffffL)) : 0;
     float bv = -INFINITY;
     int bi = -1;
     // every block of the cluster has started before one writes to the first
     if (c.token) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-    for (int r0 = rank * c.run; r0 < c.vocab; r0 += LG_C * c.run) {
-        const int m = min(c.run, c.vocab - r0);
-        if (hist || bias) {
-            __syncthreads();                    // the counters of the run before are read
-            for (int i = tid; i < m; i += LG_T) {
-                if (hist) cnt[i] = 0;
-                if (bias) link[i] = LG_NONE;
-            }
-            __syncthreads();
-            for (int i = tid; i < hl; i += LG_T) {
-                const unsigned k = (unsigned)(__ldcg(hist + i) - r0);
-                if (k < (unsigned)m) {
-                    if (i >= np) atomicAdd(cnt + k, 1u);
-                    else atomicOr(cnt + k, LG_SEEN);
+    for (long at = 0; at < c.vocab; at += (long)LG_C * c.run) {
+        const int r0 = (int)at, here = min(LG_C * c.run, c.vocab - r0);       // the cluster's tokens
+        const int chunks = (here + LG_CHUNK - 1) / LG_CHUNK, m = (chunks - rank + LG_C - 1) / LG_C * LG_CHUNK;
+        // fn(i, k) for the first n entries i of a list of tokens, k the
+        // block's number of the token, ~0 for one that is not its own; whole
+        // warps, four loads in flight
+        auto each = [&](const int *ids, int n, auto fn) {
+            for (int i0 = tid & ~31; i0 < n; i0 += 4 * LG_T) {
+                unsigned u[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int i = i0 + j * LG_T + lane;
+                    u[j] = i < n ? (unsigned)__ldcg(ids + i) - (unsigned)r0 : 0xFFFFFFFFu;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const unsigned q = u[j] / LG_CHUNK;
+                    const bool own = u[j] < (unsigned)here && q % LG_C == (unsigned)rank;
+                    fn(i0 + j * LG_T + lane, own ? q / LG_C * LG_CHUNK + u[j] % LG_CHUNK : 0xFFFFFFFFu);
                 }
             }
-            for (int i = tid; i < bl; i += LG_T) {
-                const unsigned k = (unsigned)(__ldcg(bid + i) - r0);
-                if (k < (unsigned)m) atomicMin(link + k, (unsigned)i);
+        };
+        auto place = [&](int w0, int w1) {      // slots of the marked tokens of bitmap words w0 .. w1
+            for (int w = w0 + (tid & ~31); w < w1; w += LG_T) {
+                const int n = w + lane < w1 ? __popc(bits[w + lane]) : 0;
+                int to = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, to, o);
+                    if (lane >= o) to += up;
+                }
+                unsigned first = 0;
+                if (lane == 31) first = atomicAdd(&n_slots, (unsigned)to);
+                first = __shfl_sync(0xffffffffu, first, 31);
+                if (w + lane < w1) base[w + lane] = (unsigned short)(first + to - n);
             }
+            for (int i = tid; i < LG_SLOTS; i += LG_T) {
+                cnt[i] = 0;
+                if (bias) link[i] = LG_NONE;
+            }
+            if (bias)
+                for (int i = tid; i < LG_SLOTS / 32; i += LG_T) many[i] = 0;
+        };
+        auto slot_of = [&](unsigned k) { return base[k >> 5] + __popc(bits[k >> 5] & ((1u << (k & 31)) - 1u)); };
+        if (named) {
+            __syncthreads();                    // the run before is done
+            for (int i = tid; i < (m + 31) >> 5; i += LG_T) bits[i] = 0;
+            if (tid == 0) n_list = n_slots = 0;
             __syncthreads();
-            if (bl > 1) {
-                for (int i = tid; i < bl; i += LG_T) {
-                    const unsigned k = (unsigned)(__ldcg(bid + i) - r0);
-                    if (k < (unsigned)m && (link[k] & ~LG_MORE) != (unsigned)i) atomicOr(link + k, LG_MORE);
+            each(hist, hl, [&](int i, unsigned k) {
+                const bool own = k != 0xFFFFFFFFu;
+                const unsigned who = __ballot_sync(0xffffffffu, own);
+                if (!who) return;
+                unsigned p = 0;
+                if (lane == 0) p = atomicAdd(&n_list, (unsigned)__popc(who));
+                p = __shfl_sync(0xffffffffu, p, 0) + __popc(who & ((1u << lane) - 1u));
+                if (own) {
+                    atomicOr(bits + (k >> 5), 1u << (k & 31));
+                    if (p < LG_LIST) list[p] = k | (i < np ? LG_SEEN : 0u);
+                }
+            });
+            each(bid, bl, [&](int, unsigned k) {
+                if (k != 0xFFFFFFFFu) atomicOr(bits + (k >> 5), 1u << (k & 31));
+            });
+            __syncthreads();
+            place(0, (m + 31) >> 5);
+            __syncthreads();
+        }
+        const bool whole = !named || n_slots <= LG_SLOTS;
+        const int part = whole ? m : LG_SLOTS;
+        for (int s0 = 0; s0 < m; s0 += part) {
+            const int len = min(part, m - s0);
+            if (!whole) {
+                __syncthreads();                // the part before is done
+                if (tid == 0) n_slots = 0;
+                __syncthreads();
+                place(s0 >> 5, (s0 + len + 31) >> 5);
+                __syncthreads();
+            }
+            if (named) {
+                auto count = [&](unsigned k, bool prompt) {
+                    if (k - s0 >= (unsigned)len) return;
+                    const int s = slot_of(k);
+                    tok[s] = (unsigned short)k;
+                    if (prompt) atomicOr(cnt + s, LG_SEEN);
+                    else atomicAdd(cnt + s, 1u);
+                };
+                const int nl = (int)n_list;
+                if (nl <= LG_LIST)
+                    for (int i = tid; i < nl; i += LG_T) count(list[i] & ~LG_SEEN, list[i] & LG_SEEN);
+                else                            // the list is cut short: the history again
+                    each(hist, hl, [&](int i, unsigned k) { count(k, i < np); });
+                each(bid, bl, [&](int i, unsigned k) {
+                    if (k - s0 >= (unsigned)len) return;
+                    const int s = slot_of(k);
+                    tok[s] = (unsigned short)k;
+                    if (atomicMin(link + s, (unsigned)i) != LG_NONE) atomicOr(many + (s >> 5), 1u << (s & 31));
+                });
+                __syncthreads();
+                const int ns = (int)n_slots;
+                for (int j0 = tid & ~31; j0 < ns; j0 += LG_T) {
+                    const int j = j0 + lane;
+                    const bool on = j < ns;
+                    const int t = on ? token_of(r0, tok[j]) : 0;
+                    const unsigned w = on ? cnt[j] : 0;
+                    float v = on ? ld_row1<DT>(x, (size_t)t) : 0.0f;
+                    if (w) {
+                        const unsigned n = w & ~LG_SEEN;
+                        const float rep = a.rep ? __ldcg(a.rep + row) : 1.0f;
+                        v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+                        if (n) {
+                            v = __fsub_rn(v, __fmul_rn(a.freq ? __ldcg(a.freq + row) : 0.0f, (float)n));
+                            v = __fsub_rn(v, a.pres ? __ldcg(a.pres + row) : 0.0f);
+                        }
+                    }
+                    if (bias) {
+                        const unsigned l = on ? link[j] : LG_NONE;
+                        double s = l != LG_NONE ? (double)__ldcg(bias + l) : 0.0;
+                        // a token that is named again: the warp looks for its
+                        // other entries and adds them in list order
+                        for (unsigned rest = many[j0 >> 5]; rest; rest &= rest - 1) {
+                            const int who = __ffs(rest) - 1;
+                            const int want = __shfl_sync(0xffffffffu, t, who);
+                            for (int i0 = __shfl_sync(0xffffffffu, (int)l, who) + 1; i0 < bl; i0 += 128) {
+                                int id[4];
+#pragma unroll
+                                for (int u = 0; u < 4; u++) {
+                                    const int i = i0 + u * 32 + lane;
+                                    id[u] = i < bl ? __ldcg(bid + i) : -1;
+                                }
+#pragma unroll
+                                for (int u = 0; u < 4; u++)
+                                    for (unsigned hit = __ballot_sync(0xffffffffu, id[u] == want); hit; hit &= hit - 1)
+                                        if (lane == who) s += (double)__ldcg(bias + i0 + u * 32 + __ffs(hit) - 1);
+                            }
+                        }
+                        if (l != LG_NONE) v = __fadd_rn(v, (float)s);
+                    }
+                    if (on) cnt[j] = __float_as_uint(v);
                 }
                 __syncthreads();
             }
-        }
-        auto adjust = [&](int k, float v, unsigned bits) {
-            if (hist) {
-                const unsigned w = cnt[k];
-                if (w) {
-                    const unsigned n = w & ~LG_SEEN;
-                    v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-                    if (n) {
-                        v = __fsub_rn(v, __fmul_rn(freq, (float)n));
-                        v = __fsub_rn(v, pres);
+            const int end = s0 + len;
+            if (r0 || s0) ask(r0, s0 + tid * 8, end);
+            for (int k = s0 + tid * 8; k < end; k += LG_T * 8) {
+                const int t0 = token_of(r0, k), left = min(8, c.vocab - t0);
+                if (left <= 0) break;
+                float v[8];
+                if (left == 8) {
+                    widen8<DT>(nx, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = j < left ? ld_row1<DT>(x, (size_t)t0 + j) : -INFINITY;
+                }
+                const unsigned on = nm;
+                ask(r0, k + LG_T * 8, end);
+                if (named) {
+                    const unsigned its = bits[k >> 5] >> (k & 31) & 0xFFu;
+                    if (its) {
+                        const unsigned *s = cnt + slot_of(k);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (its >> j & 1u) v[j] = __uint_as_float(s[__popc(its & ((1u << j) - 1u))]);
                     }
                 }
-            }
-            if (bias) {
-                const unsigned l = link[k];
-                if (l != LG_NONE) {
-                    const int i = (int)(l & ~LG_MORE);
-                    double s = (double)__ldcg(bias + i);
-                    if (l & LG_MORE)            // the token's other entries, in list order
-                        for (int j = i + 1; j < bl; j++)
-                            if (__ldcg(bid + j) == r0 + k) s += (double)__ldcg(bias + j);
-                    v = __fadd_rn(v, (float)s);
-                }
-            }
-            return (bits & 1u) ? v : -INFINITY;
-        };
-        if constexpr (VEC) {
-            const int groups = (m + 7) >> 3;
-            for (int g = tid; g < groups; g += LG_T) {
-                const int k0 = g << 3;
-                float v[8];
-                const int left = min(8, m - k0);
-                if (left == 8) {
-                    widen8<DT>(ld_raw8<DT, true>(x, (size_t)r0 + k0), v);
-                } else {
-                    for (int j = 0; j < 8; j++) v[j] = j < left ? ld_row1<DT>(x, (size_t)r0 + k0 + j) : -INFINITY;
-                }
-                const unsigned w = mask ? __ldcg(mask + ((r0 + k0) >> 5)) >> ((r0 + k0) & 31) : 0xFFu;
+                float top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    if (j >= left) break;
-                    v[j] = adjust(k0 + j, v[j], w >> j);
+                    if (!(on >> j & 1u)) v[j] = -INFINITY;
                     if constexpr (DT == DSV4B_BF16) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
                     if constexpr (DT == DSV4B_F16) v[j] = __half2float(__float2half_rn(v[j]));
-                    if (v[j] > bv) bv = v[j], bi = r0 + k0 + j;
+                    top = fmaxf(top, v[j]);                     // passes over NaN
+                }
+                if (top > bv) {
+                    bv = top;
+#pragma unroll
+                    for (int j = 7; j >= 0; j--)
+                        if (v[j] == top) bi = t0 + j;
                 }
                 if (out) {
-                    if (left == 8) st_row8<DT, true>(out, (size_t)r0 + k0, v);
+                    if (left == 8) st_row8<DT, VEC>(out, (size_t)t0, v);
                     else
-                        for (int j = 0; j < left; j++) st_row1<DT>(out, (size_t)r0 + k0 + j, v[j]);
+                        for (int j = 0; j < left; j++) st_row1<DT>(out, (size_t)t0 + j, v[j]);
                 }
-            }
-        } else {
-            for (int k = tid; k < m; k += LG_T) {
-                const int t = r0 + k;
-                const unsigned w = mask ? __ldcg(mask + (t >> 5)) >> (t & 31) : 1u;
-                float v = adjust(k, ld_row1<DT>(x, (size_t)t), w);
-                if constexpr (DT == DSV4B_BF16) v = __bfloat162float(__float2bfloat16_rn(v));
-                if constexpr (DT == DSV4B_F16) v = __half2float(__float2half_rn(v));
-                if (v > bv) bv = v, bi = t;
-                if (out) st_row1<DT>(out, (size_t)t, v);
             }
         }
     }
@@ -202,13 +346,16 @@ int logits(void *out, const void *x, int dt, long out_stride, long x_stride, int
 {
     if (rows <= 0 || vocab <= 0) return 0;
     LogitsCall c = {out, x, out_stride, x_stride, token, a, vocab, 0};
-    const int share = ((vocab + LG_C - 1) / LG_C + 31) & ~31;     // whole mask words a run
+    const int nb = rows <= LG_FEW ? 8 : 4;
+    const int share = ((vocab + nb - 1) / nb + LG_CHUNK - 1) / LG_CHUNK * LG_CHUNK;
     c.run = share < LG_RUN ? share : LG_RUN;
     const int sz = row_dt_size(dt);
     const bool vec = !(((uintptr_t)x | (uintptr_t)out) & 15) && !((x_stride * sz) & 15) && !((out_stride * sz) & 15);
-    const size_t smem = (size_t)c.run * 4 * (a.bias ? 2 : 1);
+    const size_t smem = lg_smem(c.run, a.hist || a.bias, a.bias), most = lg_smem(LG_RUN, true, true);
     DSV4B_ROW_DT(dt, DT, {
-        if (smem_optin(k_logits<DT, true>, LG_RUN * 8) || smem_optin(k_logits<DT, false>, LG_RUN * 8)) return -2;
+        const auto k = nb == 8 ? (vec ? k_logits<DT, true, 8> : k_logits<DT, false, 8>)
+                               : (vec ? k_logits<DT, true, 4> : k_logits<DT, false, 4>);
+        if (smem_optin(k, most)) return -2;
         for (int r0 = 0; r0 < rows; r0 += 32768) {
             const int nr = rows - r0 < 32768 ? rows - r0 : 32768;
             LogitsCall p = c;
@@ -222,8 +369,7 @@ int logits(void *out, const void *x, int dt, long out_stride, long x_stride, int
             if (a.pres) p.a.pres += r0;
             if (a.bias) p.a.bias += (size_t)r0 * a.bias_stride, p.a.bias_ids += (size_t)r0 * a.bias_stride, p.a.bias_len += r0;
             if (a.mask) p.a.mask += (size_t)r0 * a.mask_stride;
-            if (vec) launch(k_logits<DT, true>, dim3(LG_C, nr), dim3(LG_T), smem, st, p);
-            else launch(k_logits<DT, false>, dim3(LG_C, nr), dim3(LG_T), smem, st, p);
+            launch(k, dim3(nb, nr), dim3(LG_T), smem, st, p);
         }
     });
     return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;

@@ -660,6 +660,50 @@ def test_logits_plain_and_special_values():
     assert tok.tolist() == [-1] * 4
 
 
+@pytest.mark.parametrize("v,hist,span,nb,dt", [
+    (129280, 60000, 129280, 3000, "f32"),       # more named tokens in a block's share than it settles at once
+    (129280, 60000, 9000, 0, "bf16"),           # the same in the first shares alone
+    (129280, 5000, 700, 0, "f32"),              # a long history of few tokens
+    (40000, 0, 40000, 30000, "f16"),            # biases alone
+    (600001, 40000, 600001, 500, "f32"),        # a vocabulary of two runs a block
+    (600001, 70000, 150000, 9, "bf16")])
+def test_logits_many_named(v, hist, span, nb, dt):
+    """Histories and bias lists that fill, and overflow, what a block settles at once."""
+    g = gen(v + hist)
+    x = (3 * normal(g, 2, v)).to(DT[dt])
+    kw = {}
+    y, size = x.double(), x.double().abs()
+    if hist:
+        h = torch.randint(0, span, (2, hist), generator=g, device="cuda", dtype=torch.int32)
+        n = torch.tensor([hist // 3, 0], dtype=torch.int32, device="cuda")
+        rep, freq, pres = 0.5 + torch.rand(2, generator=g, device="cuda"), 0.1 * normal(g, 2), normal(g, 2)
+        kw.update(hist=h, hist_len=torch.full((2,), hist, dtype=torch.int32, device="cuda"), n_prompt=n, rep=rep,
+                  freq=freq, pres=pres)
+        for i in range(2):
+            seen = torch.bincount(h[i].long(), minlength=v) > 0
+            count = torch.bincount(h[i, int(n[i]):].long(), minlength=v).double()
+            r = rep[i].double()
+            y[i] = torch.where(seen, torch.where(y[i] > 0, y[i] / r, y[i] * r), y[i])
+            size[i] = torch.maximum(size[i], y[i].abs()) + (freq[i].double() * count).abs() + pres[i].double().abs()
+            y[i] -= freq[i].double() * count + pres[i].double() * (count > 0)
+    if nb:
+        ids = torch.randint(0, v, (2, nb), generator=g, device="cuda", dtype=torch.int32)
+        bias = normal(g, 2, nb)
+        kw.update(bias_ids=ids, bias=bias, bias_len=torch.full((2,), nb, dtype=torch.int32, device="cuda"))
+        for i in range(2):
+            y[i].index_add_(0, ids[i].long(), bias[i].double())
+            size[i].index_add_(0, ids[i].long(), bias[i].double().abs())
+    rel, low = unit(DT[dt])
+    # at most six float roundings on the way, then the output's
+    tol = 6.01 * U32 * size + rel * (1 + 2 ** -20) * y.abs() + low
+    out, tok = torch.empty_like(x), torch.empty(2, dtype=torch.int32, device="cuda")
+    B.logits_dev(out, x, tok, B.LogitAdjust(**kw))
+    close(out, y, tol)
+    assert tok.tolist() == greedy(out)
+    B.logits_dev(x, x, None, B.LogitAdjust(**kw))
+    assert torch.equal(x, out)
+
+
 def test_logits_duplicate_biases_are_ordered():
     """A token named many times gets the sum in list order, the same every time."""
     v, n = 5000, 900

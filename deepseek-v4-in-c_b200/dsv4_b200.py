@@ -372,52 +372,58 @@ def sparse_attn_dev(o, q, kv, kv_dt, seq_kv_rows, sink, idxs, n_heads, d, topk_n
 # device, so they are ordered after the torch work that made their tensors.
 
 F16 = 3
-_row_dt = None
+_t = None                       # torch, imported by the first of these calls
+_row_dt = {}
+
+
+def _torch():
+    global _t
+    if _t is None:
+        import torch
+        _row_dt.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+        _t = torch
+    return _t
 
 
 def _dt(t, what):
     """The row type (F32, BF16, F16) of a tensor."""
-    global _row_dt
-    if _row_dt is None:
-        import torch
-        _row_dt = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
     dt = _row_dt.get(t.dtype)
     if dt is None:
         raise ValueError("%s must be float32, bfloat16 or float16" % what)
     return dt
 
 
-def _want(t, what, dev, dtype, shape):
-    """A contiguous tensor of dev with the given element type name and shape
-    (None: any); None passes through."""
-    if t is None:
-        return None
-    if t.device != dev or not t.is_cuda:
+def _want(t, what, dev, dtype, shape=None):
+    """Address of a contiguous tensor on CUDA device `dev` (its index) of the
+    given type and shape (None: any)."""
+    if t.get_device() != dev:
         raise ValueError("%s must be on the device of the other tensors" % what)
-    if dtype is not None and str(t.dtype)[6:] not in dtype:
-        raise ValueError("%s must be %s" % (what, " or ".join(dtype)))
-    if shape is not None and tuple(t.shape) != shape:
+    if t.dtype is not dtype:
+        raise ValueError("%s must be %s" % (what, dtype))
+    if shape is not None and t.shape != shape:
         raise ValueError("%s must have shape %s" % (what, shape))
     if not t.is_contiguous():
         raise ValueError("%s must be contiguous" % what)
     return t.data_ptr()
 
 
-def _enqueue(fn, what, dev, stream, *args):
-    """Call fn(*args, stream) with dev current; torch's current stream for None
+def _stream(dev, stream):
+    """The handle to enqueue on: torch's current stream of the device for None
     (its default stream by the legacy handle, as NULL is the backend's own)."""
-    import torch
     if stream is None:
-        s = torch._C._cuda_getCurrentRawStream(dev.index)
+        return _t._C._cuda_getCurrentRawStream(dev) or 1
+    if stream.device.index != dev:
+        raise ValueError("the stream belongs to another device than the tensors")
+    return stream.cuda_stream or 1
+
+
+def _enqueue(fn, what, dev, *args):
+    """fn(*args) with device dev current."""
+    if _t._C._cuda_getDevice() == dev:
+        rc = fn(*args)
     else:
-        if stream.device != dev:
-            raise ValueError("the stream belongs to another device than the tensors")
-        s = stream.cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, s or 1)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, s or 1)
+        with _t.cuda.device(dev):
+            rc = fn(*args)
     if rc != 0:
         raise RuntimeError("%s %s (rc=%d)" % (what, "refused its arguments" if rc == -1 else "could not launch", rc))
 
@@ -435,22 +441,20 @@ def rope_dev(out, x, pos, cfg, first, inverse=False, stream=None):
     """out = x [tokens, heads, width] with elements first .. first + cfg.rd of
     every head rotated to pos [tokens] (int32); inverse rotates back. Any
     strides with unit-stride heads; out may be x."""
-    dev = x.device
-    if x.dim() != 3 or out.shape != x.shape or x.stride(2) != 1 or out.stride(2) != 1:
+    i32 = _torch().int32
+    dev = x.get_device()
+    xs, os_, shape = x.stride(), out.stride(), x.shape
+    if len(shape) != 3 or out.shape != shape or xs[2] != 1 or os_[2] != 1:
         raise ValueError("x and out must be [tokens, heads, width] with unit-stride heads")
-    if out.device != dev or not x.is_cuda:
+    if dev < 0 or out.get_device() != dev:
         raise ValueError("x and out must be on one CUDA device")
-    n, h, w = x.shape
-    p = _want(pos, "pos", dev, ("int32",), (n,))
-
-    def strides(t):                 # torch leaves the stride of a length-1 axis free
-        sh = t.stride(1) if h > 1 else w
-        return (t.stride(0) if n > 1 else (h - 1) * sh + w), sh
-
-    ot, oh = strides(out)
-    xt, xh = strides(x)
-    _enqueue(lib().dsv4b_rope, "dsv4b_rope", dev, stream, out.data_ptr(), _dt(out, "out"), ot, oh, x.data_ptr(),
-             _dt(x, "x"), xt, xh, C.byref(cfg), p, n, h, w, int(first), 1 if inverse else 0)
+    n, h, w = shape
+    # torch leaves the stride of a length-1 axis free
+    xh, oh = (xs[1], os_[1]) if h > 1 else (w, w)
+    xt, ot = (xs[0], os_[0]) if n > 1 else ((h - 1) * xh + w, (h - 1) * oh + w)
+    _enqueue(lib().dsv4b_rope, "dsv4b_rope", dev, out.data_ptr(), _dt(out, "out"), ot, oh, x.data_ptr(), _dt(x, "x"),
+             xt, xh, C.addressof(cfg), _want(pos, "pos", dev, i32, (n,)), n, h, w, int(first), 1 if inverse else 0,
+             _stream(dev, stream))
 
 
 class KvCache:
@@ -466,11 +470,14 @@ class KvCache:
             raise ValueError("d must be a multiple of 64 up to %d, tail one up to d" % KVQ_MAX_D)
         if rows < 1 or rows & (rows - 1) or pages < 1:
             raise ValueError("page_rows must be a power of two, and there must be a page")
-        self.device = codes.device
-        self.c = KvqC(_want(codes, "codes", self.device, ("uint8",), None),
-                      _want(scales, "scales", self.device, ("uint8",), (pages, rows)), pages, rows, d, tail)
+        self.device = codes.get_device()
+        if self.device < 0:
+            raise ValueError("codes must be on a CUDA device")
+        u8 = _torch().uint8
+        self.c = KvqC(_want(codes, "codes", self.device, u8), _want(scales, "scales", self.device, u8, (pages, rows)),
+                      pages, rows, d, tail)
         self.codes, self.scales, self.d, self.tail = codes, scales, d, tail
-        self.ref = C.byref(self.c)
+        self.ref = C.addressof(self.c)
 
     @classmethod
     def empty(cls, pages, page_rows, d, tail, device="cuda"):
@@ -481,31 +488,32 @@ class KvCache:
 
 
 def _rows(t, what, cache):
-    if t.dim() != 2 or t.shape[1] != cache.d or t.stride(1) != 1 or t.device != cache.device:
+    s, n = t.stride(), t.shape
+    if len(n) != 2 or n[1] != cache.d or s[1] != 1 or t.get_device() != cache.device:
         raise ValueError("%s must be [n, d] with unit-stride rows on the cache's device" % what)
-    return t.data_ptr(), _dt(t, what), t.stride(0) if t.shape[0] > 1 else cache.d
+    return t.data_ptr(), _dt(t, what), s[0] if n[0] > 1 else cache.d, n[0]
 
 
 def kv_write_dev(cache, rows, slots, rope=None, pos=None, stream=None):
     """Quantise rows [n, d] into the cache's slots [n] (int64, distinct; -1
     skips a row). With rope and pos [n] (int32) the last rope.rd elements of
     each row are rotated first."""
-    p, dt, st = _rows(rows, "rows", cache)
-    n, dev = rows.shape[0], cache.device
+    p, dt, st, n = _rows(rows, "rows", cache)
+    dev = cache.device
     if (rope is None) != (pos is None):
         raise ValueError("rope and pos go together")
-    _enqueue(lib().dsv4b_kv_write, "dsv4b_kv_write", dev, stream, cache.ref, p, dt, st,
-             _want(slots, "slots", dev, ("int64",), (n,)), n, None if rope is None else C.byref(rope),
-             _want(pos, "pos", dev, ("int32",), (n,)))
+    _enqueue(lib().dsv4b_kv_write, "dsv4b_kv_write", dev, cache.ref, p, dt, st,
+             _want(slots, "slots", dev, _t.int64, (n,)), n, None if rope is None else C.addressof(rope),
+             None if pos is None else _want(pos, "pos", dev, _t.int32, (n,)), _stream(dev, stream))
 
 
 def kv_read_dev(out, cache, slots, stream=None):
     """out [n, d] = the values of the cache's rows slots [n]; zeros for a slot
     outside the cache."""
-    p, dt, st = _rows(out, "out", cache)
-    n, dev = out.shape[0], cache.device
-    _enqueue(lib().dsv4b_kv_read, "dsv4b_kv_read", dev, stream, cache.ref, p, dt, st,
-             _want(slots, "slots", dev, ("int64",), (n,)), n)
+    p, dt, st, n = _rows(out, "out", cache)
+    dev = cache.device
+    _enqueue(lib().dsv4b_kv_read, "dsv4b_kv_read", dev, cache.ref, p, dt, st,
+             _want(slots, "slots", dev, _t.int64, (n,)), n, _stream(dev, stream))
 
 
 def tree_mask(parents):
@@ -534,14 +542,14 @@ def tree_attn_dev(o, q, cache, pages, ctx, n_draft, mask, sink, max_ctx, scale, 
     ctx [batch] and n_draft [batch] (or None) are int32, mask [batch, tokens]
     int64 (tree_mask), sink [heads] float32 or None, scratch at least
     tree_attn_scratch() bytes that no other call uses meanwhile."""
-    dev = cache.device
-    if q.dim() != 4 or o.shape != q.shape or o.dtype != q.dtype or q.shape[3] != cache.d:
+    dev, shape = cache.device, q.shape
+    if len(shape) != 4 or o.shape != shape or o.dtype is not q.dtype or shape[3] != cache.d:
         raise ValueError("q and o must be [batch, tokens, heads, d] of one type")
-    b, t, h, d = q.shape
+    b, t, h, d = shape
     tok = []
     for x, what in ((o, "o"), (q, "q")):
         s = x.stride()
-        if x.device != dev or s[3] != 1 or (h > 1 and s[2] != d):
+        if x.get_device() != dev or s[3] != 1 or (h > 1 and s[2] != d):
             raise ValueError("%s must have contiguous heads on the cache's device" % what)
         st = s[1] if t > 1 else (s[0] if b > 1 else h * d)
         if b > 1 and s[0] != t * st:
@@ -549,13 +557,15 @@ def tree_attn_dev(o, q, cache, pages, ctx, n_draft, mask, sink, max_ctx, scale, 
         tok.append(st)
     if pages.dim() != 2 or pages.shape[0] != b:
         raise ValueError("pages must be [batch, max_pages]")
-    if scratch.device != dev or not scratch.is_contiguous():
+    if scratch.get_device() != dev or not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous, on the cache's device")
-    _enqueue(lib().dsv4b_tree_attn, "dsv4b_tree_attn", dev, stream, o.data_ptr(), q.data_ptr(), _dt(q, "q"), tok[0],
-             tok[1], cache.ref, _want(pages, "pages", dev, ("int32",), None), pages.shape[1],
-             _want(ctx, "ctx", dev, ("int32",), (b,)), _want(n_draft, "n_draft", dev, ("int32",), (b,)),
-             _want(mask, "mask", dev, ("int64",), (b, t)), _want(sink, "sink", dev, ("float32",), (h,)), h, t, b,
-             int(max_ctx), float(scale), scratch.data_ptr(), scratch.numel() * scratch.element_size())
+    i32 = _t.int32
+    _enqueue(lib().dsv4b_tree_attn, "dsv4b_tree_attn", dev, o.data_ptr(), q.data_ptr(), _dt(q, "q"), tok[0], tok[1],
+             cache.ref, _want(pages, "pages", dev, i32), pages.shape[1], _want(ctx, "ctx", dev, i32, (b,)),
+             None if n_draft is None else _want(n_draft, "n_draft", dev, i32, (b,)),
+             _want(mask, "mask", dev, _t.int64, (b, t)),
+             None if sink is None else _want(sink, "sink", dev, _t.float32, (h,)), h, t, b, int(max_ctx),
+             float(scale), scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream(dev, stream))
 
 
 class LogitAdjust:
@@ -573,48 +583,54 @@ class LogitAdjust:
             bias = bias_ids = bias_len = None
         given = [t for t in (hist, bias, mask) if t is not None]
         self.rows = given[0].shape[0] if given else None
-        self.device = given[0].device if given else None
+        self.device = given[0].get_device() if given else None
+        if given and self.device < 0:
+            raise ValueError("the tensors must be on a CUDA device")
         if (hist is None) != (hist_len is None) or (bias is None) != (bias_ids is None) or \
                 (bias is None) != (bias_len is None):
             raise ValueError("hist goes with hist_len, bias with bias_ids and bias_len")
         if hist is None and any(t is not None for t in (n_prompt, rep, freq, pres)):
             raise ValueError("penalties need hist")
-        r, dev = (self.rows,), self.device
         two = [t for t in (hist, bias_ids, bias, mask) if t is not None]
         if any(t.dim() != 2 or t.shape[0] != self.rows for t in two):
             raise ValueError("hist, bias_ids, bias and mask must be [rows, n]")
         if bias is not None and bias.shape != bias_ids.shape:
             raise ValueError("bias and bias_ids must have one shape")
-        i32, f32 = ("int32",), ("float32",)
+        i32, f32 = _torch().int32, _torch().float32
+
+        def want(t, what, dtype, shape=None):
+            return None if t is None else _want(t, what, self.device, dtype, shape)
+
+        r = (self.rows,)
         self.keep = (hist, hist_len, n_prompt, rep, freq, pres, bias_ids, bias, bias_len, mask)
-        self.words = 0 if mask is None else mask.shape[1]
-        self.masked = mask is not None
         self.c = LogitAdjustC(
-            _want(hist, "hist", dev, i32, None), 0 if hist is None else hist.shape[1],
-            _want(hist_len, "hist_len", dev, i32, r), _want(n_prompt, "n_prompt", dev, i32, r),
-            _want(rep, "rep", dev, f32, r), _want(freq, "freq", dev, f32, r), _want(pres, "pres", dev, f32, r),
-            _want(bias_ids, "bias_ids", dev, i32, None), _want(bias, "bias", dev, f32, None),
-            0 if bias is None else bias.shape[1], _want(bias_len, "bias_len", dev, i32, r),
-            _want(mask, "mask", dev, i32, None), self.words)
-        self.ref = C.byref(self.c)
+            want(hist, "hist", i32), 0 if hist is None else hist.shape[1], want(hist_len, "hist_len", i32, r),
+            want(n_prompt, "n_prompt", i32, r), want(rep, "rep", f32, r), want(freq, "freq", f32, r),
+            want(pres, "pres", f32, r), want(bias_ids, "bias_ids", i32), want(bias, "bias", f32),
+            0 if bias is None else bias.shape[1], want(bias_len, "bias_len", i32, r), want(mask, "mask", i32),
+            0 if mask is None else mask.shape[1])
+        self.ref = C.addressof(self.c)
 
 
 def logits_dev(out, x, token, adjust=None, stream=None):
     """Adjusted logits of x [rows, vocab] into out (None: not wanted; may be
     x), and the greedy tokens into token [rows] (int32, or None)."""
-    dev = x.device
-    if x.dim() != 2 or x.stride(1) != 1 or not x.is_cuda:
+    i32 = _torch().int32
+    dev, shape, xs = x.get_device(), x.shape, x.stride()
+    if len(shape) != 2 or xs[1] != 1 or dev < 0:
         raise ValueError("x must be a CUDA tensor [rows, vocab] with unit-stride rows")
-    r, v = x.shape
-    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != dev or out.stride(1) != 1):
-        raise ValueError("out must be like x")
+    r, v = shape
+    po = so = 0
+    if out is not None:
+        so = out.stride()
+        if out.shape != shape or out.dtype is not x.dtype or out.get_device() != dev or so[1] != 1:
+            raise ValueError("out must be like x")
+        po, so = out.data_ptr(), so[0] if r > 1 else v
     if adjust is not None and adjust.rows is not None and (adjust.rows != r or adjust.device != dev):
         raise ValueError("the adjustments are for other rows or another device")
-    xs = x.stride(0) if r > 1 else v
-    os_ = 0 if out is None else (out.stride(0) if r > 1 else v)
-    _enqueue(lib().dsv4b_logits, "dsv4b_logits", dev, stream, None if out is None else out.data_ptr(), x.data_ptr(),
-             _dt(x, "x"), os_, xs, _want(token, "token", dev, ("int32",), (r,)),
-             None if adjust is None else adjust.ref, r, v)
+    _enqueue(lib().dsv4b_logits, "dsv4b_logits", dev, po, x.data_ptr(), _dt(x, "x"), so, xs[0] if r > 1 else v,
+             None if token is None else _want(token, "token", dev, i32, (r,)), None if adjust is None else adjust.ref,
+             r, v, _stream(dev, stream))
 
 
 # ------------------------------------------------------------- whole model

@@ -112,19 +112,33 @@ __device__ __forceinline__ void st_row8(void *p, size_t i, const float (&v)[8])
     }
 }
 
-// Cosine and sine of pos * freq. The product and its reduction to [-pi, pi]
-// are in double (2 pi as a double and its remainder: for |angle| < 2^31 the
-// reduced angle is off by less than 1e-15); both results are rounded to float
-// once.
+// Cosine and sine of pos * freq. The product and its reduction to [-pi/4,
+// pi/4] are in double (pi/2 as a double and its remainder: for |angle| < 2^31
+// the reduced angle is off by less than 1e-15), and so are the Taylor sums,
+// cut at r^13 / 13! and r^12 / 12!, which leaves less than 2^-40: the one
+// rounding that counts is the float's. Twelve independent-by-halves fused
+// steps, where the general double functions take 5 us of an 8 us rotation.
 __device__ __forceinline__ float2 rope_angle(int pos, double freq)
 {
     const double th = (double)pos * freq;
-    const double n = rint(th * 0.15915494309189535);
-    double r = fma(-n, 6.283185307179586, th);
-    r = fma(-n, 2.4492935982947064e-16, r);
-    double s, c;
-    sincos(r, &s, &c);
-    return make_float2((float)c, (float)s);
+    const double n = rint(th * 0.63661977236758134);
+    double r = fma(-n, 1.5707963267948966, th);
+    r = fma(-n, 6.123233995736766e-17, r);
+    const double z = r * r;
+    double s = fma(z, 1.0 / 6227020800.0, -1.0 / 39916800.0);
+    double c = fma(z, 1.0 / 479001600.0, -1.0 / 3628800.0);
+    s = fma(z, s, 1.0 / 362880.0);
+    c = fma(z, c, 1.0 / 40320.0);
+    s = fma(z, s, -1.0 / 5040.0);
+    c = fma(z, c, -1.0 / 720.0);
+    s = fma(z, s, 1.0 / 120.0);
+    c = fma(z, c, 1.0 / 24.0);
+    s = fma(z, s, -1.0 / 6.0);
+    c = fma(z, c, -0.5);
+    const float fs = (float)fma(r * z, s, r), fc = (float)fma(z, c, 1.0);
+    const int q = (int)__double2ll_rn(n) & 3;      // quarter turns
+    const float x = q & 1 ? fs : fc, y = q & 1 ? fc : fs;
+    return make_float2((q + 1) & 2 ? -x : x, q & 2 ? -y : y);
 }
 
 // (a, b) turned by the angle of cs = (cos, sin), each product rounded.

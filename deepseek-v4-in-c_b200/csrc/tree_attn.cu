@@ -84,15 +84,17 @@ constexpr int TA_SPLITS = 128;
 constexpr int TA_NONE = -1000;                      // scale reference before the first tile
 constexpr float TA_RAISE = 8.0f;                    // log2 of a weight that raises the reference
 
-struct Parts {              // one entry per (sequence, split, row)
-    float *o;               // [d] the split's own average
+struct Parts {              // one entry per (block, row of its tile)
+    float *o;               // [d] the block's own average
     float2 *ml;             // reference (log2) and sum of its weights
+    int2 *seq;              // per sequence: its first block, blocks a row tile
 };
 
 struct Args {
     TreeAttn a;
     Parts part;
-    int nch, stages, ring, page_shift, nsplit, per; // chunks of a row; TMEM pairs; tiles of a split
+    int nch, stages, ring, page_shift, nr;          // chunks of a row; TMEM pairs; rows of a tile
+    int nsplit, per;                                // splits and their key tiles when all contexts are the longest
 };
 
 struct Shared {             // behind the operand tiles
@@ -103,6 +105,7 @@ struct Shared {             // behind the operand tiles
     float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
     int wk[TA_SOFT], kx[TA_KEYS];       // (raises); scale byte of each key of the tile, -1: not there
     float scale[2];         // 2^E of each half of the rows
+    int seq, tile, tb, nt;  // the block's share: sequence (-1: none), row tile, first key tile, key tiles
     uint32_t tmem;
     int dead;
 };
@@ -272,6 +275,71 @@ __device__ __forceinline__ float across(const float (&x)[N], float none, int lan
     return v[0];
 }
 
+// The block's share of the work, by one warp. The host cuts every context as
+// if it were the longest (it does not know the lengths); here the blocks that
+// shorter contexts and smaller trees leave over go to the others: key tiles a
+// block = the fewest for which all sequences' blocks fit in the grid. (Eight
+// contexts of 9k to 32k positions: 126 us cut by the longest, SHARE_US so.)
+// Sequences are numbered through, a sequence's row tiles in turn, the splits
+// of a row tile side by side.
+constexpr int TA_STASH = 4096;              // sequences whose lengths fit in `len`; more keep the host's cut
+template <int NR>
+__device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int lane)
+{
+    const TreeAttn &a = g.a;
+    const bool even = g.nsplit > 1 && a.batch <= TA_STASH;
+    auto length = [&](int b) {              // key tiles and row tiles of sequence b
+        const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
+        const int n = min(max(__ldcg(a.ctx + b), 0), a.max_ctx) + nd;
+        return nd ? make_int2((n + TA_KEYS - 1) / TA_KEYS, (nd * a.n_heads + NR - 1) / NR) : make_int2(0, 0);
+    };
+    int per = g.per;
+    if (even) {
+        int top = 1;
+        for (int b = lane; b < a.batch; b += 32) {
+            len[b] = length(b);
+            top = max(top, len[b].x);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        for (int lo = (top + TA_SPLITS - 1) / TA_SPLITS; lo < per;) {
+            const int mid = (lo + per) >> 1;
+            unsigned blocks = 0;
+            for (int b = lane; b < a.batch; b += 32)
+                blocks = min(blocks + len[b].y * ((len[b].x + mid - 1) / mid), 1u << 26);
+            if (__reduce_add_sync(0xffffffffu, blocks) <= gridDim.x) per = mid;
+            else lo = mid + 1;
+        }
+    }
+    unsigned first = 0;                     // block of sequence b0's first
+    int seq = -1, tile = 0, tb = 0, nt = 0;
+    for (int b0 = 0; b0 < a.batch && seq < 0; b0 += 32) {
+        const int b = b0 + lane;
+        const int2 l = b >= a.batch ? make_int2(0, 0) : even ? len[b] : length(b);
+        const int ns = (l.x + per - 1) / per;
+        const unsigned mine = l.y * ns;
+        unsigned end = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned up = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += up;
+        }
+        end += first;
+        const unsigned here = __ballot_sync(0xffffffffu, blockIdx.x < end);
+        first = __shfl_sync(0xffffffffu, end, 31);
+        if (!here) continue;
+        seq = b0 + __ffs(here) - 1;
+        if (lane == __ffs(here) - 1) {
+            const int at = blockIdx.x - (end - mine), split = at % ns, even_per = (l.x + ns - 1) / ns;
+            tile = at / ns;
+            tb = split * even_per;
+            nt = min(l.x - tb, even_per);
+            if (at == 0 && g.nsplit > 1) g.part.seq[b] = make_int2((int)(end - mine), ns);
+            sh.tile = tile, sh.tb = tb, sh.nt = nt;
+        }
+    }
+    if (lane == 0) sh.seq = seq;
+}
+
 template <int NR>
 __global__ void __launch_bounds__(TA_T, 1)
 k_tree_attn(const __grid_constant__ Args g)
@@ -282,18 +350,7 @@ k_tree_attn(const __grid_constant__ Args g)
     const TreeAttn &a = g.a;
     extern __shared__ unsigned char ta_raw[];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int split = blockIdx.x, b = blockIdx.z, H = a.n_heads, d = a.c.d, nch = g.nch, ST = g.stages;
-    const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
-    const int r0 = blockIdx.y * NR, R = nd * H;
-    if (r0 >= R) return;
-    const int nr = min(NR, R - r0);
-    const int ctx = min(max(__ldcg(a.ctx + b), 0), a.max_ctx), n = ctx + nd;
-    const int tb = split * g.per, nt = min((n + TA_KEYS - 1) / TA_KEYS - tb, g.per);
-    const size_t prow = ((size_t)b * g.nsplit + split) * a.n_tok * H + r0;
-    if (nt <= 0) {
-        for (int r = tid; r < nr; r += TA_T) g.part.ml[prow + r] = make_float2(-INFINITY, 0.0f);
-        return;
-    }
+    const int H = a.n_heads, d = a.c.d, nch = g.nch, ST = g.stages;
     const uint32_t base = (tc::smem_u32(ta_raw) + 1023u) & ~1023u;
     const uint32_t q_s = base, p_s = q_s + nch * NR * 128, kv_s = p_s + TA_KEYS * 128;
     Shared &sh = *reinterpret_cast<Shared *>(ta_raw + (kv_s - tc::smem_u32(ta_raw)) + ST * nch * TA_SLOT);
@@ -301,6 +358,7 @@ k_tree_attn(const __grid_constant__ Args g)
     const int npair = (nch + 1) >> 1;
 
     if (warp == TA_WMMA) tc::tmem_alloc(tc::smem_u32(&sh.tmem), 512);
+    if (warp == 1) share<NR>(g, sh, reinterpret_cast<int2 *>(ta_raw + (base - tc::smem_u32(ta_raw))), lane);
     if (tid == 0) {
         for (int p = 0; p < npair; p++)
             for (int s = 0; s < ST; s++) {
@@ -324,6 +382,18 @@ k_tree_attn(const __grid_constant__ Args g)
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = sh.tmem;
+    // the same in every lane, which the compiler cannot see of a load
+    auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const int b = uniform(sh.seq);
+    if (b < 0) {
+        __syncthreads();
+        if (warp == TA_WMMA) tc::tmem_free(tmem, 512);
+        return;
+    }
+    const int r0 = uniform(sh.tile) * NR, tb = uniform(sh.tb), nt = uniform(sh.nt);
+    const int nd = uniform(a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok);
+    const int nr = min(NR, nd * H - r0), ctx = uniform(min(max(__ldcg(a.ctx + b), 0), a.max_ctx)), n = ctx + nd;
+    const size_t prow = (size_t)blockIdx.x * NR;
     const int nblk = npair;                             // 128-element blocks of O^T
     const uint32_t o_col = 0, s_col = nblk * NR, k_col = s_col + NR;    // TMEM columns
     const int KR = g.ring;
@@ -597,13 +667,14 @@ k_tree_attn(const __grid_constant__ Args g)
         float l[NC];
 #pragma unroll
         for (int i = 0; i < NC; i++) l[i] = 0.0f;
+        const int old = ctx - tb * TA_KEYS;             // context positions from the first tile on
         int E = TA_NONE;
         for (int j = 0; j < nt; j++) {
             warp_wait(&sh.key_full, j & 1, dead);
             const int kx = sh.kx[key];
             const bool valid = kx >= 0;
-            const int draft = (tb + j) * TA_KEYS + key - ctx;
-            const bool drafts = (tb + j + 1) * TA_KEYS > ctx;     // the tile holds drafted rows
+            const int draft = j * TA_KEYS + key - old;
+            const bool drafts = (j + 1) * TA_KEYS > old;          // the tile holds drafted rows
             const float ks = e8m0((uint8_t)kx);         // NaN for a NaN row: so are its scores and weights
             warp_wait(&sh.s_full, j & 1, dead);
             tc::fence_after();
@@ -795,14 +866,16 @@ k_tree_join(const __grid_constant__ Args g)
     const int H = a.n_heads, r = blockIdx.x, b = blockIdx.y, t = r / H, d = a.c.d, tid = threadIdx.x, lane = tid & 31;
     const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
     if (t >= nd) return;
-    const size_t rows = (size_t)a.n_tok * H, p0 = (size_t)b * g.nsplit * rows + r;
+    const int2 seq = __ldcg(g.part.seq + b);
+    const int nsplit = seq.y;
+    const size_t rows = g.nr, p0 = ((size_t)seq.x + (size_t)(r / g.nr) * nsplit) * rows + r % g.nr;
     if (tid < 32) {
         float2 ml[TA_SPLITS / 32];
         float M = -INFINITY;
 #pragma unroll
         for (int i = 0; i < TA_SPLITS / 32; i++) {
             const int s = lane + 32 * i;
-            ml[i] = s < g.nsplit ? __ldcg(g.part.ml + p0 + s * rows) : make_float2(-INFINITY, 0.0f);
+            ml[i] = s < nsplit ? __ldcg(g.part.ml + p0 + s * rows) : make_float2(-INFINITY, 0.0f);
             M = fmaxf(M, ml[i].x);
         }
         M = warp_max_f(M);
@@ -818,13 +891,13 @@ k_tree_join(const __grid_constant__ Args g)
         const float inv = den == 0.0f ? 0.0f : 1.0f / den;
 #pragma unroll
         for (int i = 0; i < TA_SPLITS / 32; i++)
-            if (lane + 32 * i < g.nsplit) wt[lane + 32 * i] = ml[i].y * inv;
+            if (lane + 32 * i < nsplit) wt[lane + 32 * i] = ml[i].y * inv;
     }
     __syncthreads();
     const size_t o = ((size_t)b * a.n_tok + t) * a.o_tok + (size_t)(r - t * H) * d;
     for (int e = 4 * tid; e < d; e += 512) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < g.nsplit; s++) {
+        for (int s = 0; s < nsplit; s++) {
             const float w = wt[s];
             if (w == 0.0f) continue;                    // nothing in it, or nothing of it left
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(g.part.o + (p0 + s * rows) * d + e));
@@ -837,9 +910,12 @@ k_tree_join(const __grid_constant__ Args g)
     }
 }
 
-// How a call is cut: rows of a tile, splits of the context, tiles of a split.
+// How a call is cut: rows of a tile, splits of the context, key tiles of a
+// split; blocks in all (where contexts are split, whole waves of 148: shorter
+// contexts leave some to the others).
 struct Plan {
     int nr, tiles, nsplit, per;
+    long blocks;
 };
 
 // The pair (rows of a tile, splits) of least time on 148 SMs, one block each,
@@ -858,8 +934,7 @@ Plan plan(int n_heads, int d, int n_tok, int batch, int max_ctx)
     for (int i = d <= 512 ? 3 : 2; i >= 0; i--) {
         const int nr = 16 * (i + 1);
         const long tiles = (R + nr - 1) / nr, units = tiles * batch;
-        if (tiles > 65535) continue;
-        for (int s = 1; s <= TA_SPLITS && s <= kt; s++) {
+        for (int s = 1; s <= TA_SPLITS && s <= kt && units * s <= 0x7fffff00l; s++) {
             const int per = (kt + s - 1) / s;
             if ((kt + per - 1) / per != s) continue;
             double c = (double)((units * s + 147) / 148) * (per * tile_us[i] + block_us[i]);
@@ -867,7 +942,7 @@ Plan plan(int n_heads, int d, int n_tok, int batch, int max_ctx)
             if (s > 1) c += 3.0 + (double)s * batch * R * d * 8 / 6.5e6;
             if (best.nr == 0 || c < cost) {
                 cost = c;
-                best = {nr, (int)tiles, s, per};
+                best = {nr, (int)tiles, s, per, s == 1 ? units : (units * s + 147) / 148 * 148};
             }
         }
     }
@@ -879,7 +954,7 @@ int run(const Args &g, const Plan &p, size_t smem, cudaStream_t st)
 {
     if (smem_optin(k_tree_attn<NR>, TA_SMEM)) return -2;
     PdlChain chain;
-    launch(k_tree_attn<NR>, dim3(p.nsplit, p.tiles, g.a.batch), dim3(TA_T), smem, st, g);
+    launch(k_tree_attn<NR>, dim3((unsigned)p.blocks), dim3(TA_T), smem, st, g);
     if (p.nsplit > 1) launch(k_tree_join, dim3(g.a.n_tok * g.a.n_heads, g.a.batch), dim3(128), 0, st, g);
     return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
 }
@@ -890,7 +965,7 @@ size_t tree_attn_bytes(int n_heads, int d, int n_tok, int batch, int max_ctx)
 {
     const Plan p = plan(n_heads, d, n_tok, batch, max_ctx);
     if (p.nsplit == 1) return 16;
-    return (size_t)batch * p.nsplit * n_tok * n_heads * ((size_t)d * 4 + sizeof(float2)) + 16;
+    return (size_t)p.blocks * p.nr * ((size_t)d * 4 + sizeof(float2)) + (size_t)batch * sizeof(int2) + 16;
 }
 
 int tree_attn(const TreeAttn &a, void *scratch, cudaStream_t st)
@@ -903,7 +978,10 @@ int tree_attn(const TreeAttn &a, void *scratch, cudaStream_t st)
     g.per = p.per;
     while ((1 << g.page_shift) < a.c.page_rows) g.page_shift++;
     g.part.o = reinterpret_cast<float *>(scratch);
-    g.part.ml = reinterpret_cast<float2 *>(g.part.o + (size_t)a.batch * p.nsplit * a.n_tok * a.n_heads * a.c.d);
+    const size_t prows = (size_t)p.blocks * p.nr;
+    g.part.ml = reinterpret_cast<float2 *>(g.part.o + prows * a.c.d);
+    g.part.seq = reinterpret_cast<int2 *>(g.part.ml + prows);
+    g.nr = p.nr;
     const int fixed = 1024 + g.nch * p.nr * 128 + TA_KEYS * 128 + (int)sizeof(Shared);
     g.stages = (TA_SMEM - fixed) / (g.nch * TA_SLOT);
     if (g.stages > TA_STAGES) g.stages = TA_STAGES;

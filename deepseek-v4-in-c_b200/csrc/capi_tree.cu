@@ -144,6 +144,8 @@ extern "C" int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long 
     if (!aligned(o, 16) || !aligned(q, 16) || !aligned(pages, 4) || !aligned(ctx, 4) || !aligned(mask, 8) ||
         !aligned(scratch, 16) || !aligned(sink, 4) || !aligned(n_draft, 4))
         return -1;
+    // the kernel holds a row's place as 32 bits of 64-byte steps
+    if ((long long)c->n_pages * c->page_rows > 0xFFFFFFFEll / ((c->d + c->tail) >> 6)) return -1;
     const long w = (long)n_heads * c->d;
     if (o_tok < w || q_tok < w || (o_tok & 7) || (q_tok & 7)) return -1;
     if (max_pages < 1 || (long long)max_pages * c->page_rows < (long long)max_ctx + n_tok) return -1;

@@ -165,6 +165,24 @@ def test_tree_attn_refusals():
         assert call("dsv4b_tree_attn", args, **bad) == -1, bad
 
 
+def test_tree_attn_refuses_caches_past_its_offsets():
+    """A row's place is kept in 32 bits of 64-byte steps."""
+    no_device()
+    args = dict(o=P, q=Q, dt=B.BF16, o_tok=64 * 512, q_tok=64 * 512, c=None, pages=P, max_pages=16, ctx=P, n_draft=None,
+                mask=P, sink=None, n_heads=64, n_tok=8, batch=2, max_ctx=1000, scale=0.1, scratch=P,
+                bytes=B.tree_attn_scratch(64, 512, 8, 2, 1000), stream=None)
+    steps = (512 + 64) // 64
+    most = (2 ** 32 - 2) // steps // 64                   # pages of 64 rows
+    assert call("dsv4b_tree_attn", args, c=cache(n_pages=most)) == -2
+    assert call("dsv4b_tree_attn", args, c=cache(n_pages=most + 1)) == -1
+    assert call("dsv4b_tree_attn", args, c=cache(n_pages=2 ** 31 - 1)) == -1
+
+
+def test_status_without_a_device():
+    no_device()
+    assert B.lib().dsv4b_tree_attn_status() == -1
+
+
 def test_logits_refusals():
     no_device()
     full = dict(hist=P, hist_stride=9, hist_len=P, n_prompt=P, rep=P, freq=P, pres=P, bias_ids=P, bias=P,

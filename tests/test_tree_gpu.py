@@ -542,6 +542,74 @@ def test_tree_attn_strides_streams_and_graphs():
         assert torch.equal(out, run_tree(k))
 
 
+def test_tree_attn_shares_blocks_by_length():
+    """Many sequences of very different lengths, some without tokens: the
+    blocks that short ones leave go to the long ones."""
+    k = tree_case(31, 70, 3, 16, 128, 64, 16, 2500, torch.bfloat16, ragged=True)
+    k["ctx"][5::7] = 0
+    k["ctx"][::11] = 2500
+    k["nd"][3::9] = 0
+    want, tol = plain_tree(k)
+    got = run_tree(k)
+    close(got, want, tol)
+    assert torch.equal(run_tree(k), got)
+    k["nd"].zero_()
+    assert torch.all(run_tree(k) == 11.0)                  # nothing drafted: nothing written
+
+
+def test_tree_attn_one_long_among_short():
+    k = tree_case(32, 33, 2, 64, 512, 64, 64, 3000, torch.float16)
+    k["ctx"].fill_(10)
+    k["ctx"][32] = 3000
+    want, tol = plain_tree(k)
+    close(run_tree(k), want, tol)
+
+
+def test_tree_attn_thousands_of_sequences():
+    """More sequences than the blocks share among, with room for long contexts."""
+    b, d, page = 4100, 64, 65536
+    c = B.KvCache.empty(2, page, d, 0)
+    x = normal(gen(33), 600, d)
+    at = torch.cat((torch.arange(300), page + torch.arange(300))).cuda()
+    B.kv_write_dev(c, x, at)
+    pages = torch.zeros((b, 17), dtype=torch.int32, device="cuda")
+    pages[:, 0] = torch.arange(b, device="cuda") % 2
+    g = gen(34)
+    ctx = torch.randint(0, 299, (b,), generator=g, device="cuda", dtype=torch.int32)
+    q = normal(g, b, 1, 2, d).bfloat16()
+    k = dict(c=c, pages=pages, ctx=ctx, nd=torch.ones(b, dtype=torch.int32, device="cuda"),
+             mask=torch.ones((b, 1), dtype=torch.int64, device="cuda"), q=q, sink=None, scale=0.2, max_ctx=1 << 20)
+    got = run_tree(k)
+    some = torch.tensor([0, 1, 31, 32, 4095, 4096, 4099], device="cuda")
+    part = dict(k, pages=pages[some], ctx=ctx[some], nd=k["nd"][some], mask=k["mask"][some], q=q[some])
+    want, tol = plain_tree(part)
+    close(got[some], want, tol)
+    assert torch.all((got != 11.0).any(-1))                # every sequence has been written
+
+
+def test_two_streams_at_once():
+    """Calls on two streams at a time, each with scratch of its own."""
+    k = [tree_case(35 + i, 2, 4, 64, 512, 64, 64, 1500, torch.bfloat16, ragged=bool(i)) for i in range(2)]
+    ref = [run_tree(x) for x in k]
+    x = 3 * normal(gen(37), 2, 20000)
+    tok = torch.empty(2, dtype=torch.int32, device="cuda")
+    B.logits_dev(None, x, tok)
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    room = [torch.empty(B.tree_attn_scratch(64, 512, 4, 2, 1500), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    outs = [[torch.full_like(r, 11.0) for _ in range(6)] for r in ref]
+    toks = [[torch.empty_like(tok) for _ in range(6)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for n in range(6):
+        for i in range(2):
+            run_tree(k[i], out=outs[i][n], scratch=room[i], stream=side[i])
+            B.logits_dev(None, x, toks[i][n], stream=side[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, ref[i]) for o in outs[i]) and all(torch.equal(t, tok) for t in toks[i])
+    assert B.lib().dsv4b_tree_attn_status() == 0           # no bounded wait has run out
+
+
 def _after(stream, fn):
     out = fn()
     stream.synchronize()

@@ -72,8 +72,8 @@ constexpr int TA_T = 32 * (TA_WMMA + 4);
 // leaves next to no L1, so a spilled register comes back from L2).
 template <int NR>
 struct Regs {
-    static constexpr int soft = NR == 64 ? 128 : NR == 48 ? 112 : 88, load = NR == 64 ? 64 : 72;
-    static constexpr int copy = NR >= 48 ? 48 : 56, mma = NR == 64 ? 24 : 40;
+    static constexpr int soft = NR == 64 ? 128 : NR == 48 ? 112 : 88, load = NR == 64 ? 56 : 72;
+    static constexpr int copy = NR >= 48 ? 48 : 56, mma = 40;
     static_assert(2 * (soft + load + copy) + mma <= 7 * 72, "more registers than the block is launched with");
 };
 constexpr int TA_ROWS = 64;                         // most rows of a tile (N)
@@ -106,6 +106,7 @@ struct Shared {             // behind the operand tiles
     int wk[TA_SOFT], kx[TA_KEYS];       // (raises); scale byte of each key of the tile, -1: not there
     float scale[2];         // 2^E of each half of the rows
     int seq, tile, tb, nt;  // the block's share: sequence (-1: none), row tile, first key tile, key tiles
+    int ctx, nd;            // the sequence's context and drafted tokens
     uint32_t tmem;
     int dead;
 };
@@ -197,23 +198,27 @@ template <int NR>
 __device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t q_s, int r0, int nr, int b, int w, int lane)
 {
     const int H = a.n_heads, d = a.c.d;
-#pragma unroll 1
-    for (int r = w; r < NR; r += TA_SOFT + TA_COPY) {
+    constexpr int NV = NR == 64 ? 2 : 3;        // 256-element parts of a row: 64 rows go with d <= 512
+    auto row = [&](int r) {
         const int t = (r0 + r) / H;
-        const unsigned short *q = reinterpret_cast<const unsigned short *>(a.q) +
-                                  ((size_t)b * a.n_tok + t) * a.q_tok + (size_t)(r0 + r - t * H) * d;
-        uint4 v[3];
+        return reinterpret_cast<const unsigned short *>(a.q) + ((size_t)b * a.n_tok + t) * a.q_tok +
+               (size_t)(r0 + r - t * H) * d;
+    };
+    auto read = [&](int r, uint4 (&v)[NV]) {
+        const unsigned short *q = row(r);
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
+        for (int i = 0; i < NV; i++) {
             const int e = i * 256 + lane * 8;
             v[i] = make_uint4(0, 0, 0, 0);
             if (r < nr && e < d) v[i] = __ldcg(reinterpret_cast<const uint4 *>(q + e));
         }
+    };
+    auto put = [&](int r, uint4 (&v)[NV]) {
         int kq = 0;
         if (a.dt == DSV4B_BF16) {
             uint32_t top2 = 0;          // magnitudes order as 16-bit integers
 #pragma unroll
-            for (int i = 0; i < 3; i++) {
+            for (int i = 0; i < NV; i++) {
                 if (i * 256 >= d) break;
                 top2 = __vmaxs2(top2, __vmaxs2(__vmaxs2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu), __vmaxs2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
             }
@@ -222,7 +227,7 @@ __device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t 
                 top = 0;
 #pragma unroll 1
                 for (int i = 0; i < d / 32; i++) {
-                    const uint32_t m = r < nr ? __ldcg(q + i * 32 + lane) & 0x7FFFu : 0u;
+                    const uint32_t m = r < nr ? __ldcg(row(r) + i * 32 + lane) & 0x7FFFu : 0u;
                     if (m < 0x7F80u) top = max(top, m);
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
@@ -230,7 +235,7 @@ __device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t 
             if (top) kq = max((int)(top >> 7) - 127 - 14, -112);
             const float f = pow2i(-kq);
 #pragma unroll
-            for (int i = 0; i < 3; i++) {
+            for (int i = 0; i < NV; i++) {
                 if (i * 256 >= d) break;
                 uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
@@ -243,7 +248,7 @@ __device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t 
         }
         const uint32_t dst = q_s + r * 128;
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
+        for (int i = 0; i < NV; i++) {
             const int e = i * 256 + lane * 8;
             if (e >= d) continue;
             // elements 16 q + 4 i go to place 16 i + 4 q of the chunk
@@ -252,7 +257,26 @@ __device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t 
             st_smem8(chunk + ((32 * (i4 + 1) + 8 * q4) ^ sw), v[i].z, v[i].w);
         }
         if (lane == 0) sh.cq[r] = a.scale * 1.4426950408889634f * pow2i(kq);
+    };
+    // two rows' loads at a time
+    constexpr int W = TA_SOFT + TA_COPY;
+    uint4 v[NV], u[NV];
+#pragma unroll 1
+    for (int r = w; r < NR; r += 2 * W) {
+        read(r, v);
+        if (r + W < NR) read(r + W, u);
+        put(r, v);
+        if (r + W < NR) put(r + W, u);
     }
+}
+
+
+// The largest of a warp's values; a NaN counts only among NaN.
+__device__ __forceinline__ float warp_top(float x)
+{
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // Combine N values per lane over the 32 lanes of a warp: lane i gets the
@@ -289,9 +313,10 @@ __device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int 
 {
     const TreeAttn &a = g.a;
     const bool even = g.nsplit > 1 && a.batch <= TA_STASH;
+    auto drafted = [&](int b) { return a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok; };
+    auto context = [&](int b) { return min(max(__ldcg(a.ctx + b), 0), a.max_ctx); };
     auto length = [&](int b) {              // key tiles and row tiles of sequence b
-        const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
-        const int n = min(max(__ldcg(a.ctx + b), 0), a.max_ctx) + nd;
+        const int nd = drafted(b), n = context(b) + nd;
         return nd ? make_int2((n + TA_KEYS - 1) / TA_KEYS, (nd * a.n_heads + NR - 1) / NR) : make_int2(0, 0);
     };
     int per = g.per;
@@ -302,13 +327,23 @@ __device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int 
             top = max(top, len[b].x);
         }
         top = __reduce_max_sync(0xffffffffu, top);
+        // eight parts a step: its seven counts do not wait for one another
         for (int lo = (top + TA_SPLITS - 1) / TA_SPLITS; lo < per;) {
-            const int mid = (lo + per) >> 1;
-            unsigned blocks = 0;
-            for (int b = lane; b < a.batch; b += 32)
-                blocks = min(blocks + len[b].y * ((len[b].x + mid - 1) / mid), 1u << 26);
-            if (__reduce_add_sync(0xffffffffu, blocks) <= gridDim.x) per = mid;
-            else lo = mid + 1;
+            const int step = (per - lo + 7) >> 3;
+            unsigned blocks[7] = {};
+            for (int b = lane; b < a.batch; b += 32) {
+                const int2 l = len[b];
+#pragma unroll
+                for (int i = 0; i < 7; i++) {
+                    const int mid = lo + i * step;
+                    blocks[i] = min(blocks[i] + l.y * ((l.x + mid - 1) / mid), 1u << 26);
+                }
+            }
+            int more = 0;                   // candidates lo, lo + step, ... that need too many blocks
+#pragma unroll
+            for (int i = 0; i < 7; i++) more += __reduce_add_sync(0xffffffffu, blocks[i]) > gridDim.x;
+            if (more < 7) per = min(per, lo + more * step);
+            if (more > 0) lo = min(per, lo + (more - 1) * step + 1);
         }
     }
     unsigned first = 0;                     // block of sequence b0's first
@@ -336,6 +371,7 @@ __device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int 
             nt = min(l.x - tb, even_per);
             if (at == 0 && g.nsplit > 1) g.part.seq[b] = make_int2((int)(end - mine), ns);
             sh.tile = tile, sh.tb = tb, sh.nt = nt;
+            sh.ctx = context(b), sh.nd = drafted(b);
         }
     }
     if (lane == 0) sh.seq = seq;
@@ -392,8 +428,7 @@ k_tree_attn(const __grid_constant__ Args g)
         return;
     }
     const int r0 = uniform(sh.tile) * NR, tb = uniform(sh.tb), nt = uniform(sh.nt);
-    const int nd = uniform(a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok);
-    const int nr = min(NR, nd * H - r0), ctx = uniform(min(max(__ldcg(a.ctx + b), 0), a.max_ctx)), n = ctx + nd;
+    const int nd = uniform(sh.nd), ctx = uniform(sh.ctx), nr = min(NR, nd * H - r0), n = ctx + nd;
     const size_t prow = (size_t)blockIdx.x * NR;
     const int nblk = npair;                             // 128-element blocks of O^T
     const uint32_t o_col = 0, s_col = nblk * NR, k_col = s_col + NR;    // TMEM columns
@@ -725,7 +760,12 @@ k_tree_attn(const __grid_constant__ Args g)
                 // takes no NaN)
                 scores(false);
                 free_s();
-                const float mine = across<NC>(x, -INFINITY, lane, [](float p, float q) { return fmaxf(p, q); });
+                float mine = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    const float m = warp_top(x[i]);
+                    if (lane == i) mine = m;
+                }
                 if (lane < NC) sh.wmax[warp & 3][c0 + lane] = fmaxf(mine, -INFINITY);
                 const int kw = __reduce_max_sync(0xffffffffu, valid && kx < 255 ? kx : TA_NONE);
                 if (lane == 0) sh.wk[warp] = kw;
@@ -866,8 +906,8 @@ k_tree_join(const __grid_constant__ Args g)
     __shared__ float wt[TA_SPLITS];
     const int H = a.n_heads, r = blockIdx.x, b = blockIdx.y, t = r / H, d = a.c.d, tid = threadIdx.x, lane = tid & 31;
     const int nd = a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok;
+    const int2 seq = __ldcg(g.part.seq + b);    // of a sequence without tokens: not written, not used
     if (t >= nd) return;
-    const int2 seq = __ldcg(g.part.seq + b);
     const int nsplit = seq.y;
     const size_t rows = g.nr, p0 = ((size_t)seq.x + (size_t)(r / g.nr) * nsplit) * rows + r % g.nr;
     if (tid < 32) {
@@ -898,6 +938,7 @@ k_tree_join(const __grid_constant__ Args g)
     const size_t o = ((size_t)b * a.n_tok + t) * a.o_tok + (size_t)(r - t * H) * d;
     for (int e = 4 * tid; e < d; e += 512) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int s = 0; s < nsplit; s++) {
             const float w = wt[s];
             if (w == 0.0f) continue;                    // nothing in it, or nothing of it left

@@ -427,7 +427,8 @@ int dsv4b_kv_read(const dsv4b_kvq *c, void *out, int dt, long row_stride, const 
  * to the drafted positions ctx[b] + k whose bit k is set in mask[b][t] (its
  * ancestors, and usually itself), whose rows have been written at those
  * positions; position j is row j % page_rows of page pages[b][j / page_rows]
- * (a page outside the cache is skipped). Keys and values are the same rows,
+ * (a page outside the cache is skipped; a cache holds less than 2^38 bytes of
+ * codes). Keys and values are the same rows,
  * shared by all heads; sink[h] (may be NULL) joins the denominator only
  * (src/core/dsv4_attn.c:60-108); with nothing to attend to the output is
  * zero. Tokens t >= n_draft[b] are not written (n_draft NULL: n_tok each).
@@ -449,7 +450,8 @@ int dsv4b_tree_attn_status(void);
 
 /* What to do to the logits of each row; a NULL array is off. hist
  * [rows][hist_stride] holds the row's hist_len tokens, the first n_prompt of
- * them its prompt (ids outside the vocabulary are ignored); bias / bias_ids
+ * them its prompt (ids outside the vocabulary are ignored; hist_stride and
+ * bias_stride up to 2^30); bias / bias_ids
  * [rows][bias_stride] its bias_len biases (of a token named twice, the sum);
  * mask [rows][mask_stride] one bit per token, bit v % 32 of word v / 32, 1 =
  * allowed. rep, freq and pres need hist. */

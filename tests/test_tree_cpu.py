@@ -203,3 +203,6 @@ def test_logits_refusals():
                 dict(adj=adj(bias_ids=None)), dict(adj=adj(bias_len=None)), dict(adj=adj(bias=None)),
                 dict(adj=adj(bias_stride=-1)), dict(adj=adj(mask_stride=31)), dict(adj=adj(mask=P + 2))):
         assert call("dsv4b_logits", args, **bad) == -1, bad
+    assert call("dsv4b_logits", args, adj=adj(hist_stride=1 << 30)) == -2
+    for bad in (adj(hist_stride=(1 << 30) + 1), adj(bias_stride=(1 << 30) + 1)):
+        assert call("dsv4b_logits", args, adj=bad) == -1

@@ -35,7 +35,7 @@
 // pairs of 128 elements:
 //   8 widening warps four threads to a key: read the codes (64-byte runs, one
 //                    or two pairs in flight), widen e4m3 to f16 -- exact, the
-//                    row scale stays outside -- into a TMEM ring of 3 or 4
+//                    row scale stays outside -- into a TMEM ring of 2 to 4
 //                    pairs;
 //   8 copying warps  from there to shared memory once the second product has
 //                    freed the pair's place (128-byte swizzle; V^T is the
@@ -47,7 +47,7 @@
 //
 // Measured (d 512, 64 heads, bf16): 16 tokens on 4 contexts of 32768 positions
 // 416 us, 660 TFLOP/s; 7 tokens on 8 contexts of up to 4100 39 us; one token on
-// 700 positions 13 us. With d 576, one token on 8 contexts of 32768 122 us. What
+// 700 positions 13 us. With d 576, one token on 8 contexts of 32768 99 us. What
 // bounds it is no unit but the hand-over between the roles: a tile of 64 rows
 // takes 6300 cycles, of which the MMAs need 2600, and leaving out all MMAs,
 // all exponentials or all loads shortens the call by 3, 0 and 5 %. Shared
@@ -89,8 +89,8 @@ struct Regs {
     static_assert(2 * (soft + load + copy) + mma <= 7 * 72, "more registers than the block is launched with");
 };
 constexpr int TA_ROWS = 64;                         // most rows of a tile (N)
-constexpr int TA_STAGES = 4, TA_PAIRS = 5;
 constexpr int TA_SLOT = TA_KEYS * 128;              // bytes of one 64-element chunk
+constexpr int TA_PLACES = 7;                        // most chunk pairs in shared memory
 constexpr int TA_SMEM = 232448;                     // a block's limit
 constexpr int TA_SPLITS = 128;
 constexpr int TA_NONE = -1000;                      // scale reference before the first tile
@@ -105,12 +105,12 @@ struct Parts {              // one entry per (block, row of its tile)
 struct Args {
     TreeAttn a;
     Parts part;
-    int nch, stages, ring, page_shift, nr;          // chunks of a row; TMEM pairs; rows of a tile
+    int nch, places, ring, page_shift, nr;          // chunks of a row; pairs in shared memory and in TMEM; rows of a tile
     int nsplit, per;                                // splits and their key tiles when all contexts are the longest
 };
 
 struct Shared {             // behind the operand tiles
-    uint64_t v_full[TA_STAGES * TA_PAIRS], v_empty[TA_STAGES * TA_PAIRS], k_full[TA_RING], k_done[TA_RING];
+    uint64_t v_full[TA_PLACES], v_empty[TA_PLACES], k_full[TA_RING], k_done[TA_RING];
     uint64_t q_full, key_full, s_full, s_free, p_full, pv_done;
     uint64_t rowmask[TA_ROWS], out_at[TA_ROWS];     // a row's tree mask, and its first output element
     float cq[TA_ROWS], nm[TA_ROWS];     // score factor of a row, and its negated reference
@@ -210,7 +210,7 @@ template <int NR>
 __device__ __forceinline__ void widen_q(const TreeAttn &a, Shared &sh, uint32_t q_s, int r0, int nr, int b, int w, int lane)
 {
     const int H = a.n_heads, d = a.c.d;
-    constexpr int NV = NR == 64 ? 2 : 3;        // 256-element parts of a row: 64 rows go with d <= 512
+    constexpr int NV = 3;                       // 256-element parts of a row
     auto row = [&](int r) {
         const int t = (r0 + r) / H;
         return reinterpret_cast<const unsigned short *>(a.q) + ((size_t)b * a.n_tok + t) * a.q_tok +
@@ -399,21 +399,20 @@ k_tree_attn(const __grid_constant__ Args g)
     const TreeAttn &a = g.a;
     extern __shared__ unsigned char ta_raw[];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int H = a.n_heads, d = a.c.d, nch = g.nch, ST = g.stages;
+    const int H = a.n_heads, d = a.c.d, nch = g.nch, VP = g.places;
     const uint32_t base = (tc::smem_u32(ta_raw) + 1023u) & ~1023u;
     const uint32_t q_s = base, p_s = q_s + nch * NR * 128, kv_s = p_s + TA_KEYS * 128;
-    Shared &sh = *reinterpret_cast<Shared *>(ta_raw + (kv_s - tc::smem_u32(ta_raw)) + ST * nch * TA_SLOT);
+    Shared &sh = *reinterpret_cast<Shared *>(ta_raw + (kv_s - tc::smem_u32(ta_raw)) + VP * 2 * TA_SLOT);
     volatile int *dead = &sh.dead;
     const int npair = (nch + 1) >> 1;
 
     if (warp == TA_WMMA) tc::tmem_alloc(tc::smem_u32(&sh.tmem), 512);
     if (warp == 1) share<NR>(g, sh, reinterpret_cast<int2 *>(ta_raw + (base - tc::smem_u32(ta_raw))), lane);
     if (tid == 0) {
-        for (int p = 0; p < npair; p++)
-            for (int s = 0; s < ST; s++) {
-                tc::mbar_init(tc::smem_u32(&sh.v_full[s * TA_PAIRS + p]), TA_COPY);
-                tc::mbar_init(tc::smem_u32(&sh.v_empty[s * TA_PAIRS + p]), 1);
-            }
+        for (int s = 0; s < VP; s++) {
+            tc::mbar_init(tc::smem_u32(&sh.v_full[s]), TA_COPY);
+            tc::mbar_init(tc::smem_u32(&sh.v_empty[s]), 1);
+        }
         for (int r = 0; r < g.ring; r++) {
             tc::mbar_init(tc::smem_u32(&sh.k_full[r]), TA_LOAD);
             tc::mbar_init(tc::smem_u32(&sh.k_done[r]), 1 + TA_COPY);
@@ -563,7 +562,7 @@ k_tree_attn(const __grid_constant__ Args g)
         const int quad = warp & 3, half = (warp - TA_WCOPY) >> 2, key = quad * 32 + lane;
         const uint32_t k_mine = tmem + ((uint32_t)quad << 21) + k_col + 32 * half, sw = key & 7;
         const int pairs = nt * npair;
-        int p = 0, slot = 0, kpar = 0, stage = 0, vpar = 1;
+        int p = 0, slot = 0, kpar = 0, place = 0, vpar = 1;
         for (int i = 0; i < pairs; i++) {
             const int c = 2 * p + half;
             uint32_t h[32];
@@ -575,9 +574,9 @@ k_tree_attn(const __grid_constant__ Args g)
                 tc::fence_before();
             }
             warp_arrive(&sh.k_done[slot], lane);
-            if (i >= ST * npair) warp_wait(&sh.v_empty[stage * TA_PAIRS + p], vpar, dead);
+            if (i >= VP) warp_wait(&sh.v_empty[place], vpar, dead);
             if (c < nch) {
-                const uint32_t dst = kv_s + (stage * nch + c) * TA_SLOT + key * 128;
+                const uint32_t dst = kv_s + (2 * place + half) * TA_SLOT + key * 128;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {           // elements 8k .. 8k + 7 are at places 32 (k % 2) + 4 (k / 2)
                     const int r = 16 * (k & 1) + 2 * (k >> 1);
@@ -585,12 +584,10 @@ k_tree_attn(const __grid_constant__ Args g)
                 }
                 tc::fence_async_smem();
             }
-            warp_arrive(&sh.v_full[stage * TA_PAIRS + p], lane);
+            warp_arrive(&sh.v_full[place], lane);
             if (++slot == KR) slot = 0, kpar ^= 1;
-            if (++p == npair) {
-                p = 0;
-                if (++stage == ST) stage = 0, vpar ^= 1;
-            }
+            if (++place == VP) place = 0, vpar ^= 1;
+            if (++p == npair) p = 0;
         }
     } else if (warp >= TA_WMMA) {
         // ------------------------------------------------------- MMA issue
@@ -630,25 +627,22 @@ k_tree_attn(const __grid_constant__ Args g)
             // a last single chunk: its second half repeats the first, into
             // TMEM lanes that nothing reads
             const uint64_t v_d2 = tc::sdesc(kv_s, TA_SLOT, 1024), v_d1 = tc::sdesc(kv_s, 0, 1024);
-            int p = 0, j = 0, stage = 0, vpar = 0;
+            int p = 0, j = 0, place = 0, vpar = 0;
             for (int v = 0; v < pairs; v++) {
                 if (p == 0) warp_wait(&sh.p_full, j & 1, dead);
-                warp_wait(&sh.v_full[stage * TA_PAIRS + p], vpar, dead);
+                warp_wait(&sh.v_full[place], vpar, dead);
                 tc::fence_after();
                 if (tc::elect_one()) {
-                    const uint64_t va = (2 * p + 1 < nch ? v_d2 : v_d1) + (uint64_t)((stage * nch + 2 * p) * (TA_SLOT >> 4));
+                    const uint64_t va = (2 * p + 1 < nch ? v_d2 : v_d1) + (uint64_t)(2 * place * (TA_SLOT >> 4));
 #pragma unroll
                     for (int k = 0; k < 8; k++)
                         tc::mma_f16(tmem + o_col + p * NR, va + 128 * k, p_d + 128 * k, id_o, j > 0 || k > 0);
-                    tc::mma_commit(tc::smem_u32(&sh.v_empty[stage * TA_PAIRS + p]));
+                    tc::mma_commit(tc::smem_u32(&sh.v_empty[place]));
                     if (p == npair - 1) tc::mma_commit(tc::smem_u32(&sh.pv_done));
                 }
                 __syncwarp();
-                if (++p == npair) {
-                    p = 0;
-                    j++;
-                    if (++stage == ST) stage = 0, vpar ^= 1;
-                }
+                if (++place == VP) place = 0, vpar ^= 1;
+                if (++p == npair) p = 0, j++;
             }
         }
         if (warp > TA_WMMA + 1) {
@@ -974,18 +968,21 @@ struct Plan {
 
 // The pair (rows of a tile, splits) of least time on 148 SMs, one block each,
 // by what a block costs: microseconds per tile and beside its tiles, measured
-// at d = 512 over 700 to 32768 positions. A tile's time hardly depends on its
-// rows (the 128 keys are widened all the same), so many rows win once the
-// blocks fill the machine, and few rows before that. At 64 rows Q, P and the
-// keys fit in shared memory up to d = 512.
+// over 700 to 32768 positions. A tile's time hardly depends on its rows (the
+// 128 keys are widened all the same), so many rows win once the blocks fill
+// the machine, and few rows before that. Past d = 512 a tile of 64 rows leaves
+// TMEM two pairs of keys and shared memory four of five: 5.2 us a tile, still
+// less than two tiles of 32 (one token on 8 contexts of 32768 at d = 576: 99
+// us, with 32 rows 124, with 48 137).
 Plan plan(int n_heads, int d, int n_tok, int batch, int max_ctx)
 {
-    static const double tile_us[4] = {2.9, 3.1, 3.2, 3.4}, block_us[4] = {9.0, 11.0, 12.5, 15.0};
+    static const double tile[2][4] = {{2.9, 3.1, 3.2, 3.4}, {3.3, 3.6, 4.1, 5.2}}, block_us[4] = {9.0, 11.0, 12.5, 15.0};
+    const double *tile_us = tile[d > 512];
     Plan best = {};
     double cost = 0.0;
     const long R = (long)n_heads * n_tok;
     const int kt = (max_ctx + n_tok + TA_KEYS - 1) / TA_KEYS;
-    for (int i = d <= 512 ? 3 : 2; i >= 0; i--) {
+    for (int i = 3; i >= 0; i--) {
         const int nr = 16 * (i + 1);
         const long tiles = (R + nr - 1) / nr, units = tiles * batch;
         for (int s = 1; s <= TA_SPLITS && s <= kt && units * s <= 0x7fffff00l; s++) {
@@ -1037,12 +1034,13 @@ int tree_attn(const TreeAttn &a, void *scratch, cudaStream_t st)
     g.part.seq = reinterpret_cast<int2 *>(g.part.ml + prows);
     g.nr = p.nr;
     const int fixed = 1024 + g.nch * p.nr * 128 + TA_KEYS * 128 + (int)sizeof(Shared);
-    g.stages = (TA_SMEM - fixed) / (g.nch * TA_SLOT);
-    if (g.stages > TA_STAGES) g.stages = TA_STAGES;
-    // at least 3 pairs: d <= 512 has 4 blocks of up to 64 columns, else 5 of 48
+    // at least 4: 64 rows of 576 elements leave 135 KB
+    g.places = (TA_SMEM - fixed) / (2 * TA_SLOT);
+    if (g.places > TA_PLACES) g.places = TA_PLACES;
+    // at least 2 pairs (64 rows, d > 512: 5 blocks of 64 columns beside S)
     g.ring = (512 - ((g.nch + 1) / 2 + 1) * p.nr) / 64;
     if (g.ring > TA_RING) g.ring = TA_RING;
-    size_t smem = (size_t)fixed + (size_t)g.stages * g.nch * TA_SLOT;
+    size_t smem = (size_t)fixed + (size_t)g.places * 2 * TA_SLOT;
     // one block per SM: each takes all of TMEM
     if (smem < 120 * 1024) smem = 120 * 1024;
     switch (p.nr) {

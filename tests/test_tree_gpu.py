@@ -557,6 +557,18 @@ def test_tree_attn_shares_blocks_by_length():
     assert torch.all(run_tree(k) == 11.0)                  # nothing drafted: nothing written
 
 
+@pytest.mark.parametrize("d,tail", [(64, 64), (128, 0), (256, 64), (384, 64), (448, 64), (512, 64), (576, 64)])
+@pytest.mark.parametrize("heads", [8, 64])
+def test_tree_attn_many_tiles(d, tail, heads):
+    """Every row width through many key tiles of one block: all places for keys
+    and values are used again and again."""
+    k = tree_case(40 + d, 37, 4, heads, d, tail, 64, 1400, torch.bfloat16)
+    if heads == 64:
+        k["ctx"][1:] = torch.arange(36, dtype=torch.int32, device="cuda")
+    want, tol = plain_tree(k)
+    close(run_tree(k), want, tol)
+
+
 def test_tree_attn_one_long_among_short():
     k = tree_case(32, 33, 2, 64, 512, 64, 64, 3000, torch.float16)
     k["ctx"].fill_(10)

@@ -228,6 +228,25 @@ def test_kv_round_trip(n, d, tail, page, src):
     assert torch.all(dest[:, :3] == 5.0) and torch.all(dest[:, 3 + d:] == 5.0)
 
 
+def test_kv_moved_rows_keep_their_values():
+    """Rows read into f32 and written elsewhere read back the same: a largest
+    code that was rounded down to a power of two halves the scale, which
+    doubles codes and tail exactly."""
+    g = gen(50)
+    n, d, tail = 2000, 512, 64
+    c = B.KvCache.empty(2 * n // 16, 16, d, tail)
+    x = normal(g, n, d) * torch.exp(4 * normal(g, n, 1))
+    x[::5] = x[::5].clamp(-1, 1) * 224.01 * 2.0 ** -9       # the largest just above half the range
+    x[3], x[4] = 0.0, float("nan")
+    at = torch.randperm(2 * n, generator=g, device="cuda")
+    first, then = torch.empty_like(x), torch.empty_like(x)
+    B.kv_write_dev(c, x, at[:n])
+    B.kv_read_dev(first, c, at[:n])
+    B.kv_write_dev(c, first, at[n:])
+    B.kv_read_dev(then, c, at[n:])
+    assert torch.equal(then.nan_to_num(nan=7.0), first.nan_to_num(nan=7.0)) and then[4].isnan().all()
+
+
 def test_kv_skipped_and_bad_values():
     c = B.KvCache.empty(3, 8, 128, 64)
     x = normal(gen(1), 6, 128)

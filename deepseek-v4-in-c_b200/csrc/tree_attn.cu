@@ -325,18 +325,19 @@ __device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int 
 {
     const TreeAttn &a = g.a;
     const bool even = g.nsplit > 1 && a.batch <= TA_STASH;
-    auto drafted = [&](int b) { return a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok; };
-    auto context = [&](int b) { return min(max(__ldcg(a.ctx + b), 0), a.max_ctx); };
-    auto length = [&](int b) {              // key tiles and row tiles of sequence b
-        const int nd = drafted(b), n = context(b) + nd;
-        return nd ? make_int2((n + TA_KEYS - 1) / TA_KEYS, (nd * a.n_heads + NR - 1) / NR) : make_int2(0, 0);
+    auto length = [&](int b) {              // context and drafted tokens of sequence b
+        return make_int2(min(max(__ldcg(a.ctx + b), 0), a.max_ctx),
+                         a.n_draft ? min(max(__ldcg(a.n_draft + b), 0), a.n_tok) : a.n_tok);
+    };
+    auto tiles = [&](int2 l) {              // its key tiles and row tiles
+        return l.y ? make_int2((l.x + l.y + TA_KEYS - 1) / TA_KEYS, (l.y * a.n_heads + NR - 1) / NR) : make_int2(0, 0);
     };
     int per = g.per;
     if (even) {
         int top = 1;
         for (int b = lane; b < a.batch; b += 32) {
             len[b] = length(b);
-            top = max(top, len[b].x);
+            top = max(top, tiles(len[b]).x);
         }
         top = __reduce_max_sync(0xffffffffu, top);
         // eight parts a step: its seven counts do not wait for one another
@@ -344,7 +345,7 @@ __device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int 
             const int step = (per - lo + 7) >> 3;
             unsigned blocks[7] = {};
             for (int b = lane; b < a.batch; b += 32) {
-                const int2 l = len[b];
+                const int2 l = tiles(len[b]);
 #pragma unroll
                 for (int i = 0; i < 7; i++) {
                     const int mid = lo + i * step;
@@ -362,7 +363,7 @@ __device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int 
     int seq = -1, tile = 0, tb = 0, nt = 0;
     for (int b0 = 0; b0 < a.batch && seq < 0; b0 += 32) {
         const int b = b0 + lane;
-        const int2 l = b >= a.batch ? make_int2(0, 0) : even ? len[b] : length(b);
+        const int2 at_b = b >= a.batch ? make_int2(0, 0) : even ? len[b] : length(b), l = tiles(at_b);
         const int ns = (l.x + per - 1) / per;
         const unsigned mine = l.y * ns;
         unsigned end = mine;
@@ -383,7 +384,7 @@ __device__ __forceinline__ void share(const Args &g, Shared &sh, int2 *len, int 
             nt = min(l.x - tb, even_per);
             if (at == 0 && g.nsplit > 1) g.part.seq[b] = make_int2((int)(end - mine), ns);
             sh.tile = tile, sh.tb = tb, sh.nt = nt;
-            sh.ctx = context(b), sh.nd = drafted(b);
+            sh.ctx = at_b.x, sh.nd = at_b.y;
         }
     }
     if (lane == 0) sh.seq = seq;
@@ -476,6 +477,12 @@ k_tree_attn(const __grid_constant__ Args g)
             pg1 = page_at(pos + 8);
         };
         next_rows();
+        // the first rows into L2 at once, a cache line a lane: fetching pair by
+        // pair would wait for DRAM each time
+        for (int o = 128 * q4; o < d + a.c.tail; o += 512) {
+            if (row0 != TA_NOROW) asm volatile("prefetch.global.L2 [%0];" ::"l"(at_row(row0) - 16 * q4 + o));
+            if (row1 != TA_NOROW) asm volatile("prefetch.global.L2 [%0];" ::"l"(at_row(row1) - 16 * q4 + o));
+        }
         int fp = 0, left = nt;                          // pair to fetch; tiles left
         auto fetch = [&](Unit &u) {
             if (left == 0) return;

@@ -30,10 +30,11 @@
 // The blocks' best (value, index) pairs meet in the first block's shared
 // memory, so the greedy token needs neither scratch nor a second launch.
 //
-// Measured at 129280 floats a row: 9.4 us for one row with 600 tokens of
-// history, 31 us for 64 rows with up to 8192 (16.5 us without history and
-// biases, where the traffic alone takes 10.5); the rest is the latency of the
-// five steps, which two blocks a multiprocessor overlap only in part.
+// Measured at 129280 floats a row: 8.8 us for one row with 600 tokens of
+// history (5.7 without), 31 us for 64 rows with up to 8192 (16.1 without
+// history and biases, where the traffic alone takes 10.5); the rest is the
+// latency of the five steps, which two blocks a multiprocessor overlap only in
+// part.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -51,6 +52,7 @@ constexpr int LG_T = 512;
 constexpr int LG_CHUNK = 64;            // tokens dealt to a block at a time
 constexpr int LG_RUN = 65536;           // tokens of a block at a time: 16 bits number them
 constexpr int LG_SLOTS = 2048;          // named tokens settled at once; a run with more is cut into parts this long
+constexpr int LG_AHEAD = 4;             // history entries a thread asks for before it knows their number
 constexpr int LG_LIST = 4096;           // history entries kept; a longer list is read again
 
 // A slot's count: the generated occurrences, and the top bit when the token
@@ -118,30 +120,42 @@ k_logits(LogitsCall c)
     auto token_of = [&](int r0, int k) { return r0 + ((k / LG_CHUNK) * LG_C + rank) * LG_CHUNK + k % LG_CHUNK; };
     // eight logits and their mask bits, asked for ahead of their use
     Raw8<DT> nx;
-    unsigned nm = 0xFFu;
+    unsigned nm = 0xFFFFFFFFu;              // the mask's whole word: shifting it here would wait for it
     auto ask = [&](int r0, int k, int end) {
         const int t0 = token_of(r0, k);
         if (k >= end || t0 >= c.vocab) return;
         if (t0 + 8 <= c.vocab) nx = ld_raw8<DT, VEC>(x, (size_t)t0);
-        if (mask) nm = __ldcg(mask + (t0 >> 5)) >> (t0 & 31);
+        if (mask) nm = __ldcg(mask + (t0 >> 5));
     };
     ask(0, tid * 8, c.run);
 
-    const int hl = hist ? min(__ldcg(a.hist_len + row), (int)min(a.hist_stride, 0x7fffffffL)) : 0;
-    const int np = hist && a.n_prompt ? __ldcg(a.n_prompt + row) : 0;
-    const int bl = bias ? min(__ldcg(a.bias_len + row), (int)min(a.bias_stride, 0x7fffffffL)) : 0;
+    // so is the start of the history, and its length: used only later on
+    int ahead[LG_AHEAD];
+#pragma unroll
+    for (int j = 0; j < LG_AHEAD; j++)
+        ahead[j] = hist && j * LG_T + tid < a.hist_stride ? __ldcg(hist + j * LG_T + tid) : -1;
+    const int hist_len = hist ? __ldcg(a.hist_len + row) : 0, np = hist && a.n_prompt ? __ldcg(a.n_prompt + row) : 0;
+    const int bias_len = bias ? __ldcg(a.bias_len + row) : 0;
+    const float rep = a.rep ? __ldcg(a.rep + row) : 1.0f, freq = a.freq ? __ldcg(a.freq + row) : 0.0f;
+    const float pres = a.pres ? __ldcg(a.pres + row) : 0.0f;
     float bv = -INFINITY;
     int bi = -1;
     // every block of the cluster has started before one writes to the first
-    if (c.token) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    // (relaxed: nothing is handed over, and a release would wait for the loads)
+    if (c.token) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     for (long at = 0; at < c.vocab; at += (long)LG_C * c.run) {
         const int r0 = (int)at, here = min(LG_C * c.run, c.vocab - r0);       // the cluster's tokens
         const int chunks = (here + LG_CHUNK - 1) / LG_CHUNK, m = (chunks - rank + LG_C - 1) / LG_C * LG_CHUNK;
-        // fn(i, k) for the first n entries i of a list of tokens, k the
-        // block's number of the token, ~0 for one that is not its own; whole
-        // warps, four loads in flight
-        auto each = [&](const int *ids, int n, auto fn) {
-            for (int i0 = tid & ~31; i0 < n; i0 += 4 * LG_T) {
+        const int hl = min(hist_len, (int)a.hist_stride), bl = min(bias_len, (int)a.bias_stride);
+        // the block's number of token r0 + u, ~0 for one that is not its own
+        auto number_of = [&](unsigned u) {
+            const unsigned q = u / LG_CHUNK;
+            return u < (unsigned)here && q % LG_C == (unsigned)rank ? q / LG_C * LG_CHUNK + u % LG_CHUNK : 0xFFFFFFFFu;
+        };
+        // fn(i, k) for entries from .. n of a list of tokens, k the block's
+        // number of entry i's token; whole warps, four loads in flight
+        auto each = [&](const int *ids, int from, int n, auto fn) {
+            for (int i0 = from + (tid & ~31); i0 < n; i0 += 4 * LG_T) {
                 unsigned u[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -149,11 +163,7 @@ k_logits(LogitsCall c)
                     u[j] = i < n ? (unsigned)__ldcg(ids + i) - (unsigned)r0 : 0xFFFFFFFFu;
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const unsigned q = u[j] / LG_CHUNK;
-                    const bool own = u[j] < (unsigned)here && q % LG_C == (unsigned)rank;
-                    fn(i0 + j * LG_T + lane, own ? q / LG_C * LG_CHUNK + u[j] % LG_CHUNK : 0xFFFFFFFFu);
-                }
+                for (int j = 0; j < 4; j++) fn(i0 + j * LG_T + lane, number_of(u[j]));
             }
         };
         auto place = [&](int w0, int w1) {      // slots of the marked tokens of bitmap words w0 .. w1
@@ -183,7 +193,9 @@ k_logits(LogitsCall c)
             for (int i = tid; i < (m + 31) >> 5; i += LG_T) bits[i] = 0;
             if (tid == 0) n_list = n_slots = 0;
             __syncthreads();
-            each(hist, hl, [&](int i, unsigned k) {
+            // (one entry for equal tokens of a warp, found by matching, takes
+            // longer than the repeated atomics: 32.3 us at 64 rows against 30.7)
+            auto mark = [&](int i, unsigned k) {
                 const bool own = k != 0xFFFFFFFFu;
                 const unsigned who = __ballot_sync(0xffffffffu, own);
                 if (!who) return;
@@ -194,8 +206,15 @@ k_logits(LogitsCall c)
                     atomicOr(bits + (k >> 5), 1u << (k & 31));
                     if (p < LG_LIST) list[p] = k | (i < np ? LG_SEEN : 0u);
                 }
-            });
-            each(bid, bl, [&](int, unsigned k) {
+            };
+            if (r0 == 0)
+#pragma unroll
+                for (int j = 0; j < LG_AHEAD; j++) {
+                    const int i = j * LG_T + tid;
+                    if (j * LG_T + (tid & ~31) < hl) mark(i, i < hl ? number_of((unsigned)ahead[j]) : 0xFFFFFFFFu);
+                }
+            each(hist, r0 == 0 ? LG_AHEAD * LG_T : 0, hl, mark);
+            each(bid, 0, bl, [&](int, unsigned k) {
                 if (k != 0xFFFFFFFFu) atomicOr(bits + (k >> 5), 1u << (k & 31));
             });
             __syncthreads();
@@ -225,8 +244,8 @@ k_logits(LogitsCall c)
                 if (nl <= LG_LIST)
                     for (int i = tid; i < nl; i += LG_T) count(list[i] & ~LG_SEEN, list[i] & LG_SEEN);
                 else                            // the list is cut short: the history again
-                    each(hist, hl, [&](int i, unsigned k) { count(k, i < np); });
-                each(bid, bl, [&](int i, unsigned k) {
+                    each(hist, 0, hl, [&](int i, unsigned k) { count(k, i < np); });
+                each(bid, 0, bl, [&](int i, unsigned k) {
                     if (k - s0 >= (unsigned)len) return;
                     const int s = slot_of(k);
                     tok[s] = (unsigned short)k;
@@ -242,11 +261,10 @@ k_logits(LogitsCall c)
                     float v = on ? ld_row1<DT>(x, (size_t)t) : 0.0f;
                     if (w) {
                         const unsigned n = w & ~LG_SEEN;
-                        const float rep = a.rep ? __ldcg(a.rep + row) : 1.0f;
                         v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
                         if (n) {
-                            v = __fsub_rn(v, __fmul_rn(a.freq ? __ldcg(a.freq + row) : 0.0f, (float)n));
-                            v = __fsub_rn(v, a.pres ? __ldcg(a.pres + row) : 0.0f);
+                            v = __fsub_rn(v, __fmul_rn(freq, (float)n));
+                            v = __fsub_rn(v, pres);
                         }
                     }
                     if (bias) {
@@ -288,7 +306,7 @@ k_logits(LogitsCall c)
 #pragma unroll
                     for (int j = 0; j < 8; j++) v[j] = j < left ? ld_row1<DT>(x, (size_t)t0 + j) : -INFINITY;
                 }
-                const unsigned on = nm;
+                const unsigned on = nm >> (t0 & 31);
                 ask(r0, k + LG_T * 8, end);
                 if (named) {
                     const unsigned its = bits[k >> 5] >> (k & 31) & 0xFFu;
@@ -333,8 +351,12 @@ k_logits(LogitsCall c)
         for (int w = 1; w < LG_T / 32; w++) better(bv, bi, sv[w], si[w]);
         *cl.map_shared_rank(&best_v[rank], 0) = bv;
         *cl.map_shared_rank(&best_i[rank], 0) = bi;
+        // the pair is handed over; a releasing barrier would wait for every
+        // thread's stores of logits
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
     }
-    cl.sync();
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (rank == 0 && tid == 0) {
         for (int w = 1; w < LG_C; w++) better(bv, bi, best_v[w], best_i[w]);
         c.token[row] = bi;

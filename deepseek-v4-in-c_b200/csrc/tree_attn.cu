@@ -47,7 +47,7 @@
 //
 // Measured (d 512, 64 heads, bf16): 16 tokens on 4 contexts of 32768 positions
 // 416 us, 660 TFLOP/s; 7 tokens on 8 contexts of up to 4100 39 us; one token on
-// 700 positions 13 us. With d 576, one token on 8 contexts of 32768 99 us. What
+// 700 positions 13 us. With d 576, one token on 8 contexts of 32768 98 us. What
 // bounds it is no unit but the hand-over between the roles: a tile of 64 rows
 // takes 6300 cycles, of which the MMAs need 2600, and leaving out all MMAs,
 // all exponentials or all loads shortens the call by 3, 0 and 5 %. Shared

@@ -266,6 +266,13 @@ def decode_bytes_per_token(d, pos):
     return total
 
 
+def ref_missing():
+    """Why the reference's CPU code cannot be run here, or None."""
+    import oracle as O
+    return None if os.path.exists(O.REF_SO) else \
+        "oracle/_ref/libdsv4ref.so is not built (it is compiled from the reference's sources, where they are)"
+
+
 def cpu_decode_sample(n_pos, warm=2, prompt_len=0):
     """The reference's dsv4_layer_forward on a 3-layer Flash-geometry model
     (compress ratios 0 / 4 / 128, all 256 experts, vocab 129280): without a
@@ -446,10 +453,12 @@ def run_decode(a):
     if rank == 0 and world == 1 and not a.no_cpu:
         # the reference decodes one sequence at a time: its tok/s is the
         # batch-1 rate whatever the batch
-        s_tok, _, desc, _ = cpu_decode_sample(8)
-        out["cpu_baseline"] = {"value": 1.0 / s_tok, "unit": "tok/s",
-                               "cores": int(os.environ.get("OMP_NUM_THREADS", os.cpu_count())),
-                               "kind": "reference", "sample": desc}
+        out["cpu_baseline"] = {"unavailable": ref_missing()}
+        if not ref_missing():
+            s_tok, _, desc, _ = cpu_decode_sample(8)
+            out["cpu_baseline"] = {"value": 1.0 / s_tok, "unit": "tok/s",
+                                   "cores": int(os.environ.get("OMP_NUM_THREADS", os.cpu_count())),
+                                   "kind": "reference", "sample": desc}
     if world > 1 and L.dsv4b_model_comm_status(model.h) != 0:
         out["comm_error"] = "a peer exchange timed out waiting for a rank: results invalid"
     if rank == 0:
@@ -567,10 +576,12 @@ def run_prefill(a):
                 "api": "dsv4b_model_prefill (host prompt -> host first token), wall clock"},
     }
     if not a.no_cpu:
-        s_tok, desc = cpu_prefill_sample(CH)
-        out["cpu_baseline"] = {"value": 1.0 / s_tok, "unit": "tok/s",
-                               "cores": int(os.environ.get("OMP_NUM_THREADS", os.cpu_count())),
-                               "kind": "reference", "sample": desc}
+        out["cpu_baseline"] = {"unavailable": ref_missing()}
+        if not ref_missing():
+            s_tok, desc = cpu_prefill_sample(CH)
+            out["cpu_baseline"] = {"value": 1.0 / s_tok, "unit": "tok/s",
+                                   "cores": int(os.environ.get("OMP_NUM_THREADS", os.cpu_count())),
+                                   "kind": "reference", "sample": desc}
     print(json.dumps(out))
     model.close()
     L.dsv4_cuda_shutdown()
@@ -1038,6 +1049,9 @@ def cpu_mla_sample(qi, keys, w, q, kv, sink, scale, k_small=256):
 def run_reference(a):
     rank = int(os.environ.get("RANK", "0"))
     if rank != 0:
+        return
+    if a.workload in ("prefill", "decode") and ref_missing():
+        print(json.dumps({"impl": "reference", "unavailable": ref_missing()}))
         return
     if a.workload == "prefill":
         s_tok, desc = cpu_prefill_sample(a.chunk)

@@ -31,7 +31,7 @@
 // memory, so the greedy token needs neither scratch nor a second launch.
 //
 // Measured at 129280 floats a row: 8.8 us for one row with 600 tokens of
-// history (5.7 without), 31 us for 64 rows with up to 8192 (16.1 without
+// history (5.7 without), 29 us for 64 rows with up to 8192 (16.1 without
 // history and biases, where the traffic alone takes 10.5); the rest is the
 // latency of the five steps, which two blocks a multiprocessor overlap only in
 // part.
@@ -52,7 +52,6 @@ constexpr int LG_T = 512;
 constexpr int LG_CHUNK = 64;            // tokens dealt to a block at a time
 constexpr int LG_RUN = 65536;           // tokens of a block at a time: 16 bits number them
 constexpr int LG_SLOTS = 2048;          // named tokens settled at once; a run with more is cut into parts this long
-constexpr int LG_AHEAD = 4;             // history entries a thread asks for before it knows their number
 constexpr int LG_LIST = 4096;           // history entries kept; a longer list is read again
 
 // A slot's count: the generated occurrences, and the top bit when the token
@@ -130,9 +129,9 @@ k_logits(LogitsCall c)
     ask(0, tid * 8, c.run);
 
     // so is the start of the history, and its length: used only later on
-    int ahead[LG_AHEAD];
+    int ahead[4];
 #pragma unroll
-    for (int j = 0; j < LG_AHEAD; j++)
+    for (int j = 0; j < 4; j++)
         ahead[j] = hist && j * LG_T + tid < a.hist_stride ? __ldcg(hist + j * LG_T + tid) : -1;
     const int hist_len = hist ? __ldcg(a.hist_len + row) : 0, np = hist && a.n_prompt ? __ldcg(a.n_prompt + row) : 0;
     const int bias_len = bias ? __ldcg(a.bias_len + row) : 0;
@@ -152,18 +151,17 @@ k_logits(LogitsCall c)
             const unsigned q = u / LG_CHUNK;
             return u < (unsigned)here && q % LG_C == (unsigned)rank ? q / LG_C * LG_CHUNK + u % LG_CHUNK : 0xFFFFFFFFu;
         };
-        // fn(i, k) for entries from .. n of a list of tokens, k the block's
-        // number of entry i's token; whole warps, four loads in flight
+        // fn(i, k) for entries from .. n of a list of tokens, four at a time: k
+        // the block's number of entry i's token, then of i + LG_T's, and so on;
+        // whole warps, the four loads in flight together
         auto each = [&](const int *ids, int from, int n, auto fn) {
-            for (int i0 = from + (tid & ~31); i0 < n; i0 += 4 * LG_T) {
-                unsigned u[4];
+            for (int i = from + tid; (i & ~31) < n; i += 4 * LG_T) {
+                unsigned k[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int i = i0 + j * LG_T + lane;
-                    u[j] = i < n ? (unsigned)__ldcg(ids + i) - (unsigned)r0 : 0xFFFFFFFFu;
-                }
+                for (int j = 0; j < 4; j++) k[j] = i + j * LG_T < n ? (unsigned)__ldcg(ids + i + j * LG_T) - (unsigned)r0 : 0xFFFFFFFFu;
 #pragma unroll
-                for (int j = 0; j < 4; j++) fn(i0 + j * LG_T + lane, number_of(u[j]));
+                for (int j = 0; j < 4; j++) k[j] = number_of(k[j]);
+                fn(i, k);
             }
         };
         auto place = [&](int w0, int w1) {      // slots of the marked tokens of bitmap words w0 .. w1
@@ -194,28 +192,41 @@ k_logits(LogitsCall c)
             if (tid == 0) n_list = n_slots = 0;
             __syncthreads();
             // (one entry for equal tokens of a warp, found by matching, takes
-            // longer than the repeated atomics: 32.3 us at 64 rows against 30.7)
-            auto mark = [&](int i, unsigned k) {
-                const bool own = k != 0xFFFFFFFFu;
-                const unsigned who = __ballot_sync(0xffffffffu, own);
-                if (!who) return;
-                unsigned p = 0;
-                if (lane == 0) p = atomicAdd(&n_list, (unsigned)__popc(who));
-                p = __shfl_sync(0xffffffffu, p, 0) + __popc(who & ((1u << lane) - 1u));
-                if (own) {
-                    atomicOr(bits + (k >> 5), 1u << (k & 31));
-                    if (p < LG_LIST) list[p] = k | (i < np ? LG_SEEN : 0u);
+            // longer than the repeated atomics: 1.5 us at 64 rows)
+            // (one entry for equal tokens of a warp, found by matching, takes
+            // longer than the repeated atomics: 1.5 us at 64 rows)
+            auto mark = [&](int i, const unsigned (&k)[4]) {
+                unsigned who[4];
+                int all = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    who[j] = __ballot_sync(0xffffffffu, k[j] != 0xFFFFFFFFu);
+                    all += __popc(who[j]);
+                }
+                if (!all) return;
+                int p = 0;
+                if (lane == 0) p = (int)atomicAdd(&n_list, (unsigned)all);
+                p = __shfl_sync(0xffffffffu, p, 0);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int at = p + __popc(who[j] & ((1u << lane) - 1u));
+                    p += __popc(who[j]);
+                    if (k[j] == 0xFFFFFFFFu) continue;
+                    atomicOr(bits + (k[j] >> 5), 1u << (k[j] & 31));
+                    if (at < LG_LIST) list[at] = k[j] | (i + j * LG_T < np ? LG_SEEN : 0u);
                 }
             };
-            if (r0 == 0)
+            if (r0 == 0 && (tid & ~31) < hl) {
+                unsigned k[4];
 #pragma unroll
-                for (int j = 0; j < LG_AHEAD; j++) {
-                    const int i = j * LG_T + tid;
-                    if (j * LG_T + (tid & ~31) < hl) mark(i, i < hl ? number_of((unsigned)ahead[j]) : 0xFFFFFFFFu);
-                }
-            each(hist, r0 == 0 ? LG_AHEAD * LG_T : 0, hl, mark);
-            each(bid, 0, bl, [&](int, unsigned k) {
-                if (k != 0xFFFFFFFFu) atomicOr(bits + (k >> 5), 1u << (k & 31));
+                for (int j = 0; j < 4; j++) k[j] = j * LG_T + tid < hl ? number_of((unsigned)ahead[j]) : 0xFFFFFFFFu;
+                mark(tid, k);
+            }
+            each(hist, r0 == 0 ? 4 * LG_T : 0, hl, mark);
+            each(bid, 0, bl, [&](int, const unsigned (&k)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (k[j] != 0xFFFFFFFFu) atomicOr(bits + (k[j] >> 5), 1u << (k[j] & 31));
             });
             __syncthreads();
             place(0, (m + 31) >> 5);
@@ -244,12 +255,19 @@ k_logits(LogitsCall c)
                 if (nl <= LG_LIST)
                     for (int i = tid; i < nl; i += LG_T) count(list[i] & ~LG_SEEN, list[i] & LG_SEEN);
                 else                            // the list is cut short: the history again
-                    each(hist, 0, hl, [&](int i, unsigned k) { count(k, i < np); });
-                each(bid, 0, bl, [&](int i, unsigned k) {
-                    if (k - s0 >= (unsigned)len) return;
-                    const int s = slot_of(k);
-                    tok[s] = (unsigned short)k;
-                    if (atomicMin(link + s, (unsigned)i) != LG_NONE) atomicOr(many + (s >> 5), 1u << (s & 31));
+                    each(hist, 0, hl, [&](int i, const unsigned (&k)[4]) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) count(k[j], i + j * LG_T < np);
+                    });
+                each(bid, 0, bl, [&](int i, const unsigned (&k)[4]) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (k[j] - s0 >= (unsigned)len) continue;
+                        const int s = slot_of(k[j]);
+                        tok[s] = (unsigned short)k[j];
+                        if (atomicMin(link + s, (unsigned)(i + j * LG_T)) != LG_NONE)
+                            atomicOr(many + (s >> 5), 1u << (s & 31));
+                    }
                 });
                 __syncthreads();
                 const int ns = (int)n_slots;

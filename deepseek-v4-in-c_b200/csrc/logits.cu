@@ -47,7 +47,7 @@ namespace cg = cooperative_groups;
 namespace dsv4b {
 
 // Threads of a block, two blocks a multiprocessor. At 64 rows 512 threads take
-// 31 us, 256 take 44 (fewer loads in flight) and 1024, one block, 40.
+// 29 us, 256 take 38 (fewer loads in flight) and 1024, one block, 40.
 constexpr int LG_T = 512;
 constexpr int LG_CHUNK = 64;            // tokens dealt to a block at a time
 constexpr int LG_RUN = 65536;           // tokens of a block at a time: 16 bits number them
@@ -61,8 +61,8 @@ constexpr unsigned LG_NONE = 0xFFFFFFFFu;       // a slot without a bias
 
 // Rows that get 8 blocks each; more get 4, which read the history half as
 // often. Measured at 129280 floats, 2000 tokens of history, 50 biases, a mask
-// (us by 8 / by 4 blocks a row): 1 row 10.6 / 13.5, 16 rows 14.1 / 14.0,
-// 32 rows 16.3 / 18.3, 48 rows 30.8 / 22.7, 64 rows 31.5 / 24.1: the step
+// (us by 8 / by 4 blocks a row): 1 row 9.5 / 12.1, 16 rows 13.0 / 12.9,
+// 32 rows 15.7 / 17.6, 48 rows 27.7 / 21.8, 64 rows 29.6 / 23.0: the step
 // comes where the blocks no longer all fit on the device at once.
 constexpr int LG_FEW = 36;
 

@@ -55,14 +55,20 @@
 // tiles a block costs 9 to 15 us: the first rows' way from DRAM, q, the first
 // references, the output.
 //
-// Numbers. With s_j = 2^e_j the row scale, score = S (scale 2^e_j) in float
-// and the weight that multiplies codes is p_j 2^(e_j - E) in f16 (rounding
-// 2^-11; an output of 16 bits rounds as much again). E and the row's
-// reference M are raised only when a score passes M by 2^8 or a scale passes
-// 2^(E + 7) -- both fit f16 -- so O^T is almost never rescaled, and no tile
-// needs the exact maximum: one comparison per score and one vote per tile. q
-// is widened or scaled per row by a power of two into f16 (exact unless an
-// element is below 2^-29 of its row's largest). Sums of p, S and O are float.
+// Numbers. Cache row j has the scale byte e_j; x_j is its score as a power of
+// two. Each of the tile's rows has two references of its own over the keys it
+// sees: M for x, and R for x + e, which is what a key gives to O. p_j =
+// 2^(x_j - M) and its sum are float. The weight that multiplies codes is
+// 2^(x_j + e_j - R + 7), rounded once to f16: half a step is 2^-11 of it, or
+// 2^-32 of the row's largest below f16's normal range. So a large cache row
+// that is hidden or weighs nothing takes no bits from small ones that weigh
+// much (with one reference of scales for all rows, 2^20 between them cost 8 %
+// of the output and 2^26 all of it). References are raised only when a score
+// passes M by 2^8 or a weight 2^15, which fits f16: O^T is almost never
+// rescaled, and no tile needs the exact maximum, only two comparisons per score
+// and one vote per tile. q is widened or scaled per row by a power of two into
+// f16 (exact unless an element is below 2^-29 of its row's largest). S and O
+// are float.
 #include "common.cuh"
 #include "internal.h"
 #include "rows.cuh"
@@ -93,8 +99,9 @@ constexpr int TA_SLOT = TA_KEYS * 128;              // bytes of one 64-element c
 constexpr int TA_PLACES = 7;                        // most chunk pairs in shared memory
 constexpr int TA_SMEM = 232448;                     // a block's limit
 constexpr int TA_SPLITS = 128;
-constexpr int TA_NONE = -1000;                      // scale reference before the first tile
-constexpr float TA_RAISE = 8.0f;                    // log2 of a weight that raises the reference
+constexpr float TA_RAISE = 8.0f;                    // log2 of p that raises the references
+constexpr float TA_LIFT = 7.0f, TA_FULL = 15.0f;    // log2 of the weight at R, and of one that raises them
+constexpr float TA_UNSEEN = -120.0f;                 // 7 - (R - M) of a row that has seen nothing: any number
 
 struct Parts {              // one entry per (block, row of its tile)
     float *o;               // [d] the block's own average
@@ -113,10 +120,11 @@ struct Shared {             // behind the operand tiles
     uint64_t v_full[TA_PLACES], v_empty[TA_PLACES], k_full[TA_RING], k_done[TA_RING];
     uint64_t q_full, key_full, s_full, s_free, p_full, pv_done;
     uint64_t rowmask[TA_ROWS], out_at[TA_ROWS];     // a row's tree mask, and its first output element
-    float cq[TA_ROWS], nm[TA_ROWS];     // score factor of a row, and its negated reference
-    float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], lsum[4][TA_ROWS];
-    int wk[TA_SOFT], kx[TA_KEYS];       // largest scale byte of a softmax warp; each key's, -1: not there
-    float scale[2];         // 2^E of each half of the rows
+    float cq[TA_ROWS], nm[TA_ROWS];     // score factor of a row, and its negated reference M
+    float rr[TA_ROWS], dr[TA_ROWS];     // R - M, and 7 - (R - M) as a whole number
+    float bs[TA_ROWS], dmax[2];         // 2^(dr + 127), and the largest dr of each half of the rows
+    float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], rmax[4][TA_ROWS], lsum[4][TA_ROWS];
+    int kx[TA_KEYS];        // each key's scale byte, -1: not there
     int seq, tile, tb, nt;  // the block's share: sequence (-1: none), row tile, first key tile, key tiles
     int ctx, nd;            // the sequence's context and drafted tokens
     uint32_t tmem;
@@ -706,6 +714,10 @@ k_tree_attn(const __grid_constant__ Args g)
         if (tid < NR) {
             const int r = tid, t = (r0 + r) / H;
             sh.nm[r] = INFINITY;
+            sh.rr[r] = -INFINITY;
+            sh.dr[r] = TA_UNSEEN;
+            sh.bs[r] = pow2i((int)TA_UNSEEN + 127);
+            if (r % NC == 0) sh.dmax[r / NC] = TA_UNSEEN;
             sh.out_at[r] = ((uint64_t)b * a.n_tok + t) * a.o_tok + (uint64_t)(r0 + r - t * H) * d;
             sh.rowmask[r] = r < nr ? __ldcg(a.mask + (size_t)b * a.n_tok + t) : 0ull;
         }
@@ -716,7 +728,6 @@ k_tree_attn(const __grid_constant__ Args g)
 #pragma unroll
         for (int i = 0; i < NC; i++) l[i] = 0.0f;
         const int old = ctx - tb * TA_KEYS;             // context positions from the first tile on
-        int E = TA_NONE;
         for (int j = 0; j < nt; j++) {
             warp_wait(&sh.key_full, j & 1, dead);
             const int kx = sh.kx[key];
@@ -724,10 +735,11 @@ k_tree_attn(const __grid_constant__ Args g)
             const int draft = j * TA_KEYS + key - old;
             const bool drafts = (j + 1) * TA_KEYS > old;          // the tile holds drafted rows
             const float ks = e8m0((uint8_t)kx);         // NaN for a NaN row: so are its scores and weights
+            const float kf = (float)kx;
+            float dmax = sh.dmax[wg];
             warp_wait(&sh.s_full, j & 1, dead);
             tc::fence_after();
             float x[NC];
-            float over;
             // scores times the row's factor and key's scale; hidden ones -inf
             auto scores = [&](bool lift) {
                 __syncwarp();
@@ -752,11 +764,11 @@ k_tree_attn(const __grid_constant__ Args g)
                     for (int i = 0; i < NC; i++) x[i] = -INFINITY;
                 }
             };
-            auto load = [&]() {     // exponents (log2) of the weights against the references
-                scores(true);
-                over = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < NC; i++) over = fmaxf(over, x[i]);
+            // exponents of the weights of x[i .. i + 3], from those of p
+            auto weights = [&](int i, float2 &u, float2 &v) {
+                const float4 dr = *reinterpret_cast<const float4 *>(&sh.dr[c0 + i]);
+                u = add2(make_float2(x[i], x[i + 1]), add2(make_float2(kf, kf), make_float2(dr.x, dr.y)));
+                v = add2(make_float2(x[i + 2], x[i + 3]), add2(make_float2(kf, kf), make_float2(dr.z, dr.w)));
             };
             // S is in registers: its columns are free. Before any wait for the
             // second product, which the MMA warp issues behind the next S.
@@ -765,37 +777,62 @@ k_tree_attn(const __grid_constant__ Args g)
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sh.s_free));
             };
-            load();
-            const bool raise = over > TA_RAISE || (valid && kx < 255 && kx - E > 7);
-            if (soft_any(raise, wg)) {
+            scores(true);
+            float over = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NC; i++) over = fmaxf(over, x[i]);
+            float full = over + (kf + dmax);            // no weight is above it
+            if (full > TA_FULL && over <= TA_RAISE) {
+                full = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NC; i += 4) {
+                    float2 u, v;
+                    weights(i, u, v);
+                    full = fmaxf(fmaxf(full, fmaxf(u.x, u.y)), fmaxf(v.x, v.y));
+                }
+            }
+            if (soft_any(over > TA_RAISE || full > TA_FULL, wg)) {
                 // raise the references: the rows' maxima over the tile (fmaxf
-                // takes no NaN)
+                // takes no NaN). R is kept relative to M: scores can be so
+                // large that a scale byte added to one is lost.
                 scores(false);
                 free_s();
-                float mine = -INFINITY;
+                float mine = -INFINITY, mine_r = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < NC; i++) {
-                    const float m = warp_top(x[i]);
-                    if (lane == i) mine = m;
+                    const float m = warp_top(x[i]), q = warp_top(m == -INFINITY ? m : (x[i] - m) + kf);
+                    if (lane == i) mine = m, mine_r = q;
                 }
-                if (lane < NC) sh.wmax[warp & 3][c0 + lane] = fmaxf(mine, -INFINITY);
-                const int kw = __reduce_max_sync(0xffffffffu, valid && kx < 255 ? kx : TA_NONE);
-                if (lane == 0) sh.wk[warp] = kw;
+                if (lane < NC) {
+                    sh.wmax[warp & 3][c0 + lane] = fmaxf(mine, -INFINITY);
+                    sh.rmax[warp & 3][c0 + lane] = fmaxf(mine_r, -INFINITY);
+                }
                 soft_sync(wg);
-                int En = E;
-#pragma unroll
-                for (int w = 0; w < 4; w++) En = max(En, sh.wk[4 * wg + w]);
-                if (key < NC) {
-                    const int r = c0 + key;
-                    const float mo = -sh.nm[r];
+                if ((warp & 3) == 0) {
+                    const int r = c0 + min(lane, NC - 1);
+                    const float mo = -sh.nm[r], d0 = sh.dr[r];
                     const float mn = fmaxf(fmaxf(mo, fmaxf(sh.wmax[0][r], sh.wmax[1][r])), fmaxf(sh.wmax[2][r], sh.wmax[3][r]));
-                    const float f = mo == -INFINITY ? 0.0f : ex2(mo - mn);
-                    sh.fl[r] = f;
-                    sh.fo[r] = f * pow2i(E - En);
-                    sh.nm[r] = -mn;
+                    float rn = -INFINITY;
+                    if (mn != -INFINITY) {
+                        rn = (mo - mn) + sh.rr[r];
+#pragma unroll
+                        for (int w = 0; w < 4; w++) rn = fmaxf(rn, (sh.wmax[w][r] - mn) + sh.rmax[w][r]);
+                    }
+                    const float dn = mn == -INFINITY ? TA_UNSEEN : TA_LIFT - rintf(rn);
+                    const float top = warp_top(dn);
+                    __syncwarp();
+                    if (lane < NC) {
+                        sh.fl[r] = mo == -INFINITY ? 0.0f : ex2(mo - mn);
+                        sh.fo[r] = mo == -INFINITY ? 0.0f : ex2((mo - mn) + (dn - d0));
+                        sh.nm[r] = -mn;
+                        sh.rr[r] = rn;
+                        sh.dr[r] = dn;
+                        sh.bs[r] = pow2i(min((int)dn, 0) + 127);    // finite: a warp without keys multiplies 0 by it
+                        if (lane == 0) sh.dmax[wg] = top;
+                    }
                 }
                 soft_sync(wg);
-                E = En;
+                dmax = sh.dmax[wg];
 #pragma unroll
                 for (int i = 0; i < NC; i++) l[i] *= sh.fl[c0 + i];
                 if (j > 0) {
@@ -818,16 +855,36 @@ k_tree_attn(const __grid_constant__ Args g)
             } else {
                 free_s();
             }
-            // weights: sums in float, the f16 operand of the second product
-            const __half2 w = __float2half2_rn(valid && kx < 255 ? pow2i(kx - E) : 1.0f);
+            // weights: sums of p in float, the f16 operand of the second product.
+            // p 2^(e + dr) as p (2^(e - 127) 2^(dr + 127)) while no factor leaves
+            // float's range for any row, which takes scales 2^93 apart; else by
+            // an exponential of its own (for every weight, that takes 7 % longer:
+            // 449 us against 419 at 4 x 16 tokens on 32768).
             uint32_t pw[NC / 2];
+            if (!__any_sync(0xffffffffu, valid && !(dmax <= 0.0f && kf + dmax <= 100.0f))) {
+                const float as = valid ? ks : 0.0f;
 #pragma unroll
-            for (int i = 0; i < NC; i += 2) {
-                const float2 e = make_float2(ex2(x[i]), ex2(x[i + 1]));
-                const float2 s = add2(make_float2(l[i], l[i + 1]), e);
-                l[i] = s.x, l[i + 1] = s.y;
-                const __half2 h = __hmul2(__floats2half2_rn(e.x, e.y), w);
-                pw[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                for (int i = 0; i < NC; i += 4) {
+                    const float4 bs = *reinterpret_cast<const float4 *>(&sh.bs[c0 + i]);
+                    const float2 p = make_float2(ex2(x[i]), ex2(x[i + 1])), q = make_float2(ex2(x[i + 2]), ex2(x[i + 3]));
+                    const float2 u = mul2(p, mul2(make_float2(as, as), make_float2(bs.x, bs.y)));
+                    const float2 v = mul2(q, mul2(make_float2(as, as), make_float2(bs.z, bs.w)));
+                    pw[i / 2] = pack2<DSV4B_F16>(u.x, u.y);
+                    pw[i / 2 + 1] = pack2<DSV4B_F16>(v.x, v.y);
+                    const float2 s = add2(make_float2(l[i], l[i + 1]), p), t = add2(make_float2(l[i + 2], l[i + 3]), q);
+                    l[i] = s.x, l[i + 1] = s.y, l[i + 2] = t.x, l[i + 3] = t.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NC; i += 4) {
+                    float2 u, v;
+                    weights(i, u, v);
+                    pw[i / 2] = pack2<DSV4B_F16>(ex2(u.x), ex2(u.y));
+                    pw[i / 2 + 1] = pack2<DSV4B_F16>(ex2(v.x), ex2(v.y));
+                    const float2 s = add2(make_float2(l[i], l[i + 1]), make_float2(ex2(x[i]), ex2(x[i + 1])));
+                    const float2 t = add2(make_float2(l[i + 2], l[i + 3]), make_float2(ex2(x[i + 2]), ex2(x[i + 3])));
+                    l[i] = s.x, l[i + 1] = s.y, l[i + 2] = t.x, l[i + 3] = t.y;
+                }
             }
             if (j > 0) warp_wait(&sh.pv_done, (j - 1) & 1, dead);
             const uint32_t dst = p_s + key * 128;
@@ -854,10 +911,12 @@ k_tree_attn(const __grid_constant__ Args g)
             } else if (a.sink && m != -INFINITY) {
                 den += ex2(__ldcg(a.sink + (r0 + r) % H) * 1.4426950408889634f - m);
             }
-            // the row scales' reference goes with it; 0 where nothing was seen
-            sh.fo[r] = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / den;
+            // O = 2^dr sum p 2^e code; 0 where nothing was seen. -dr - 127 is
+            // above -2^7 - 16 and, as p passes M by 2^8 at most, below 2^7
+            const int t = -(int)sh.dr[r] - 127, h = max(t, -126);
+            sh.fo[r] = m == -INFINITY && sum == 0.0f ? 0.0f : pow2i(t - h) / den;
+            sh.fl[r] = pow2i(h);
         }
-        if (key == 0) sh.scale[wg] = E == TA_NONE ? 0.0f : e8m0((uint8_t)E);
         tc::fence_before();
     }
     __syncthreads();
@@ -880,9 +939,8 @@ k_tree_attn(const __grid_constant__ Args g)
             tc::tmem_ld8(tmem + lanes + o_col + p * NR + c0 + 8, x + 8);
             tc::tmem_wait_ld(x);
             if (e >= d) continue;
-            const float s0 = sh.scale[c0 >= NC], s1 = sh.scale[c0 + 8 >= NC];
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = x[i] * sh.fo[c0 + i] * (i < 8 ? s0 : s1);
+            for (int i = 0; i < 16; i++) x[i] = x[i] * sh.fo[c0 + i] * sh.fl[c0 + i];
             if (g.nsplit > 1) {
                 float *o = g.part.o + (prow + c0) * d + e;
 #pragma unroll

@@ -1,0 +1,126 @@
+"""The tree-verification operators on the B200 where a call is allowed but
+unusual: cache rows of very different magnitude, layouts, streams, scratch of
+another size, errors of earlier calls. Against the same 64-bit definitions and
+roundings as test_tree_gpu.py.
+"""
+import pytest
+
+import dsv4_b200 as B
+import test_tree_gpu as T
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+DT, close, gen, normal = T.DT, T.close, T.gen, T.normal
+
+
+@pytest.fixture(scope="module", autouse=True)
+def dev():
+    return B.init()
+
+
+# ---------------------------------------------- rows of different magnitude
+
+def slots_of(k, b, n):
+    page = k["c"].codes.shape[1]
+    j = torch.arange(n, device="cuda")
+    return k["pages"][b].long()[j // page] * page + j % page
+
+
+def weighted(k):
+    """o and its tolerance in double, where every error counts with the weight
+    of its key, so that rows without weight lend no slack:
+
+    * a score is a float sum whose partial sums are off by at most 2^-22 of the
+      key's sum of magnitudes, d / 16 + 4 of them (f16 products are exact; q is
+      held in f16 to 2^-38 of its largest element at least);
+    * exponents are below 2^9 and rounded in float (2^-16), ex2 adds 2^-22: a
+      weight and the sum of weights each move by less than 2^-15;
+    * a weight is rounded to f16: 2^-11 of it, or half the smallest step, 2^-25,
+      where the row's largest is held at 2^7 / sqrt(2) or more: 2^-31.5 of the
+      largest p times scale, for each code;
+    * the output is rounded once, past the type's largest value to infinity."""
+    q, c = k["q"], k["c"]
+    b, t, h, d = q.shape
+    want = torch.full(q.shape, 11.0, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(want)
+    rel, tiny = T.unit(q.dtype)
+    for i in range(b):
+        n, m = int(k["ctx"][i]), int(k["nd"][i])
+        slot = slots_of(k, i, n + m)
+        v = T.decode(c, slot)
+        s = T.two(c.scales.view(-1)[slot].long() - 127)
+        for a in range(m):
+            bits = int(k["mask"][i, a])
+            see = torch.ones(n + m, dtype=torch.bool, device="cuda")
+            for z in range(m):
+                see[n + z] = bool((bits >> z) & 1)
+            w, sc = v[see], s[see]
+            x = q[i, a].double()
+            z = x @ w.T * k["scale"]
+            top = z.amax(-1, keepdim=True)
+            p = (z - top).exp()
+            den = p.sum(-1, keepdim=True) + (k["sink"].double()[:, None] - top).exp()
+            want[i, a] = p @ w / den
+            delta = abs(k["scale"]) * ((d / 16 + 4) * 2.0 ** -22 * (x.abs() @ w.abs().T)
+                                       + 2.0 ** -38 * x.abs().amax(-1, keepdim=True) * w.abs().sum(-1))
+            pd = torch.where(p > 0, p * delta, 0.0)
+            size = p @ w.abs() / den
+            low = 2.0 ** -31.5 * (p * sc).amax(-1, keepdim=True) * (w.abs() / sc[:, None]).sum(0) / den
+            tol[i, a] = ((pd @ w.abs()) / den + size * (2.0 ** -11 + 2.0 ** -15 + pd.sum(-1, keepdim=True) / den) + low
+                         + rel * 1.001 * want[i, a].abs() + tiny)
+    f = torch.finfo(q.dtype)
+    return torch.where(want.abs() >= f.max * (1 + f.eps / 4), want * float("inf"), want), tol
+
+
+@pytest.mark.parametrize("g", [0, 4, 8, 14, 18, 22, 26, 40, 100])
+@pytest.mark.parametrize("where", ["opposite", "hidden", "both"])
+@pytest.mark.parametrize("b,t,h,ctx,dtype", [(1, 3, 64, 700, "bf16"), (2, 2, 4, 1500, "f16"), (150, 2, 8, 300, "bf16")])
+def test_small_rows_beside_large_ones(g, where, b, t, h, ctx, dtype):
+    """Rows 2^g larger than the rest that weigh nothing (opposite to q) or are
+    hidden from every token but their own: the small rows carry the output."""
+    d = 512
+    k = T.tree_case(60 + g, b, t, h, d, 64, 64, ctx, DT[dtype])
+    u = normal(gen(61), d).sign()
+    k["q"] = (normal(gen(62), b, t, h, d) + u).to(DT[dtype])
+    rows = normal(gen(63), k["c"].scales.numel(), d)
+    for i in range(b):
+        at = slots_of(k, i, ctx + t)
+        if where != "hidden":
+            rows[at[[3, ctx // 2, ctx - 1]]] = -u * 2.0 ** g
+        if where != "opposite":
+            rows[at[ctx + t - 1]] = u * 2.0 ** g             # the last token's own row
+    k["mask"] &= ~(1 << (t - 1))
+    if where == "hidden" and g < 30:
+        k["mask"][0, t - 1] |= 1 << (t - 1)                  # one token sees it: that row alone carries its output
+    B.kv_write_dev(k["c"], rows, torch.arange(rows.shape[0], device="cuda"))
+    want, tol = weighted(k)
+    close(T.run_tree(k), want, tol)
+
+
+def test_rows_of_every_magnitude():
+    """Scales over 200 powers of two in one context, each scale's rows among
+    the heaviest for some head; zero rows between them."""
+    d, n = 256, 900
+    k = T.tree_case(70, 2, 2, 16, d, 64, 64, n, torch.bfloat16)
+    g = gen(71)
+    rows = normal(g, k["c"].scales.numel(), d) * torch.exp2(torch.randint(-100, 4, (k["c"].scales.numel(), 1), generator=g,
+                                                                         device="cuda").float())
+    rows[::5] = 0.0
+    B.kv_write_dev(k["c"], rows, torch.arange(rows.shape[0], device="cuda"))
+    want, tol = weighted(k)
+    close(T.run_tree(k), want, tol)
+
+
+@pytest.mark.parametrize("f", [2.0 ** -120, 2.0 ** -126])
+def test_rows_at_the_ends_of_the_scales(f):
+    """Rows whose scale byte is 0 or near it, float's subnormal numbers among
+    them; zero rows between them."""
+    k = T.tree_case(80, 2, 3, 16, 128, 64, 64, 700, torch.bfloat16)
+    rows = normal(gen(81), k["c"].scales.numel(), 128)
+    rows[::9] = 0.0
+    rows[1::9] *= 2.0 ** -6
+    B.kv_write_dev(k["c"], rows * f, torch.arange(rows.shape[0], device="cuda"))
+    k["scale"] = min(128 ** -0.5 / f, 2.0 ** 100)
+    want, tol = weighted(k)
+    close(T.run_tree(k), want, tol)

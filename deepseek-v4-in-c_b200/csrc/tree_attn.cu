@@ -750,8 +750,10 @@ k_tree_attn(const __grid_constant__ Args g)
                 for (int i = 0; i < NC; i += 4) {
                     const float4 cq = *reinterpret_cast<const float4 *>(&sh.cq[c0 + i]);
                     const float4 nm = lift ? *reinterpret_cast<const float4 *>(&sh.nm[c0 + i]) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    const float2 u = fma2(mul2(make_float2(x[i], x[i + 1]), make_float2(ks, ks)), make_float2(cq.x, cq.y), make_float2(nm.x, nm.y));
-                    const float2 v = fma2(mul2(make_float2(x[i + 2], x[i + 3]), make_float2(ks, ks)), make_float2(cq.z, cq.w), make_float2(nm.z, nm.w));
+                    // factors first: a large row's scale times S alone can pass
+                    // float's range where the score does not
+                    const float2 u = fma2(make_float2(x[i], x[i + 1]), mul2(make_float2(ks, ks), make_float2(cq.x, cq.y)), make_float2(nm.x, nm.y));
+                    const float2 v = fma2(make_float2(x[i + 2], x[i + 3]), mul2(make_float2(ks, ks), make_float2(cq.z, cq.w)), make_float2(nm.z, nm.w));
                     x[i] = u.x, x[i + 1] = u.y, x[i + 2] = v.x, x[i + 3] = v.y;
                 }
                 if (drafts && draft >= 0) {

@@ -112,10 +112,10 @@ def test_rows_of_every_magnitude():
     close(T.run_tree(k), want, tol)
 
 
-@pytest.mark.parametrize("f", [2.0 ** -120, 2.0 ** -126])
+@pytest.mark.parametrize("f", [2.0 ** -120, 2.0 ** -126, 2.0 ** 110])
 def test_rows_at_the_ends_of_the_scales(f):
-    """Rows whose scale byte is 0 or near it, float's subnormal numbers among
-    them; zero rows between them."""
+    """Rows whose scale byte is 0 or near it (float's subnormal numbers among
+    them), and rows near float's largest; zero rows between them."""
     k = T.tree_case(80, 2, 3, 16, 128, 64, 64, 700, torch.bfloat16)
     rows = normal(gen(81), k["c"].scales.numel(), 128)
     rows[::9] = 0.0

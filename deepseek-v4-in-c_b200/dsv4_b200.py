@@ -529,7 +529,7 @@ def tree_mask(parents):
 
 
 def tree_attn_scratch(n_heads, d, n_tok, batch, max_ctx):
-    """Bytes of scratch a tree_attn_dev call of these sizes needs."""
+    """Bytes of scratch a tree_attn_dev call of these sizes, or smaller ones, needs."""
     n = lib().dsv4b_tree_attn_scratch(int(n_heads), int(d), int(n_tok), int(batch), int(max_ctx))
     if n == 0:
         raise ValueError("sizes that dsv4b_tree_attn does not take")

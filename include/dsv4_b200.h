@@ -438,7 +438,9 @@ int dsv4b_kv_read(const dsv4b_kvq *c, void *out, int dt, long row_stride, const 
  * see: by 2^-11 of itself, or 2^-32 of that largest if more.
  * ctx[b] is at most max_ctx, which sizes the launch; n_tok <= DSV4B_TREE_MAX.
  * `scratch` holds dsv4b_tree_attn_scratch() bytes, 16-byte aligned, for the
- * duration of the call: calls that may overlap need their own. */
+ * duration of the call: calls that may overlap need their own. The size grows
+ * with every argument, up to 220 MB, so scratch for the largest call serves the
+ * smaller ones. */
 #define DSV4B_TREE_MAX 64
 size_t dsv4b_tree_attn_scratch(int n_heads, int d, int n_tok, int batch, int max_ctx);
 int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long q_tok, const dsv4b_kvq *c,

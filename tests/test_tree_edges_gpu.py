@@ -124,3 +124,17 @@ def test_rows_at_the_ends_of_the_scales(f):
     k["scale"] = min(128 ** -0.5 / f, 2.0 ** 100)
     want, tol = weighted(k)
     close(T.run_tree(k), want, tol)
+
+
+# ------------------------------------------------------------------- scratch
+
+def test_one_scratch_for_smaller_calls():
+    """Scratch of the largest call, its bytes NaN, serves smaller batches, trees
+    and contexts, which are cut otherwise."""
+    h, d = 64, 128
+    room = torch.empty(B.tree_attn_scratch(h, d, 16, 40, 6000), dtype=torch.uint8, device="cuda")
+    for b, t, ctx in ((40, 16, 900), (16, 16, 2000), (3, 2, 6000), (1, 1, 6000), (40, 1, 300), (1, 16, 0)):
+        k = T.tree_case(90 + b, b, t, h, d, 64, 64, ctx, torch.bfloat16, ragged=b > 1)
+        room.fill_(255)
+        want, tol = T.plain_tree(k)
+        close(T.run_tree(k, scratch=room), want, tol)

@@ -1138,6 +1138,8 @@ int tree_attn(const TreeAttn &a, void *scratch, cudaStream_t st)
 int tree_attn_status()
 {
     int v = 0;
+    // the copy alone would wait for no stream that was made non-blocking
+    if (cudaDeviceSynchronize() != cudaSuccess) return -1;
     return cudaMemcpyFromSymbol(&v, g_gave_up, sizeof v) == cudaSuccess ? (v ? 1 : 0) : -1;
 }
 

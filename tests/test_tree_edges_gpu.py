@@ -138,3 +138,22 @@ def test_one_scratch_for_smaller_calls():
         room.fill_(255)
         want, tol = T.plain_tree(k)
         close(T.run_tree(k, scratch=room), want, tol)
+
+
+# -------------------------------------------------------------------- status
+
+def test_status_waits_for_every_stream():
+    """A call that is still queued on a side stream has ended before its status
+    is given."""
+    k = T.tree_case(95, 1, 1, 8, 128, 64, 64, 300, torch.bfloat16)
+    ref = T.run_tree(k)
+    out = torch.full_like(ref, 11.0)
+    room = torch.empty(B.tree_attn_scratch(8, 128, 1, 1, 300), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)                     # about 50 ms
+        T.run_tree(k, out=out, scratch=room)
+    assert B.lib().dsv4b_tree_attn_status() == 0
+    assert side.query()
+    assert torch.equal(out, ref)

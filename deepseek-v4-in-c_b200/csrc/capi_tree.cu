@@ -159,6 +159,12 @@ extern "C" int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long 
 
 extern "C" int dsv4b_tree_attn_status(void) { return tree_attn_status(); }
 
+extern "C" int dsv4b_tree_attn_selftest(int limit_us, void *stream)
+{
+    if (limit_us < 1 || limit_us > 1000000) return -1;
+    return tree_attn_selftest(limit_us, stream_of(stream));
+}
+
 extern "C" int dsv4b_logits(void *out, const void *x, int dt, long out_stride, long x_stride, int *token,
                             const dsv4b_logit_adjust *adj, int rows, int vocab, void *stream)
 {

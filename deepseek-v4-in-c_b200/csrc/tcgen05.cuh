@@ -51,13 +51,13 @@ __device__ __forceinline__ uint64_t now_ns()
 }
 
 // A whole warp waits for the phase of `parity` to complete. A wait of more
-// than two seconds sets *dead, and once that is set every wait returns: the
+// than limit_ns sets *dead, and once that is set every wait returns: the
 // block runs to its end with results that are not valid. The votes keep the
 // control flow uniform, so that loop counters, barrier addresses and operand
 // descriptors around a wait can live in uniform registers: without them an
 // MMA's issue took 80 cycles instead of 27. (The clock is read once in 256
 // tries: a wait's instructions take issue slots from the warps that work.)
-__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatile int *dead)
+__device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatile int *dead, uint64_t limit_ns = 2000000000ull)
 {
     if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return;
     uint64_t t0 = 0;
@@ -68,7 +68,7 @@ __device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatil
         if (__any_sync(0xffffffffu, *dead)) return;
         const uint64_t t = now_ns();
         if (t0 == 0) t0 = t;
-        if (t - t0 > 2000000000ull) *dead = 1;
+        if (t - t0 > limit_ns) *dead = 1;
     }
 }
 

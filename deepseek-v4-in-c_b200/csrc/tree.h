@@ -56,6 +56,7 @@ size_t tree_attn_bytes(int n_heads, int d, int n_tok, int batch, int max_ctx);
 int tree_attn(const TreeAttn &a, void *scratch, cudaStream_t st);
 
 int tree_attn_status();
+int tree_attn_selftest(int limit_us, cudaStream_t st);
 
 int logits(void *out, const void *x, int dt, long out_stride, long x_stride, int *token,
            const dsv4b_logit_adjust &a, int rows, int vocab, cudaStream_t st);

@@ -1027,6 +1027,22 @@ k_tree_join(const __grid_constant__ Args g)
     }
 }
 
+// A wait that nothing ends: it runs out, as a call's would, and is reported.
+__global__ void __launch_bounds__(32) k_tree_wait_test(uint64_t limit_ns)
+{
+    __shared__ uint64_t bar;
+    __shared__ int dead;
+    if (threadIdx.x == 0) {
+        tc::mbar_init(tc::smem_u32(&bar), 1);
+        tc::mbar_init_fence();
+        dead = 0;
+    }
+    __syncwarp();
+    tc::warp_wait(tc::smem_u32(&bar), 0, &dead, limit_ns);
+    __syncwarp();
+    if (threadIdx.x == 0 && *(volatile int *)&dead) g_gave_up = 1;
+}
+
 // How a call is cut: rows of a tile, splits of the context, key tiles of a
 // split; blocks in all (where contexts are split, whole waves of 148: shorter
 // contexts leave some to the others).
@@ -1140,7 +1156,15 @@ int tree_attn_status()
     int v = 0;
     // the copy alone would wait for no stream that was made non-blocking
     if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-    return cudaMemcpyFromSymbol(&v, g_gave_up, sizeof v) == cudaSuccess ? (v ? 1 : 0) : -1;
+    if (cudaMemcpyFromSymbol(&v, g_gave_up, sizeof v) != cudaSuccess) return -1;
+    if (v == 0) return 0;
+    v = 0;
+    return cudaMemcpyToSymbol(g_gave_up, &v, sizeof v) == cudaSuccess ? 1 : -1;
+}
+
+int tree_attn_selftest(int limit_us, cudaStream_t st)
+{
+    return launch(k_tree_wait_test, dim3(1), dim3(32), 0, st, (uint64_t)limit_us * 1000) == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace dsv4b

@@ -106,6 +106,7 @@ def _declare(L):
         "dsv4b_tree_attn_scratch": ([i, i, i, i, i], sz),
         "dsv4b_tree_attn": ([vp, vp, i, C.c_long, C.c_long, vp, vp, i, vp, vp, vp, vp, i, i, i, i, f, vp, sz, vp], i),
         "dsv4b_tree_attn_status": ([], i),
+        "dsv4b_tree_attn_selftest": ([i, vp], i),
         "dsv4b_logits": ([vp, vp, i, C.c_long, C.c_long, vp, vp, i, i, vp], i),
         "dsv4_cuda_model_create": ([vp, vp, vp, vp, i], vp),
         "dsv4_cuda_model_begin": ([vp, vp, i], i),
@@ -566,6 +567,18 @@ def tree_attn_dev(o, q, cache, pages, ctx, n_draft, mask, sink, max_ctx, scale, 
              _want(mask, "mask", dev, _t.int64, (b, t)),
              None if sink is None else _want(sink, "sink", dev, _t.float32, (h,)), h, t, b, int(max_ctx),
              float(scale), scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream(dev, stream))
+
+
+def tree_attn_status(device=None):
+    """Waits for the device (the current one for None); True when every
+    tree_attn_dev there since the last status has run to its end. False: one of
+    them gave up a wait inside the kernel, and its output is not valid."""
+    _torch()
+    with _t.cuda.device(device):
+        rc = lib().dsv4b_tree_attn_status()
+    if rc < 0:
+        raise RuntimeError("dsv4b_tree_attn_status failed (rc=%d)" % rc)
+    return rc == 0
 
 
 class LogitAdjust:

@@ -448,11 +448,16 @@ int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long q_tok, cons
                     const unsigned long long *mask, const float *sink, int n_heads, int n_tok, int batch,
                     int max_ctx, float scale, void *scratch, size_t scratch_bytes, void *stream);
 
-/* 0 while every dsv4b_tree_attn on the current device has run to its end; 1
- * once one of its blocks gave up a wait inside the kernel (each is bounded by
- * two seconds; its outputs are then not valid); -1 without a device. Waits for
- * the device. */
+/* 0 when every dsv4b_tree_attn on the current device since the last status
+ * has run to its end; 1 when a block of one gave up a wait inside the kernel (each
+ * is bounded by two seconds; that call's outputs are not valid), which this
+ * call forgets; -1 without a device, or while a stream is being captured.
+ * Waits for the device. */
 int dsv4b_tree_attn_status(void);
+
+/* Such a wait, which nothing ends, in a kernel of its own: it runs out after
+ * limit_us (1 .. 1000000) microseconds, and the next status is 1. */
+int dsv4b_tree_attn_selftest(int limit_us, void *stream);
 
 /* What to do to the logits of each row; a NULL array is off. hist
  * [rows][hist_stride] holds the row's hist_len tokens, the first n_prompt of

@@ -35,3 +35,11 @@ def test_a_smaller_call_takes_the_largest_call_s_scratch():
                         max_pages=513, ctx=P, n_draft=None, mask=P, sink=None, n_heads=64, n_tok=tok, batch=batch,
                         max_ctx=32768, scale=0.1, scratch=P, bytes=room, stream=None)
             assert T.call("dsv4b_tree_attn", args) == -2, (batch, tok)
+
+
+def test_selftest_refusals():
+    T.no_device()
+    f = B.lib().dsv4b_tree_attn_selftest
+    assert f(1000, None) == -2
+    for bad in (0, -1, 1000001):
+        assert f(bad, None) == -1

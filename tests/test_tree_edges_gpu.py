@@ -157,3 +157,17 @@ def test_status_waits_for_every_stream():
     assert B.lib().dsv4b_tree_attn_status() == 0
     assert side.query()
     assert torch.equal(out, ref)
+
+
+def test_status_reports_a_wait_once():
+    """A wait that ran out is in the next status, and not in the one after."""
+    assert B.tree_attn_status()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert B.lib().dsv4b_tree_attn_selftest(1000, side.cuda_stream) == 0
+    assert not B.tree_attn_status()
+    assert B.tree_attn_status() and B.lib().dsv4b_tree_attn_status() == 0
+    k = T.tree_case(96, 1, 1, 8, 128, 64, 64, 300, torch.bfloat16)
+    want, tol = T.plain_tree(k)
+    close(T.run_tree(k), want, tol)
+    assert B.tree_attn_status(torch.cuda.current_device())

@@ -89,8 +89,11 @@ extern "C" int dsv4b_rope(void *out, int out_dt, long out_tok, long out_head, co
     if (n_tok == 0 || n_heads == 0) return 0;
     const int os = row_dt_size(out_dt), xs = row_dt_size(x_dt);
     if (!out || !x || !pos || !aligned(out, os) || !aligned(x, xs) || !aligned(pos, 4)) return -1;
-    // heads of a token and tokens do not overlap
-    if (x_head < 0 || x_tok < 0 || out_head < width || out_tok < (long)(n_heads - 1) * out_head + width) return -1;
+    if (x_head < 0 || x_tok < 0) return -1;
+    // no two heads of out overlap: a token's heads lie together, or a head's tokens
+    if (!(out_head >= width && out_tok >= (long)(n_heads - 1) * out_head + width) &&
+        !(out_tok >= width && out_head >= (long)(n_tok - 1) * out_tok + width))
+        return -1;
     const bool inplace = out == x && out_dt == x_dt && out_tok == x_tok && out_head == x_head;
     if (!inplace && Span(out, os, n_tok, out_tok, n_heads, out_head, width)
                         .meets(Span(x, xs, n_tok, x_tok, n_heads, x_head, width)))

@@ -440,8 +440,9 @@ def rope_cfg(rd, base, layout=ROPE_INTERLEAVED, factor=1.0, orig=0, beta_fast=32
 
 def rope_dev(out, x, pos, cfg, first, inverse=False, stream=None):
     """out = x [tokens, heads, width] with elements first .. first + cfg.rd of
-    every head rotated to pos [tokens] (int32); inverse rotates back. Any
-    strides with unit-stride heads; out may be x."""
+    every head rotated to pos [tokens] (int32); inverse rotates back. Unit-stride
+    heads, else any strides of x, and of out those in which no two heads
+    interleave (a transposed [heads, tokens, width] too); out may be x."""
     i32 = _torch().int32
     dev = x.get_device()
     xs, os_, shape = x.stride(), out.stride(), x.shape

@@ -385,7 +385,8 @@ int dsv4b_rope_init(dsv4b_rope_cfg *r, int rd, int layout, double base, double f
 /* out[t][h][0..width) = x[t][h][0..width) with elements first .. first + rd of
  * every head rotated to position pos[t] (inverse != 0: rotated back, which is
  * also the gradient). Strides in elements from token to token and head to
- * head; out is x with the same type and strides (in place: only the rotated
+ * head, either of which may be the longer (in out, the heads of a token lie
+ * between two tokens or the tokens of a head between two heads); out is x with the same type and strides (in place: only the rotated
  * part is written), or does not overlap it. Any int position; angles are
  * reduced in double. */
 int dsv4b_rope(void *out, int out_dt, long out_tok, long out_head, const void *x, int x_dt, long x_tok,

@@ -43,3 +43,16 @@ def test_selftest_refusals():
     assert f(1000, None) == -2
     for bad in (0, -1, 1000001):
         assert f(bad, None) == -1
+
+
+def test_rope_takes_heads_by_heads():
+    """out may lie heads first, in place too; overlapping heads are refused."""
+    T.no_device()
+    c = B.rope_cfg(64, 1e4)
+    args = dict(T.ROPE, cfg=C.byref(c), out_tok=512, out_head=3 * 512)
+    assert T.call("dsv4b_rope", args) == -2
+    assert T.call("dsv4b_rope", args, x_tok=512, x_head=3 * 512) == -2
+    assert T.call("dsv4b_rope", args, x=P, x_dt=B.F32, x_tok=512, x_head=3 * 512) == -2
+    for bad in (dict(out_head=3 * 512 - 1), dict(out_tok=511), dict(out_tok=0), dict(out_tok=-512),
+                dict(x=P, x_dt=B.F32)):
+        assert T.call("dsv4b_rope", args, **bad) == -1, bad

@@ -126,6 +126,27 @@ def test_rows_at_the_ends_of_the_scales(f):
     close(T.run_tree(k), want, tol)
 
 
+# ------------------------------------------------------------------- layouts
+
+@pytest.mark.parametrize("n,h,w,rd,first,layout,src,dst", [(5, 8, 512, 64, 448, 0, "f32", "bf16"), (33, 3, 64, 32, 16, 1, "bf16", "f32"),
+                                                           (7, 4, 37, 34, 3, 0, "f16", "f16"), (200, 2, 24, 8, 8, 1, "f32", "f32")])
+def test_rope_heads_first(n, h, w, rd, first, layout, src, dst):
+    """[heads, tokens, width] seen as [tokens, heads, width], in x, out or both, and in place."""
+    g = gen(n)
+    cfg = B.rope_cfg(rd, 1e4, layout=layout)
+    x = normal(g, n, h, w).to(DT[src])
+    pos = torch.randint(0, 1 << 20, (n,), generator=g, device="cuda", dtype=torch.int32)
+    want, size = T.turned(x, pos, cfg, first, False)
+    xt = x.transpose(0, 1).contiguous()
+    for a in (x, xt.transpose(0, 1)):
+        out = torch.full((h, n + 2, w), 7.0, dtype=DT[dst], device="cuda")
+        B.rope_dev(out[:, 1:1 + n].transpose(0, 1), a, pos, cfg, first)
+        close(out[:, 1:1 + n].transpose(0, 1), want, T.rope_tol(want, size, DT[dst]))
+        assert torch.all(out[:, 0] == 7.0) and torch.all(out[:, 1 + n:] == 7.0)
+    B.rope_dev(xt.transpose(0, 1), xt.transpose(0, 1), pos, cfg, first)
+    close(xt.transpose(0, 1), want, T.rope_tol(want, size, DT[src]))
+
+
 # ------------------------------------------------------------------- scratch
 
 def test_one_scratch_for_smaller_calls():

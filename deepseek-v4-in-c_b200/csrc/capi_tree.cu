@@ -32,14 +32,35 @@ bool rope_arg(const dsv4b_rope_cfg *r, RopeArg &a)
     return true;
 }
 
-// Bytes [lo, hi) that a strided array spans; strides in elements, all >= 0.
+// A strided array [n0][n1][n2] in bytes; strides in elements, all >= 0.
 struct Span {
-    uintptr_t lo, hi;
+    uintptr_t at;
+    long n[2], step[2], row;
     Span(const void *p, int size, long n0, long s0, long n1, long s1, long n2)
-        : lo((uintptr_t)p), hi((uintptr_t)p + (size_t)((n0 - 1) * s0 + (n1 - 1) * s1 + n2) * size)
+        : at((uintptr_t)p), n{n0, n1}, step{s0 * size, s1 * size}, row(n2 * size)
     {
     }
-    bool meets(const Span &o) const { return lo < o.hi && o.lo < hi; }
+    // Bytes past `at` that its elements reach, by their place modulo `period`
+    // (0: their place itself).
+    uintptr_t reach(long period) const
+    {
+        uintptr_t r = (uintptr_t)row;
+        for (int i = 0; i < 2; i++)
+            if (period == 0 || step[i] % period) r += (uintptr_t)(n[i] - 1) * step[i];
+        return r;
+    }
+    // Whether an element may lie in both: not when the whole ranges are apart,
+    // or the places within a common period (column ranges of one wider array).
+    bool meets(const Span &o) const
+    {
+        if (at + reach(0) <= o.at || o.at + o.reach(0) <= at) return false;
+        for (long p : step) {
+            if (p <= 0) continue;
+            const uintptr_t d = (o.at % p + p - at % p) % p;
+            if (d >= reach(p) && d + o.reach(p) <= (uintptr_t)p) return false;
+        }
+        return true;
+    }
 };
 
 bool aligned(const void *p, size_t n) { return ((uintptr_t)p % n) == 0; }

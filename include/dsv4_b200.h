@@ -430,7 +430,7 @@ int dsv4b_kv_read(const dsv4b_kvq *c, void *out, int dt, long row_stride, const 
  * positions; position j is row j % page_rows of page pages[b][j / page_rows]
  * (a page outside the cache is skipped; a cache holds less than 2^38 bytes of
  * codes). Keys and values are the same rows,
- * shared by all heads; sink[h] (may be NULL) joins the denominator only
+ * shared by all heads; o does not overlap q; sink[h] (may be NULL) joins the denominator only
  * (src/core/dsv4_attn.c:60-108); with nothing to attend to the output is
  * zero. Tokens t >= n_draft[b] are not written (n_draft NULL: n_tok each).
  * Scores, the softmax's sums and the output are float until the output is

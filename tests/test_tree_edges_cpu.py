@@ -56,3 +56,32 @@ def test_rope_takes_heads_by_heads():
     for bad in (dict(out_head=3 * 512 - 1), dict(out_tok=511), dict(out_tok=0), dict(out_tok=-512),
                 dict(x=P, x_dt=B.F32)):
         assert T.call("dsv4b_rope", args, **bad) == -1, bad
+
+
+def test_column_ranges_of_one_array_do_not_overlap():
+    """Input and output as parts of the same rows, tokens or heads."""
+    T.no_device()
+    c = B.rope_cfg(64, 1e4)
+    w, h, n = 512, 8, 3
+    rope = dict(T.ROPE, cfg=C.byref(c), x_dt=B.F32, x=P, out_tok=2 * h * w, x_tok=2 * h * w)
+    assert T.call("dsv4b_rope", rope, out=P + 4 * h * w) == -2               # heads 8 .. 15 of each token
+    assert T.call("dsv4b_rope", rope, out=P, x=P + 4 * h * w) == -2
+    heads = dict(rope, out_head=2 * w, x_head=2 * w)
+    assert T.call("dsv4b_rope", heads, out=P + 4 * w) == -2                  # the second half of each head
+    by_head = dict(rope, out_tok=w, x_tok=w, out_head=2 * n * w, x_head=2 * n * w)
+    assert T.call("dsv4b_rope", by_head, out=P + 4 * n * w) == -2
+    for bad in (dict(rope, out=P + 4 * h * w - 4), dict(rope, out=P + 4 * h * w + 4), dict(heads, out=P + 4 * w - 4),
+                dict(heads, out=P + 4 * w + 4), dict(by_head, out=P + 4 * n * w + 4),
+                dict(rope, out=P + 4 * h * w, x_tok=2 * h * w + 1), dict(rope, out=P + 4 * h * w, x_dt=B.BF16),
+                dict(rope, out=P + 4 * w, x_head=0, x_tok=w)):
+        assert T.call("dsv4b_rope", bad) == -1
+    assert T.call("dsv4b_rope", rope, out=P + 4 * h * w, x_head=0) == -2     # one head of x for all
+    t = 64 * 512
+    attn = dict(o=P + 2 * t, q=P, dt=B.BF16, o_tok=2 * t, q_tok=2 * t, c=T.cache(), pages=P, max_pages=16, ctx=P,
+                n_draft=None, mask=P, sink=None, n_heads=64, n_tok=8, batch=2, max_ctx=1000, scale=0.1, scratch=P,
+                bytes=B.tree_attn_scratch(64, 512, 8, 2, 1000), stream=None)
+    assert T.call("dsv4b_tree_attn", attn) == -2 and T.call("dsv4b_tree_attn", attn, o=P, q=P + 2 * t) == -2
+    assert T.call("dsv4b_tree_attn", attn, o=P + 2 * t - 16) == -1 and T.call("dsv4b_tree_attn", attn, q_tok=t) == -1
+    lg = dict(out=P + 4000, x=P, dt=B.F32, os=2000, xs=2000, token=P, adj=None, rows=3, vocab=1000, stream=None)
+    assert T.call("dsv4b_logits", lg) == -2
+    assert T.call("dsv4b_logits", lg, out=P + 3996) == -1 and T.call("dsv4b_logits", lg, xs=1000) == -1

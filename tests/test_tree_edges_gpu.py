@@ -147,6 +147,26 @@ def test_rope_heads_first(n, h, w, rd, first, layout, src, dst):
     close(xt.transpose(0, 1), want, T.rope_tol(want, size, DT[src]))
 
 
+def test_parts_of_one_array():
+    """Input and output beside each other in the same tokens, heads or rows."""
+    g = gen(55)
+    cfg = B.rope_cfg(32, 1e4)
+    buf = normal(g, 6, 4, 128)
+    x, pos = buf[..., :64].clone(), torch.arange(6, dtype=torch.int32, device="cuda") * 9
+    want, size = T.turned(x, pos, cfg, 16, False)
+    B.rope_dev(buf[..., 64:], buf[..., :64], pos, cfg, 16)
+    close(buf[..., 64:], want, T.rope_tol(want, size, torch.float32))
+    assert torch.equal(buf[..., :64], x)
+    k = T.tree_case(56, 2, 3, 8, 128, 64, 64, 300, torch.bfloat16)
+    ref = T.run_tree(k)
+    both = torch.cat((k["q"], torch.full_like(k["q"], 11.0)), 2)
+    T.run_tree(dict(k, q=both[:, :, :8]), out=both[:, :, 8:])
+    assert torch.equal(both[:, :, 8:], ref) and torch.equal(both[:, :, :8], k["q"])
+    rows = torch.cat((3 * normal(g, 5, 1000), torch.zeros((5, 1000), device="cuda")), 1)
+    B.logits_dev(rows[:, 1000:], rows[:, :1000], None)
+    assert torch.equal(rows[:, 1000:], rows[:, :1000])
+
+
 # ------------------------------------------------------------------- scratch
 
 def test_one_scratch_for_smaller_calls():

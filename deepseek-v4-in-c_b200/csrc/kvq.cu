@@ -187,15 +187,16 @@ int kv_write(const dsv4b_kvq &c, const void *rows, int dt, long row_stride, cons
     if (n <= 0) return 0;
     RopeArg none = {};
     const dim3 grid((n + KQ_W - 1) / KQ_W);
+    cudaError_t e = cudaSuccess;
     DSV4B_ROW_DT(dt, DT, {
         if (rows_vec(rows, dt, row_stride))
-            launch(k_kv_write<DT, true>, grid, dim3(KQ_W * 32), 0, st, c, rows, row_stride, slots, n, r ? 1 : 0,
-                   r ? *r : none, pos);
+            e = launch(k_kv_write<DT, true>, grid, dim3(KQ_W * 32), 0, st, c, rows, row_stride, slots, n, r ? 1 : 0,
+                       r ? *r : none, pos);
         else
-            launch(k_kv_write<DT, false>, grid, dim3(KQ_W * 32), 0, st, c, rows, row_stride, slots, n, r ? 1 : 0,
-                   r ? *r : none, pos);
+            e = launch(k_kv_write<DT, false>, grid, dim3(KQ_W * 32), 0, st, c, rows, row_stride, slots, n, r ? 1 : 0,
+                       r ? *r : none, pos);
     });
-    return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
+    return e == cudaSuccess ? 0 : -2;
 }
 
 int kv_read(const dsv4b_kvq &c, void *out, int dt, long row_stride, const long long *slots, int n,
@@ -203,13 +204,14 @@ int kv_read(const dsv4b_kvq &c, void *out, int dt, long row_stride, const long l
 {
     if (n <= 0) return 0;
     const dim3 grid((n + KQ_W - 1) / KQ_W);
+    cudaError_t e = cudaSuccess;
     DSV4B_ROW_DT(dt, DT, {
         if (rows_vec(out, dt, row_stride))
-            launch(k_kv_read<DT, true>, grid, dim3(KQ_W * 32), 0, st, c, out, row_stride, slots, n);
+            e = launch(k_kv_read<DT, true>, grid, dim3(KQ_W * 32), 0, st, c, out, row_stride, slots, n);
         else
-            launch(k_kv_read<DT, false>, grid, dim3(KQ_W * 32), 0, st, c, out, row_stride, slots, n);
+            e = launch(k_kv_read<DT, false>, grid, dim3(KQ_W * 32), 0, st, c, out, row_stride, slots, n);
     });
-    return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
+    return e == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace dsv4b

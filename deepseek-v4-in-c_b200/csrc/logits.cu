@@ -392,11 +392,12 @@ int logits(void *out, const void *x, int dt, long out_stride, long x_stride, int
     const int sz = row_dt_size(dt);
     const bool vec = !(((uintptr_t)x | (uintptr_t)out) & 15) && !((x_stride * sz) & 15) && !((out_stride * sz) & 15);
     const size_t smem = lg_smem(c.run, a.hist || a.bias, a.bias), most = lg_smem(LG_RUN, true, true);
+    cudaError_t e = cudaSuccess;
     DSV4B_ROW_DT(dt, DT, {
         const auto k = nb == 8 ? (vec ? k_logits<DT, true, 8> : k_logits<DT, false, 8>)
                                : (vec ? k_logits<DT, true, 4> : k_logits<DT, false, 4>);
         if (smem_optin(k, most)) return -2;
-        for (int r0 = 0; r0 < rows; r0 += 32768) {
+        for (int r0 = 0; r0 < rows && e == cudaSuccess; r0 += 32768) {
             const int nr = rows - r0 < 32768 ? rows - r0 : 32768;
             LogitsCall p = c;
             p.x = reinterpret_cast<const char *>(x) + (size_t)r0 * x_stride * sz;
@@ -409,10 +410,10 @@ int logits(void *out, const void *x, int dt, long out_stride, long x_stride, int
             if (a.pres) p.a.pres += r0;
             if (a.bias) p.a.bias += (size_t)r0 * a.bias_stride, p.a.bias_ids += (size_t)r0 * a.bias_stride, p.a.bias_len += r0;
             if (a.mask) p.a.mask += (size_t)r0 * a.mask_stride;
-            launch(k, dim3(nb, nr), dim3(LG_T), smem, st, p);
+            e = launch(k, dim3(nb, nr), dim3(LG_T), smem, st, p);
         }
     });
-    return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
+    return e == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace dsv4b

@@ -145,11 +145,12 @@ int rope(const RopeCall &c, const RopeArg &r, cudaStream_t st)
     while (hpb > 1 && (long)c.n_tok * ((c.n_heads + hpb - 1) / hpb) < 148) hpb = (hpb + 1) / 2;
     const dim3 grid(c.n_tok, (c.n_heads + hpb - 1) / hpb);
     if (grid.y > 65535) return -1;
+    cudaError_t e = cudaSuccess;
     DSV4B_ROW_DT(c.x_dt, XDT, DSV4B_ROW_DT(c.out_dt, ODT, {
-        if (vec) launch(k_rope<XDT, ODT>, grid, dim3(RP_T), 0, st, c, r, hpb);
-        else launch(k_rope_any<XDT, ODT>, grid, dim3(RP_T), 0, st, c, r, hpb);
+        if (vec) e = launch(k_rope<XDT, ODT>, grid, dim3(RP_T), 0, st, c, r, hpb);
+        else e = launch(k_rope_any<XDT, ODT>, grid, dim3(RP_T), 0, st, c, r, hpb);
     }));
-    return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
+    return e == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace dsv4b

@@ -1107,9 +1107,9 @@ int run(const Args &g, const Plan &p, size_t smem, cudaStream_t st)
 {
     if (smem_optin(k_tree_attn<NR>, TA_SMEM)) return -2;
     PdlChain chain;
-    launch(k_tree_attn<NR>, dim3((unsigned)p.blocks), dim3(TA_T), smem, st, g);
-    if (p.nsplit > 1) launch(k_tree_join, dim3(g.a.n_tok * g.a.n_heads, g.a.batch), dim3(128), 0, st, g);
-    return cudaPeekAtLastError() == cudaSuccess ? 0 : -2;
+    cudaError_t e = launch(k_tree_attn<NR>, dim3((unsigned)p.blocks), dim3(TA_T), smem, st, g);
+    if (p.nsplit > 1 && e == cudaSuccess) e = launch(k_tree_join, dim3(g.a.n_tok * g.a.n_heads, g.a.batch), dim3(128), 0, st, g);
+    return e == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace

@@ -3,6 +3,10 @@ unusual: cache rows of very different magnitude, layouts, streams, scratch of
 another size, errors of earlier calls. Against the same 64-bit definitions and
 roundings as test_tree_gpu.py.
 """
+import os
+import subprocess
+import sys
+
 import pytest
 
 import dsv4_b200 as B
@@ -212,3 +216,34 @@ def test_status_reports_a_wait_once():
     want, tol = T.plain_tree(k)
     close(T.run_tree(k), want, tol)
     assert B.tree_attn_status(torch.cuda.current_device())
+
+
+# -------------------------------------------------------------------- errors
+
+def test_an_earlier_error_is_not_this_call_s():
+    """An allocation of this library that failed (824 GB, refused at once) leaves
+    its error code behind; launches that follow succeed, and say so. In a
+    process of its own, as the code stays there."""
+    code = """
+import ctypes as C, numpy as np, torch, dsv4_b200 as B, test_tree_gpu as T
+B.init()
+buf = np.zeros(4, np.float32)
+fail = C.CDLL(B.LIB_PATH).dsv4b_peer_selftest
+fail.argtypes = [C.c_int, C.c_int, C.c_uint, C.c_int, C.c_void_p, C.c_void_p]
+assert fail(64, (1 << 30) - 4, 1, 1, buf.ctypes.data, buf.ctypes.data) == -1
+x = T.normal(T.gen(57), 2, 3, 64)
+out, pos = torch.empty_like(x), torch.arange(2, dtype=torch.int32, device="cuda")
+B.rope_dev(out, x, pos, B.rope_cfg(64, 1e4), 0)
+c, at = B.KvCache.empty(1, 16, 64, 0), torch.arange(2, device="cuda")
+B.kv_write_dev(c, x[:, 0].contiguous(), at)
+B.kv_read_dev(out[:, 0], c, at)
+B.logits_dev(None, x[:, 0], torch.empty(2, dtype=torch.int32, device="cuda"))
+k = T.tree_case(58, 1, 2, 8, 128, 64, 64, 2000, torch.bfloat16)
+want, tol = T.plain_tree(k)
+T.close(T.run_tree(k), want, tol)
+print("every launch succeeded")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join((here, os.path.dirname(B.LIB_PATH))))
+    r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "every launch succeeded" in r.stdout, r.stderr

@@ -370,7 +370,9 @@ def sparse_attn_dev(o, q, kv, kv_dt, seq_kv_rows, sink, idxs, n_heads, d, topk_n
 #
 # These take torch CUDA tensors of one device and check them (ValueError) before
 # the C ABI does. With stream=None they run on torch's current stream of that
-# device, so they are ordered after the torch work that made their tensors.
+# device, so they are ordered after the torch work that made their tensors. With
+# another stream the caller orders it (Stream.wait_stream); its tensors' memory is
+# not given out again before the call there has ended.
 
 F16 = 3
 _t = None                       # torch, imported by the first of these calls
@@ -408,13 +410,17 @@ def _want(t, what, dev, dtype, shape=None):
     return t.data_ptr()
 
 
-def _stream(dev, stream):
+def _stream(dev, stream, tensors):
     """The handle to enqueue on: torch's current stream of the device for None
-    (its default stream by the legacy handle, as NULL is the backend's own)."""
+    (its default stream by the legacy handle, as NULL is the backend's own).
+    The tensors of a call on a given stream are recorded there."""
     if stream is None:
         return _t._C._cuda_getCurrentRawStream(dev) or 1
     if stream.device.index != dev:
         raise ValueError("the stream belongs to another device than the tensors")
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
     return stream.cuda_stream or 1
 
 
@@ -456,7 +462,7 @@ def rope_dev(out, x, pos, cfg, first, inverse=False, stream=None):
     xt, ot = (xs[0], os_[0]) if n > 1 else ((h - 1) * xh + w, (h - 1) * oh + w)
     _enqueue(lib().dsv4b_rope, "dsv4b_rope", dev, out.data_ptr(), _dt(out, "out"), ot, oh, x.data_ptr(), _dt(x, "x"),
              xt, xh, C.addressof(cfg), _want(pos, "pos", dev, i32, (n,)), n, h, w, int(first), 1 if inverse else 0,
-             _stream(dev, stream))
+             _stream(dev, stream, (out, x, pos)))
 
 
 class KvCache:
@@ -506,7 +512,8 @@ def kv_write_dev(cache, rows, slots, rope=None, pos=None, stream=None):
         raise ValueError("rope and pos go together")
     _enqueue(lib().dsv4b_kv_write, "dsv4b_kv_write", dev, cache.ref, p, dt, st,
              _want(slots, "slots", dev, _t.int64, (n,)), n, None if rope is None else C.addressof(rope),
-             None if pos is None else _want(pos, "pos", dev, _t.int32, (n,)), _stream(dev, stream))
+             None if pos is None else _want(pos, "pos", dev, _t.int32, (n,)),
+             _stream(dev, stream, (cache.codes, cache.scales, rows, slots, pos)))
 
 
 def kv_read_dev(out, cache, slots, stream=None):
@@ -515,7 +522,8 @@ def kv_read_dev(out, cache, slots, stream=None):
     p, dt, st, n = _rows(out, "out", cache)
     dev = cache.device
     _enqueue(lib().dsv4b_kv_read, "dsv4b_kv_read", dev, cache.ref, p, dt, st,
-             _want(slots, "slots", dev, _t.int64, (n,)), n, _stream(dev, stream))
+             _want(slots, "slots", dev, _t.int64, (n,)), n,
+             _stream(dev, stream, (out, cache.codes, cache.scales, slots)))
 
 
 def tree_mask(parents):
@@ -567,7 +575,8 @@ def tree_attn_dev(o, q, cache, pages, ctx, n_draft, mask, sink, max_ctx, scale, 
              None if n_draft is None else _want(n_draft, "n_draft", dev, i32, (b,)),
              _want(mask, "mask", dev, _t.int64, (b, t)),
              None if sink is None else _want(sink, "sink", dev, _t.float32, (h,)), h, t, b, int(max_ctx),
-             float(scale), scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream(dev, stream))
+             float(scale), scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+             _stream(dev, stream, (o, q, cache.codes, cache.scales, pages, ctx, n_draft, mask, sink, scratch)))
 
 
 def tree_attn_status(device=None):
@@ -644,7 +653,7 @@ def logits_dev(out, x, token, adjust=None, stream=None):
         raise ValueError("the adjustments are for other rows or another device")
     _enqueue(lib().dsv4b_logits, "dsv4b_logits", dev, po, x.data_ptr(), _dt(x, "x"), so, xs[0] if r > 1 else v,
              None if token is None else _want(token, "token", dev, i32, (r,)), None if adjust is None else adjust.ref,
-             r, v, _stream(dev, stream))
+             r, v, _stream(dev, stream, (out, x, token) + (adjust.keep if adjust is not None else ())))
 
 
 # ------------------------------------------------------------- whole model

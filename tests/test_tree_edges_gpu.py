@@ -247,3 +247,50 @@ print("every launch succeeded")
     env = dict(os.environ, PYTHONPATH=os.pathsep.join((here, os.path.dirname(B.LIB_PATH))))
     r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "every launch succeeded" in r.stdout, r.stderr
+
+
+# ------------------------------------------------------------------- streams
+
+def test_memory_of_a_call_on_another_stream_is_kept():
+    """Tensors dropped while a side stream has yet to run the call that reads or
+    writes them: their memory is not given out before."""
+    side = torch.cuda.Stream()
+    g = gen(59)
+    cfg = B.rope_cfg(64, 1e4)
+    cache = B.KvCache.empty(4, 64, 512, 64)
+    k = T.tree_case(60, 1, 2, 8, 128, 64, 64, 2000, torch.bfloat16)
+    hist = torch.randint(0, 3000, (5, 700), generator=g, device="cuda", dtype=torch.int32)
+    ref = T.run_tree(k)
+
+    def calls(stream):
+        """A call of each kind on tensors of its own; the outputs, and where the rest lay."""
+        x, pos = normal(gen(1), 300, 2, 512), torch.arange(300, dtype=torch.int32, device="cuda")
+        rows, slots = normal(gen(2), 200, 512), torch.arange(200, device="cuda")
+        lg, rep = 3 * normal(gen(3), 5, 3000), torch.full((5,), 1.3, device="cuda")
+        adj = B.LogitAdjust(hist=hist.clone(), hist_len=torch.full((5,), 700, dtype=torch.int32, device="cuda"), rep=rep)
+        q, mask = k["q"].clone(), k["mask"].clone()
+        scratch = torch.empty(B.tree_attn_scratch(8, 128, 2, 1, 2000), dtype=torch.uint8, device="cuda")
+        outs = [torch.zeros_like(x), torch.zeros((200, 512), device="cuda"), torch.zeros_like(lg),
+                torch.zeros(5, dtype=torch.int32, device="cuda"), torch.zeros_like(q)]
+        if stream is not None:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                torch.cuda._sleep(200_000_000)             # about 100 ms
+        B.rope_dev(outs[0], x, pos, cfg, 0, stream=stream)
+        B.kv_write_dev(cache, rows, slots, rope=cfg, pos=pos[:200], stream=stream)
+        B.kv_read_dev(outs[1], cache, slots, stream=stream)
+        B.logits_dev(outs[2], lg, outs[3], adj, stream=stream)
+        T.run_tree(dict(k, q=q, mask=mask), out=outs[4], scratch=scratch, stream=stream)
+        return outs, [t.data_ptr() for t in (x, pos, rows, slots, lg, rep, adj.keep[0], adj.keep[1], q, mask, scratch)], \
+            [(t.shape, t.dtype) for t in (x, pos, rows, slots, lg, rep, adj.keep[0], adj.keep[1], q, mask, scratch)]
+
+    want = calls(None)[0]
+    torch.cuda.synchronize()
+    got, at, kinds = calls(side)
+    later = [torch.zeros(s, dtype=d, device="cuda") for s, d in kinds for _ in range(3)]
+    assert not side.query()                                # the calls are still to come
+    assert not {t.data_ptr() for t in later} & set(at)
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert torch.equal(got[4], ref)

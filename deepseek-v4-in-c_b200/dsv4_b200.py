@@ -388,6 +388,18 @@ def _torch():
     return _t
 
 
+def _int(v, what):
+    """v as a C int: ctypes would keep its low 32 bits."""
+    v = int(v)
+    if not -0x80000000 <= v <= 0x7FFFFFFF:
+        raise ValueError("%s is out of range" % what)
+    return v
+
+
+def _too_long():
+    raise ValueError("a size or an offset is not in 0 .. 2^31 - 1")
+
+
 def _dt(t, what):
     """The row type (F32, BF16, F16) of a tensor."""
     dt = _row_dt.get(t.dtype)
@@ -439,8 +451,8 @@ def rope_cfg(rd, base, layout=ROPE_INTERLEAVED, factor=1.0, orig=0, beta_fast=32
     """Frequencies of a rotation of rd elements (dsv4b_rope_init); orig > 0
     scales them by factor for contexts beyond orig positions."""
     r = RopeCfg()
-    check(lib().dsv4b_rope_init(C.byref(r), int(rd), int(layout), float(base), float(factor), int(orig),
-                                float(beta_fast), float(beta_slow)), "dsv4b_rope_init")
+    check(lib().dsv4b_rope_init(C.byref(r), _int(rd, "rd"), _int(layout, "layout"), float(base), float(factor),
+                                _int(orig, "orig"), float(beta_fast), float(beta_slow)), "dsv4b_rope_init")
     return r
 
 
@@ -457,11 +469,14 @@ def rope_dev(out, x, pos, cfg, first, inverse=False, stream=None):
     if dev < 0 or out.get_device() != dev:
         raise ValueError("x and out must be on one CUDA device")
     n, h, w = shape
+    first = int(first)
+    if (n | h | w | first) >> 31:
+        _too_long()
     # torch leaves the stride of a length-1 axis free
     xh, oh = (xs[1], os_[1]) if h > 1 else (w, w)
     xt, ot = (xs[0], os_[0]) if n > 1 else ((h - 1) * xh + w, (h - 1) * oh + w)
     _enqueue(lib().dsv4b_rope, "dsv4b_rope", dev, out.data_ptr(), _dt(out, "out"), ot, oh, x.data_ptr(), _dt(x, "x"),
-             xt, xh, C.addressof(cfg), _want(pos, "pos", dev, i32, (n,)), n, h, w, int(first), 1 if inverse else 0,
+             xt, xh, C.addressof(cfg), _want(pos, "pos", dev, i32, (n,)), n, h, w, first, 1 if inverse else 0,
              _stream(dev, stream, (out, x, pos)))
 
 
@@ -499,6 +514,8 @@ def _rows(t, what, cache):
     s, n = t.stride(), t.shape
     if len(n) != 2 or n[1] != cache.d or s[1] != 1 or t.get_device() != cache.device:
         raise ValueError("%s must be [n, d] with unit-stride rows on the cache's device" % what)
+    if n[0] >> 31:
+        _too_long()
     return t.data_ptr(), _dt(t, what), s[0] if n[0] > 1 else cache.d, n[0]
 
 
@@ -540,7 +557,8 @@ def tree_mask(parents):
 
 def tree_attn_scratch(n_heads, d, n_tok, batch, max_ctx):
     """Bytes of scratch a tree_attn_dev call of these sizes, or smaller ones, needs."""
-    n = lib().dsv4b_tree_attn_scratch(int(n_heads), int(d), int(n_tok), int(batch), int(max_ctx))
+    n = lib().dsv4b_tree_attn_scratch(_int(n_heads, "n_heads"), _int(d, "d"), _int(n_tok, "n_tok"), _int(batch, "batch"),
+                                      _int(max_ctx, "max_ctx"))
     if n == 0:
         raise ValueError("sizes that dsv4b_tree_attn does not take")
     return n
@@ -567,6 +585,9 @@ def tree_attn_dev(o, q, cache, pages, ctx, n_draft, mask, sink, max_ctx, scale, 
         tok.append(st)
     if pages.dim() != 2 or pages.shape[0] != b:
         raise ValueError("pages must be [batch, max_pages]")
+    max_ctx = int(max_ctx)
+    if (b | t | h | max_ctx | pages.shape[1]) >> 31:
+        _too_long()
     if scratch.get_device() != dev or not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous, on the cache's device")
     i32 = _t.int32
@@ -574,7 +595,7 @@ def tree_attn_dev(o, q, cache, pages, ctx, n_draft, mask, sink, max_ctx, scale, 
              cache.ref, _want(pages, "pages", dev, i32), pages.shape[1], _want(ctx, "ctx", dev, i32, (b,)),
              None if n_draft is None else _want(n_draft, "n_draft", dev, i32, (b,)),
              _want(mask, "mask", dev, _t.int64, (b, t)),
-             None if sink is None else _want(sink, "sink", dev, _t.float32, (h,)), h, t, b, int(max_ctx),
+             None if sink is None else _want(sink, "sink", dev, _t.float32, (h,)), h, t, b, max_ctx,
              float(scale), scratch.data_ptr(), scratch.numel() * scratch.element_size(),
              _stream(dev, stream, (o, q, cache.codes, cache.scales, pages, ctx, n_draft, mask, sink, scratch)))
 
@@ -643,6 +664,8 @@ def logits_dev(out, x, token, adjust=None, stream=None):
     if len(shape) != 2 or xs[1] != 1 or dev < 0:
         raise ValueError("x must be a CUDA tensor [rows, vocab] with unit-stride rows")
     r, v = shape
+    if (r | v) >> 31:
+        _too_long()
     po = so = 0
     if out is not None:
         so = out.stride()

@@ -85,3 +85,15 @@ def test_column_ranges_of_one_array_do_not_overlap():
     lg = dict(out=P + 4000, x=P, dt=B.F32, os=2000, xs=2000, token=P, adj=None, rows=3, vocab=1000, stream=None)
     assert T.call("dsv4b_logits", lg) == -2
     assert T.call("dsv4b_logits", lg, out=P + 3996) == -1 and T.call("dsv4b_logits", lg, xs=1000) == -1
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Not cut to their low 32 bits."""
+    far = 1 << 32
+    for bad in ((64 + far, 512, 1, 1, 1), (64, 512 + far, 1, 1, 1), (64, 512, 1 + far, 1, 1), (64, 512, 1, 1 + far, 1),
+                (64, 512, 1, 1, 1 + far), (64, 512, 1, 1, -far)):
+        with pytest.raises(ValueError):
+            B.tree_attn_scratch(*bad)
+    for bad in (dict(rd=64 + far), dict(layout=far), dict(orig=far + 8)):
+        with pytest.raises(ValueError):
+            B.rope_cfg(**dict(dict(rd=64, base=1e4), **bad))

@@ -294,3 +294,14 @@ def test_memory_of_a_call_on_another_stream_is_kept():
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert torch.equal(got[4], ref)
+
+
+def test_sizes_past_32_bits_are_refused():
+    far = 1 << 32
+    x = torch.zeros((3, 1, 128), device="cuda")
+    pos = torch.zeros(3, dtype=torch.int32, device="cuda")
+    k = T.tree_case(97, 1, 1, 8, 128, 64, 64, 60, torch.bfloat16)
+    scratch = torch.empty(B.tree_attn_scratch(8, 128, 1, 1, 60), dtype=torch.uint8, device="cuda")
+    for bad in (lambda: B.rope_dev(x, x, pos, B.rope_cfg(64, 1e4), far), lambda: T.run_tree(dict(k, max_ctx=60 + far), scratch=scratch)):
+        with pytest.raises(ValueError):
+            bad()

@@ -305,3 +305,106 @@ def test_sizes_past_32_bits_are_refused():
     for bad in (lambda: B.rope_dev(x, x, pos, B.rope_cfg(64, 1e4), far), lambda: T.run_tree(dict(k, max_ctx=60 + far), scratch=scratch)):
         with pytest.raises(ValueError):
             bad()
+
+
+# ------------------------------------------------------- values and sizes
+
+def test_query_rows_that_are_not_finite_spoil_no_others():
+    for dtype in (torch.bfloat16, torch.float16):
+        k = T.tree_case(100, 2, 3, 16, 256, 64, 64, 900, dtype)
+        want, tol = T.plain_tree(k)
+        ref = T.run_tree(k)
+        bad = torch.zeros(k["q"].shape[:3], dtype=torch.bool, device="cuda")
+        k["q"][0, 1, 3, 7], k["q"][1, 2, 15, 255], k["q"][1, 0, 0] = float("nan"), float("inf"), -float("inf")
+        bad[0, 1, 3] = bad[1, 2, 15] = bad[1, 0, 0] = True
+        out = T.run_tree(k)
+        assert torch.isnan(out[bad]).all()
+        close(out[~bad], want[~bad], tol[~bad])
+        assert torch.equal(out[~bad], ref[~bad])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 2.0 ** -140])
+def test_scales_of_any_sign(scale):
+    k = dict(T.tree_case(101, 2, 3, 16, 256, 64, 64, 900, torch.bfloat16), scale=scale)
+    want, tol = T.plain_tree(k)
+    close(T.run_tree(k), want, tol)
+
+
+def test_sinks_at_their_ends():
+    """An infinite sink takes everything, one of -infinity nothing, NaN its own head."""
+    k = T.tree_case(102, 2, 2, 8, 128, 64, 64, 1500, torch.bfloat16)
+    free, tol = T.plain_tree(dict(k, sink=None))
+    want, tol2 = T.plain_tree(k)
+    k["sink"][1], k["sink"][2], k["sink"][3] = float("inf"), -float("inf"), float("nan")
+    out = T.run_tree(k)
+    assert not out[:, :, 1].any() and torch.isnan(out[:, :, 3]).all()
+    close(out[:, :, 2], free[:, :, 2], tol[:, :, 2])
+    for h in (0, 4, 5, 6, 7):
+        close(out[:, :, h], want[:, :, h], tol2[:, :, h])
+
+
+def test_most_heads_and_tokens():
+    k = T.tree_case(103, 1, 64, 1024, 64, 0, 64, 200, torch.bfloat16)
+    out = T.run_tree(k)
+    for t in (0, 1, 31, 63):
+        part = dict(k, q=k["q"][:, t:t + 1], mask=k["mask"][:, t:t + 1])
+        # one token's row of the definition: its mask over all 64 drafted rows
+        n = 200 + 64
+        v = T.decode(k["c"], slots_of(k, 0, n))
+        see = torch.ones(n, dtype=torch.bool, device="cuda")
+        bits = int(part["mask"][0, 0])
+        for z in range(64):
+            see[200 + z] = bool((bits >> z) & 1)
+        z = part["q"][0, 0].double() @ v[see].T * k["scale"]
+        w = torch.cat((z, k["sink"].double()[:, None]), -1).softmax(-1)[:, :-1]
+        mag = (k["scale"] * part["q"][0, 0].double().abs() @ v[see].abs().T).amax(-1, keepdim=True)
+        delta = mag * 8 * 2.0 ** -22 + 2.0 ** -15               # d / 16 + 4 partial sums of a score, as above
+        want = w @ v[see]
+        size = w @ v[see].abs()
+        close(out[0, t], want, size * (2.0 ** -11 + 2 * delta) + 2.0 ** -20 * v.abs().amax() + 2.0 ** -8 * 1.001 * want.abs())
+
+
+def test_a_given_stream_inside_a_capture():
+    """stream= naming the stream that is being captured."""
+    k = T.tree_case(104, 1, 2, 8, 128, 64, 64, 900, torch.bfloat16)
+    ref = T.run_tree(k)
+    out = torch.full_like(ref, 11.0)
+    scratch = torch.empty(B.tree_attn_scratch(8, 128, 2, 1, 900), dtype=torch.uint8, device="cuda")
+    x = 3 * normal(gen(105), 2, 5000)
+    tok, first = torch.empty(2, dtype=torch.int32, device="cuda"), torch.empty(2, dtype=torch.int32, device="cuda")
+    B.logits_dev(None, x, first)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        T.run_tree(k, out=out, scratch=scratch, stream=side)
+        B.logits_dev(None, x, tok, stream=side)
+    for _ in range(2):
+        out.fill_(11.0)
+        tok.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref) and torch.equal(tok, first)
+
+
+def test_more_rows_of_logits_than_a_launch_takes():
+    r, v = 32770, 40
+    g = gen(106)
+    x = 3 * normal(g, r, v)
+    kw = dict(hist=torch.randint(0, v, (r, 5), generator=g, device="cuda", dtype=torch.int32),
+              hist_len=torch.randint(0, 6, (r,), generator=g, device="cuda", dtype=torch.int32),
+              n_prompt=torch.randint(0, 3, (r,), generator=g, device="cuda", dtype=torch.int32),
+              rep=0.5 + torch.rand(r, generator=g, device="cuda"), freq=0.3 * normal(g, r), pres=normal(g, r),
+              bias_ids=torch.randint(0, v, (r, 3), generator=g, device="cuda", dtype=torch.int32), bias=normal(g, r, 3),
+              bias_len=torch.full((r,), 3, dtype=torch.int32, device="cuda"),
+              mask=torch.randint(-2 ** 31, 2 ** 31, (r, 2), generator=g, device="cuda").to(torch.int32))
+    out, tok = torch.empty_like(x), torch.empty(r, dtype=torch.int32, device="cuda")
+    B.logits_dev(out, x, tok, B.LogitAdjust(**kw))
+    rows = torch.tensor([0, 1, 32766, 32767, 32768, 32769], device="cuda")
+    part = {n: t[rows] for n, t in kw.items()}
+    want, size = T.plain_logits(x[rows], part["hist"], part["hist_len"], part["n_prompt"], part["rep"], part["freq"],
+                                part["pres"], part["bias_ids"], part["bias"], part["bias_len"], part["mask"])
+    # at most six float roundings on the way, then the output's
+    close(out[rows], want, 6.01 * T.U32 * size + T.U32 * (1 + 2 ** -20) * want.abs().nan_to_num(posinf=0) + 2.0 ** -149)
+    top = out.amax(-1)
+    first = torch.where(out == top[:, None], torch.arange(v, device="cuda"), v).amin(-1)
+    assert torch.equal(tok.long(), torch.where(top > -float("inf"), first, -1))

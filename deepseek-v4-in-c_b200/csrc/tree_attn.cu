@@ -864,7 +864,7 @@ k_tree_attn(const __grid_constant__ Args g)
             // 449 us against 419 at 4 x 16 tokens on 32768).
             uint32_t pw[NC / 2];
             if (!__any_sync(0xffffffffu, valid && !(dmax <= 0.0f && kf + dmax <= 100.0f))) {
-                const float as = valid ? ks : 0.0f;
+                const float as = valid && kx < 255 ? ks : 0.0f;     // a NaN row's p is NaN, or 0 where it is hidden
 #pragma unroll
                 for (int i = 0; i < NC; i += 4) {
                     const float4 bs = *reinterpret_cast<const float4 *>(&sh.bs[c0 + i]);

@@ -408,3 +408,21 @@ def test_more_rows_of_logits_than_a_launch_takes():
     top = out.amax(-1)
     first = torch.where(out == top[:, None], torch.arange(v, device="cuda"), v).amin(-1)
     assert torch.equal(tok.long(), torch.where(top > -float("inf"), first, -1))
+
+
+@pytest.mark.parametrize("g", [-60, 0, 20, 60, 90])
+def test_hidden_nan_rows_at_any_magnitude(g):
+    """A NaN row that one token sees and the others do not, among rows near 2^g."""
+    k = T.tree_case(107, 1, 4, 16, 128, 64, 64, 500, torch.bfloat16)
+    rows = normal(gen(108), k["c"].scales.numel(), 128) * 2.0 ** g
+    at = slots_of(k, 0, 504)
+    rows[at[502]] = float("nan")
+    k["mask"][0] = torch.tensor([1, 3, 4, 11], device="cuda")
+    B.kv_write_dev(k["c"], rows, torch.arange(rows.shape[0], device="cuda"))
+    k["scale"] *= 2.0 ** -g
+    out = T.run_tree(k)
+    assert torch.isnan(out[0, 2]).all()
+    B.kv_write_dev(k["c"], torch.zeros((1, 128), device="cuda"), at[502:503])
+    want, tol = weighted(k)
+    keep = torch.tensor([0, 1, 3], device="cuda")
+    close(out[:, keep], want[:, keep], tol[:, keep])

@@ -756,10 +756,10 @@ k_tree_attn(const __grid_constant__ Args g)
                     const float2 v = fma2(make_float2(x[i + 2], x[i + 3]), mul2(make_float2(ks, ks), make_float2(cq.z, cq.w)), make_float2(nm.z, nm.w));
                     x[i] = u.x, x[i + 1] = u.y, x[i + 2] = v.x, x[i + 3] = v.y;
                 }
-                if (drafts && valid && draft >= 0) {        // a key that is there is one of 64 drafted at most
+                if (drafts && draft >= 0) {             // past 63: no key, set below
 #pragma unroll
                     for (int i = 0; i < NC; i++)
-                        if (!((sh.rowmask[c0 + i] >> draft) & 1)) x[i] = -INFINITY;
+                        if (!((sh.rowmask[c0 + i] >> (draft & 63)) & 1)) x[i] = -INFINITY;
                 }
                 if (!valid) {
 #pragma unroll

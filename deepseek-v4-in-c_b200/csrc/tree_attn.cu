@@ -59,12 +59,12 @@
 // two. Each of the tile's rows has two references of its own over the keys it
 // sees: M for x, and R for x + e, which is what a key gives to O. p_j =
 // 2^(x_j - M) and its sum are float. The weight that multiplies codes is
-// 2^(x_j + e_j - R + 7), rounded once to f16: half a step is 2^-11 of it, or
-// 2^-32 of the row's largest below f16's normal range. So a large cache row
+// 2^(x_j + e_j - R + 8), rounded once to f16: half a step is 2^-11 of it, or
+// 2^-31 of the row's largest below f16's normal range. So a large cache row
 // that is hidden or weighs nothing takes no bits from small ones that weigh
 // much (with one reference of scales for all rows, 2^20 between them cost 8 %
 // of the output and 2^26 all of it). References are raised only when a score
-// passes M by 2^8 or a weight 2^15, which fits f16: O^T is almost never
+// passes M by 2^8 or a weight 2^15.5, which fits f16: O^T is almost never
 // rescaled, and no tile needs the exact maximum, only two comparisons per score
 // and one vote per tile. q is widened or scaled per row by a power of two into
 // f16 (exact unless an element is below 2^-29 of its row's largest). S and O
@@ -100,8 +100,8 @@ constexpr int TA_PLACES = 7;                        // most chunk pairs in share
 constexpr int TA_SMEM = 232448;                     // a block's limit
 constexpr int TA_SPLITS = 128;
 constexpr float TA_RAISE = 8.0f;                    // log2 of p that raises the references
-constexpr float TA_LIFT = 7.0f, TA_FULL = 15.0f;    // log2 of the weight at R, and of one that raises them
-constexpr float TA_UNSEEN = -120.0f;                 // 7 - (R - M) of a row that has seen nothing: any number
+constexpr float TA_LIFT = 8.0f, TA_FULL = 15.5f;    // log2 of the weight at R, and of one that raises them
+constexpr float TA_UNSEEN = -120.0f;                // 8 - (R - M) of a row that has seen nothing: any number
 
 struct Parts {              // one entry per (block, row of its tile)
     float *o;               // [d] the block's own average
@@ -121,7 +121,7 @@ struct Shared {             // behind the operand tiles
     uint64_t q_full, key_full, s_full, s_free, p_full, pv_done;
     uint64_t rowmask[TA_ROWS], out_at[TA_ROWS];     // a row's tree mask, and its first output element
     float cq[TA_ROWS], nm[TA_ROWS];     // score factor of a row, and its negated reference M
-    float rr[TA_ROWS], dr[TA_ROWS];     // R - M, and 7 - (R - M) as a whole number
+    float rr[TA_ROWS], dr[TA_ROWS];     // R - M, and 8 - (R - M) as a whole number
     float bs[TA_ROWS], dmax[2];         // 2^(dr + 127), and the largest dr of each half of the rows
     float fo[TA_ROWS], fl[TA_ROWS], wmax[4][TA_ROWS], rmax[4][TA_ROWS], lsum[4][TA_ROWS];
     int kx[TA_KEYS];        // each key's scale byte, -1: not there
@@ -802,8 +802,24 @@ k_tree_attn(const __grid_constant__ Args g)
                 float mine = -INFINITY, mine_r = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < NC; i++) {
-                    const float m = warp_top(x[i]), q = warp_top(m == -INFINITY ? m : (x[i] - m) + kf);
-                    if (lane == i) mine = m, mine_r = q;
+                    const float m = warp_top(x[i]);
+                    if (lane == i) mine = m;
+                }
+                // scales within a factor of two: the largest of them serves as
+                // the maxima of x + e - m, one too high at most (one maximum a
+                // row instead of two: 22.6 us at 3 x 5 tokens of d = 256 on up to
+                // 8000 became 24.1 without this, 23.3 with it)
+                const bool some = valid && kx < 255;
+                const int most = __reduce_max_sync(0xffffffffu, some ? kx : -1);
+                if (most - __reduce_min_sync(0xffffffffu, some ? kx : 255) <= 1) {
+                    if (mine != -INFINITY) mine_r = (float)most;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NC; i++) {
+                        const float m = __shfl_sync(0xffffffffu, mine, i);
+                        const float q = warp_top(m == -INFINITY ? m : (x[i] - m) + kf);
+                        if (lane == i) mine_r = q;
+                    }
                 }
                 if (lane < NC) {
                     sh.wmax[warp & 3][c0 + lane] = fmaxf(mine, -INFINITY);
@@ -913,8 +929,8 @@ k_tree_attn(const __grid_constant__ Args g)
             } else if (a.sink && m != -INFINITY) {
                 den += ex2(__ldcg(a.sink + (r0 + r) % H) * 1.4426950408889634f - m);
             }
-            // O = 2^dr sum p 2^e code; 0 where nothing was seen. -dr - 127 is
-            // above -2^7 - 16 and, as p passes M by 2^8 at most, below 2^7
+            // O = 2^dr sum p 2^e code; 0 where nothing was seen. dr lies in
+            // -247 .. 8: it is set where the largest p is 1
             const int t = -(int)sh.dr[r] - 127, h = max(t, -126);
             sh.fo[r] = m == -INFINITY && sum == 0.0f ? 0.0f : pow2i(t - h) / den;
             sh.fl[r] = pow2i(h);

@@ -436,7 +436,7 @@ int dsv4b_kv_read(const dsv4b_kvq *c, void *out, int dt, long row_stride, const 
  * Scores, the softmax's sums and the output are float until the output is
  * rounded; what a position adds to the output (its weight times its row's
  * scale) is rounded to f16 relative to the largest one that the token and head
- * see: by 2^-11 of itself, or 2^-32 of that largest if more.
+ * see: by 2^-11 of itself, or 2^-31 of that largest if more.
  * ctx[b] is at most max_ctx, which sizes the launch; n_tok <= DSV4B_TREE_MAX.
  * `scratch` holds dsv4b_tree_attn_scratch() bytes, 16-byte aligned, for the
  * duration of the call: calls that may overlap need their own. The size grows

@@ -14,11 +14,13 @@
 //
 // Bound by HBM (d * size + d + tail + 1 bytes a row). One warp per row, 8
 // elements per lane and group of 256: the row stays in registers between the
-// maximum and the codes, so it is read once. Measured at d 512, tail 64: 16000
-// bf16 rows rotated and written in 8.1 us, 16384 read in 5.9 us, both with
-// about 2 us of launch and ramp on traffic that takes 4.4 and 4.0 us; 64 rows
-// written in 3.1 us. Blocks of 4 or 8 warps take the same, of 2 or 16 longer
-// (9.6, 9.1 us).
+// maximum and the codes, so it is read once. Measured at tail 64: 16000 bf16 rows
+// of d 576 written in 7.7 to 8.1 us, 16384 of d 512 read in 5.9 us, both with
+// about 2 us of launch and ramp on traffic that takes 4.4 and 4.0 us. At d 512,
+// 16000 rows take 6.8 us, and rotated 9.9 (13.3 from float): a rotated row costs
+// 427 warp instructions, one of d 576 that is not 295, and 62 to 66 % of the issue
+// slots are used. 64 rows rotated and written in 3.0 us. Blocks of 4 or 8 warps take
+// the same, of 2 or 16 longer (9.6, 9.1 us).
 #include "common.cuh"
 #include "internal.h"
 #include "rows.cuh"

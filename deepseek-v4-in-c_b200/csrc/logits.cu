@@ -34,7 +34,11 @@
 // history (5.7 without), 29 us for 64 rows with up to 8192 (16.1 without
 // history and biases, where the traffic alone takes 10.5); the rest is the
 // latency of the five steps, which two blocks a multiprocessor overlap only in
-// part.
+// part. A block keeps 4096 entries of the history that fall to it and 2048 named
+// tokens; past either it reads the lists again, past the second once for every
+// 2048 of its tokens: 167 us for 64 rows with up to 20000 tokens of text, 351
+// with up to 60000 (418 with 60000 drawn evenly, 48000 of them distinct); one row
+// 20, 87 and 159 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -191,8 +195,6 @@ k_logits(LogitsCall c)
             for (int i = tid; i < (m + 31) >> 5; i += LG_T) bits[i] = 0;
             if (tid == 0) n_list = n_slots = 0;
             __syncthreads();
-            // (one entry for equal tokens of a warp, found by matching, takes
-            // longer than the repeated atomics: 1.5 us at 64 rows)
             // (one entry for equal tokens of a warp, found by matching, takes
             // longer than the repeated atomics: 1.5 us at 64 rows)
             auto mark = [&](int i, const unsigned (&k)[4]) {

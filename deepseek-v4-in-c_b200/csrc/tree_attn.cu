@@ -46,8 +46,8 @@
 //   8 softmax warps  thread = one key and half of the rows.
 //
 // Measured (d 512, 64 heads, bf16): 16 tokens on 4 contexts of 32768 positions
-// 416 us, 660 TFLOP/s; 7 tokens on 8 contexts of up to 4100 39 us; one token on
-// 700 positions 13 us. With d 576, one token on 8 contexts of 32768 98 us. What
+// 420 us, 655 TFLOP/s; 7 tokens on 8 contexts of up to 4100 40 us; one token on
+// 700 positions 14 us. With d 576, one token on 8 contexts of 32768 99 us. What
 // bounds it is no unit but the hand-over between the roles: a tile of 64 rows
 // takes 6300 cycles, of which the MMAs need 2600, and leaving out all MMAs,
 // all exponentials or all loads shortens the call by 3, 0 and 5 %. Shared
@@ -324,7 +324,10 @@ __device__ __forceinline__ float across(const float (&x)[N], float none, int lan
 // shorter contexts and smaller trees leave over go to the others: key tiles a
 // block = the fewest for which all sequences' blocks fit in the grid. (Eight
 // contexts of up to 4100 positions, 7 drafted tokens: 72 us cut by the longest,
-// 42 so; equal contexts pay 0.4 us a block for it.)
+// 42 so; equal contexts pay 0.4 us a block for it.) Not where the host's plan
+// leaves contexts whole: 8 sequences of 16 tokens, 64 heads, under a longest
+// context of 32768 fill 128 blocks uncut, and take 787 us also when seven of the
+// contexts have 1000 positions, as the blocks of the eighth walk it alone.
 // Sequences are numbered through, a sequence's row tiles in turn, the splits
 // of a row tile side by side.
 constexpr int TA_STASH = 4096;              // sequences whose lengths fit in `len`; more keep the host's cut
@@ -1084,7 +1087,8 @@ long part_rows(int n_heads, int n_tok, int batch, int max_ctx)
 
 // The pair (rows of a tile, splits) of least time on 148 SMs, one block each,
 // by what a block costs: microseconds per tile and beside its tiles, measured
-// over 700 to 32768 positions. A tile's time hardly depends on its rows (the
+// over 700 to 32768 positions at d = 512 and, past it, 576 (a narrower row's
+// tiles take less, but the pairs compare much the same). A tile's time hardly depends on its rows (the
 // 128 keys are widened all the same), so many rows win once the blocks fill
 // the machine, and few rows before that. Past d = 512 a tile of 64 rows leaves
 // TMEM two pairs of keys and shared memory four of five: 5.2 us a tile, still

@@ -426,12 +426,13 @@ int dsv4b_kv_read(const dsv4b_kvq *c, void *out, int dt, long row_stride, const 
  * one token to the next, sequences n_tok tokens apart). Token t < n_draft[b]
  * of sequence b attends to its sequence's cached positions 0 .. ctx[b] - 1 and
  * to the drafted positions ctx[b] + k whose bit k is set in mask[b][t] (its
- * ancestors, and usually itself), whose rows have been written at those
- * positions; position j is row j % page_rows of page pages[b][j / page_rows]
- * (a page outside the cache is skipped; a cache holds less than 2^38 bytes of
- * codes). Keys and values are the same rows,
- * shared by all heads; o does not overlap q; sink[h] (may be NULL) joins the denominator only
- * (src/core/dsv4_attn.c:60-108); with nothing to attend to the output is
+ * ancestors, and usually itself). The rows of all these positions have been
+ * written, those of hidden ones too (a code that is NaN would pass a mask; no row
+ * that dsv4b_kv_write leaves has one). Position j is row j % page_rows of page
+ * pages[b][j / page_rows] (a page outside the cache is skipped; a cache holds
+ * less than 2^38 bytes of codes). Keys and values are the same rows, shared by
+ * all heads; o does not overlap q; sink[h] (may be NULL) joins the denominator
+ * only (src/core/dsv4_attn.c:60-108); with nothing to attend to the output is
  * zero. Tokens t >= n_draft[b] are not written (n_draft NULL: n_tok each).
  * Scores, the softmax's sums and the output are float until the output is
  * rounded; what a position adds to the output (its weight times its row's
@@ -449,10 +450,10 @@ int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long q_tok, cons
                     const unsigned long long *mask, const float *sink, int n_heads, int n_tok, int batch,
                     int max_ctx, float scale, void *scratch, size_t scratch_bytes, void *stream);
 
-/* 0 when every dsv4b_tree_attn on the current device since the last status
- * has run to its end; 1 when a block of one gave up a wait inside the kernel (each
+/* 0 when every dsv4b_tree_attn on the current device since the last status has
+ * run to its end; 1 when a block of one gave up a wait inside the kernel (each
  * is bounded by two seconds; that call's outputs are not valid), which this
- * call forgets; -1 without a device, or while a stream is being captured.
+ * call then forgets; -1 without a device, or while a stream is being captured.
  * Waits for the device. */
 int dsv4b_tree_attn_status(void);
 

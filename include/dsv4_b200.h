@@ -453,8 +453,8 @@ int dsv4b_tree_attn(void *o, const void *q, int dt, long o_tok, long q_tok, cons
 /* 0 when every dsv4b_tree_attn on the current device since the last status has
  * run to its end; 1 when a block of one gave up a wait inside the kernel (each
  * is bounded by two seconds; that call's outputs are not valid), which this
- * call then forgets; -1 without a device, or while a stream is being captured.
- * Waits for the device. */
+ * call then forgets; -1 without a device, or while a stream is being captured,
+ * which the call would spoil. Waits for the device. */
 int dsv4b_tree_attn_status(void);
 
 /* Such a wait, which nothing ends, in a kernel of its own: it runs out after
